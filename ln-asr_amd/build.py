@@ -25,7 +25,10 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "lnasr", "liblnasr_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
+# packed fp32 instructions stay off in device code (some of their forms have given wrong results on this part); the host pass
+# does not know the feature and says so
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = NO_PACKED_F32 + ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
          "-Wno-unused-variable", "-ffp-contract=on", "-I/opt/rocm/include"]
 
 
@@ -37,7 +40,7 @@ def _stale(target, deps):
 
 
 ASAN_LIB = os.path.join(HERE, "lnasr", "liblnasr_hip_asan.so")
-ASAN_FLAGS = ["--offload-arch=gfx950", "-O1", "-g", "-DLNASR_DEBUG_GUARDS", "-std=c++17", "-fPIC", "-fno-omit-frame-pointer",
+ASAN_FLAGS = NO_PACKED_F32 + ["--offload-arch=gfx950", "-O1", "-g", "-DLNASR_DEBUG_GUARDS", "-std=c++17", "-fPIC", "-fno-omit-frame-pointer",
               "-fsanitize=address,undefined", "-fno-gpu-sanitize", "-fno-sanitize-recover=undefined",
               "-Wno-unused-function", "-Wno-unused-variable", "-ffp-contract=on", "-I/opt/rocm/include"]
 
