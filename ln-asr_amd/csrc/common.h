@@ -157,7 +157,8 @@ struct ProfRec {
 
 struct lnasr_ctx {
     int device = 0;
-    hipStream_t stream = nullptr;
+    hipStream_t stream = nullptr;             // the stream of the context's calls: its own, or the caller's (lnasr_ctx_use_stream)
+    hipStream_t own_stream = nullptr;
     hipStream_t stream2 = nullptr;            // side stream: the backward pass runs beside the forward pass
     hipEvent_t ev_fork = nullptr, ev_join = nullptr;
     std::vector<hipEvent_t> copy_events;      // one per upload chunk of emit_batch
@@ -197,6 +198,11 @@ struct lnasr_ctx {
     int64_t* mfcc_meta = nullptr;                          // pinned: sample offsets [U+1] then frame offsets [U+1] of the call
     size_t mfcc_meta_cap = 0;                              // ... in elements
     hipEvent_t mfcc_meta_ev = nullptr;                     // the upload that last read mfcc_meta
+    // feature transforms (transform.hip): workspaces, grow-only.  Once a stream of this context has been captured into a graph,
+    // a buffer that has to grow is kept in `tr_retired` instead of being freed: a replay may still use it
+    lnasr::DevBuf tr_ws[18];
+    std::vector<void*> tr_retired;
+    bool tr_captured = false;
     // profiling
     bool prof_on = false;
     std::vector<std::string> prof_names;

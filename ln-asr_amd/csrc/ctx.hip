@@ -284,6 +284,7 @@ int lnasr_ctx_create(int device_id, lnasr_ctx** out) {
         return fail(LNASR_E_NODEVICE, "device %d is %s; this library is built for gfx950 only", device_id, arch.c_str());
     }
     LN_HIP(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));
+    ctx->own_stream = ctx->stream;
     LN_HIP(hipStreamCreateWithFlags(&ctx->stream2, hipStreamNonBlocking));
     LN_HIP(hipEventCreateWithFlags(&ctx->ev_fork, hipEventDisableTiming));
     LN_HIP(hipEventCreateWithFlags(&ctx->ev_join, hipEventDisableTiming));
@@ -298,6 +299,9 @@ int lnasr_ctx_create(int device_id, lnasr_ctx** out) {
 void lnasr_ctx_destroy(lnasr_ctx* ctx) {
     if (!ctx) return;
     (void)hipSetDevice(ctx->device);
+    // (a caller's stream may be gone by now: wait for the whole device instead)
+    if (ctx->stream != ctx->own_stream) (void)hipDeviceSynchronize();
+    ctx->stream = ctx->own_stream;
     (void)hipStreamSynchronize(ctx->stream);
     lnasr_comm_destroy(ctx);
     ctx->model.release();
@@ -305,6 +309,8 @@ void lnasr_ctx_destroy(lnasr_ctx* ctx) {
                      &ctx->ws_out3, &ctx->ws_b, &ctx->ws_bm, &ctx->ws_v, &ctx->ws_alpha, &ctx->ws_beta,
                      &ctx->ws_misc, &ctx->ws_misc2, &ctx->ws_lens, &ctx->ws_stats, &ctx->ws_p, &ctx->ws_q, &ctx->ws_raw, &ctx->ws_w1, &ctx->ws_w2, &ctx->ws_w3, &ctx->ws_pad, &ctx->ws_bp, &ctx->ws_btb, &ctx->ws_clock, &ctx->ws_fs, &ctx->ws_lvl, &ctx->ws_lvl2, &ctx->mfcc_const, &ctx->nan_flag, &ctx->nan_slots};
     for (DevBuf* b : all) b->release();
+    for (DevBuf& b : ctx->tr_ws) b.release();
+    for (void* p : ctx->tr_retired) (void)hipFree(p);
     for (auto& r : ctx->prof_recs) {
         (void)hipEventDestroy(r.e0);
         (void)hipEventDestroy(r.e1);
@@ -328,6 +334,25 @@ int lnasr_sync(lnasr_ctx* ctx) {
     LN_ENTER(ctx);
     LN_REQUIRE(ctx, "null ctx");
     LN_HIP(hipStreamSynchronize(ctx->stream));
+    return 0;
+}
+
+int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own) {
+    LN_ENTER(ctx);
+    LN_REQUIRE(ctx, "null ctx");
+    const hipStream_t to = own ? ctx->own_stream : (hipStream_t)stream;
+    if (to == ctx->stream) return 0;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    for (hipStream_t s : {ctx->stream, to}) {
+        if (hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+            (void)hipGetLastError();
+            return fail(LNASR_E_INVALID, "a stream is being captured: choose the context's stream before the capture begins");
+        }
+    }
+    // what was enqueued so far comes first: the context's workspaces are shared by both streams
+    LN_HIP(hipEventRecord(ctx->ev_fork, ctx->stream));
+    LN_HIP(hipStreamWaitEvent(to, ctx->ev_fork, 0));
+    ctx->stream = to;
     return 0;
 }
 

@@ -1,0 +1,175 @@
+// Feature transforms: affine maps per group of rows, and a shared projection with low-rank adapters (transform.hip: entry
+// points and dispatch; transform_rows.hip: products with one result row per feature row; transform_grad.hip: products that
+// sum over rows).  Internal.
+#pragma once
+#include "common.h"
+
+namespace lnasr {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// One 16 x 16 block of a product by the matrix cores.  Every type moves in pieces of 16 bytes: lane l of the wave holds, for
+// row (l & 15) of its operand, the E consecutive k of piece (l >> 4) of a 64-byte run.  Which k an instruction contracts is
+// free as long as both operands agree, so the piece feeds E / 8 (16 bit), 4 (f32) or 2 (f64) instructions as it lies.
+// D[m, n]: lane l holds column n = l & 15 and the four rows m = row(r, l >> 4).
+template <typename T>
+struct Mat;
+template <>
+struct Mat<double> {
+    using Acc = f64x4;
+    using Sum = double;
+    static constexpr int E = 2;
+    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+        const f64x2 x = __builtin_bit_cast(f64x2, a), y = __builtin_bit_cast(f64x2, b);
+        c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[0], y[0], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f64_16x16x4f64(x[1], y[1], c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ int row(int r, int kk) { return 4 * r + kk; }
+};
+template <>
+struct Mat<float> {
+    using Acc = f32x4;
+    using Sum = float;
+    static constexpr int E = 4;
+    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
+};
+template <>
+struct Mat<_Float16> {
+    using Acc = f32x4;
+    using Sum = float;
+    static constexpr int E = 8;
+    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
+};
+template <>
+struct Mat<__bf16> {
+    using Acc = f32x4;
+    using Sum = float;
+    static constexpr int E = 8;
+    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
+};
+
+// Segments of rows.  offsets may come from device memory that the host has not looked at: every value is brought into
+// [0, rows] before it is used, so that an offset out of order gives meaningless numbers but no access out of range.
+struct Segments {
+    const int64_t* off;      // [S + 1]
+    const int32_t* slots;    // [S] or null: segment s belongs to group s
+    int S, G;
+    int64_t rows;
+};
+__device__ __forceinline__ int64_t seg_off(const Segments& sg, int s) {
+    const int64_t o = sg.off[s];
+    return o < 0 ? 0 : o > sg.rows ? sg.rows : o;
+}
+// group of segment s, or -1
+__device__ __forceinline__ int seg_slot(const Segments& sg, int s) {
+    const int k = sg.slots ? sg.slots[s] : s;
+    return (unsigned)k < (unsigned)sg.G ? k : -1;
+}
+// The last i in [0, n) with first(i) <= t, -1 if there is none; first must not fall.  The 64 lanes of a wave probe 64 candidates
+// at a time: two rounds for 4096 segments.
+template <typename F>
+__device__ __forceinline__ int wave_search(int n, int64_t t, F first) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    while (true) {
+        const int step = (n + 63) / 64;
+        const int64_t at = (int64_t)lane * step;
+        const bool below = at < n && first(lo + (int)at) <= t;
+        const int cnt = __popcll(__ballot(below));
+        if (cnt == 0) return -1;
+        const int skip = (cnt - 1) * step;
+        lo += skip;
+        n = min(step, n - skip);
+        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+    }
+}
+// The spans of 2^ts rows of a ragged batch, without a table: give segment s the numbers floor(off[s] / 2^ts) + s and on.  They
+// never collide (a segment of n rows needs ceil(n / 2^ts) numbers and has at least floor(n / 2^ts) + 1), so floor(rows / 2^ts)
+// + S numbers cover every batch; some of them are empty spans.  Returns the segment of span t and its rows r0 .. r1 - 1
+// (wave-uniform), -1 if the span is empty.
+__device__ __forceinline__ int find_span(const int64_t* off, int S, int64_t rows, int64_t t, int ts, int64_t* r0, int64_t* r1) {
+    auto clamped = [&](int s) {
+        const int64_t o = off[s];
+        return o < 0 ? (int64_t)0 : o > rows ? rows : o;
+    };
+    const int s = wave_search(S, t, [&](int i) { return (clamped(i) >> ts) + i; });
+    if (s < 0) return -1;
+    const int64_t o = clamped(s), e = clamped(s + 1);
+    *r0 = o + ((t - ((o >> ts) + s)) << ts);
+    *r1 = *r0 + (1ll << ts) < e ? *r0 + (1ll << ts) : e;
+    return *r0 < *r1 ? s : -1;
+}
+
+// 16 bytes of E consecutive elements from element c of a line that ends before `end`; what lies past the end is 0.  The
+// address need not be aligned (odd widths: rows of 39 or 351 values).
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* line, long c, long end) {
+    constexpr int E = Mat<T>::E;
+    u32x4 v;
+    if (c + E <= end) {
+        __builtin_memcpy(&v, line + c, 16);
+        return v;
+    }
+    T e[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) e[j] = c + j < end ? line[c + j] : (T)0;
+    __builtin_memcpy(&v, e, 16);
+    return v;
+}
+
+// y[r, :] = scale_k * (x[r, :] W_k') + bias_k  for the rows of the segments; W_k' = W_k^T (kn false, W_k [n, k]) or W_k (kn
+// true, W_k [k, n]).  w_stride 0: one W for all rows, tiles of rows then run across segments; with `low` each row also gets
+// p[r, :] L_k' of its segment's group (none where the group is negative).
+struct RowsArgs {
+    Segments sg;
+    const void *x, *w, *bias, *p, *low;
+    const double* scale;
+    void* y;
+    int64_t ldx, ldy, ldp;
+    int64_t w_stride, bias_stride, low_stride;
+    int K, N, R;
+    bool kn;
+};
+int transform_rows(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name);
+
+// out[k, i, j] = sum over the rows r of group k of a[r, i] b[r, j];  cols[k, i] = sum of a[r, i] (or null).  Every group is
+// written, zeros where it has no rows.
+struct SumArgs {
+    Segments sg;
+    const int64_t* group_off;   // group g: places group_off[g * group_step] .. group_off[(g + 1) * group_step] of `rowmap`
+    int64_t group_step;         // 1; S: all segments as one group
+    const int64_t* rowmap;      // row at each place of the sorted order, or null: the rows as they lie
+    const void *a, *b;
+    void *out, *cols;
+    int64_t lda, ldb;
+    int groups, I, J;
+};
+int transform_sum(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
+// Sorts the segments by group (stable): *group_off [G + 1], *rowmap [rows].  Without slots both are the segments' own.
+int transform_sort(lnasr_ctx* ctx, const Segments& sg, const int64_t** group_off, const int64_t** rowmap);
+
+// Workspace `i` of the feature transforms with room for `bytes`
+int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out);
+enum { kTrX, kTrOff, kTrSlots, kTrW, kTrBias, kTrA, kTrB, kTrScale, kTrDy, kTrOut0, kTrOut1, kTrOut2, kTrOut3, kTrOut4, kTrLow, kTrDlow,
+       kTrSort, kTrPart, kTrCount };
+
+inline size_t transform_size(int dtype) { return dtype == LNASR_F64 ? 8 : dtype == LNASR_F32 ? 4 : 2; }
+
+}  // namespace lnasr

@@ -9,7 +9,7 @@ import threading
 
 import numpy as np
 
-F64, F32 = 0, 1
+F64, F32, F16, BF16 = 0, 1, 2, 3
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # LNASR_LIB selects another build of the same library (the host-sanitizer build of build.py --host-asan)
 _LIB_PATH = os.environ.get("LNASR_LIB") or os.path.join(_HERE, "liblnasr_hip.so")
@@ -36,6 +36,7 @@ SIGNATURES = {
     "lnasr_ctx_create": [_i, _P(_vp)],
     "lnasr_ctx_destroy": [_vp],
     "lnasr_sync": [_vp],
+    "lnasr_ctx_use_stream": [_vp, _vp, _i],
     "lnasr_device_sync": [_vp],
     "lnasr_reload_switches": [],
     "lnasr_host_alloc": [_vp, _sz, _P(_vp)],
@@ -86,6 +87,11 @@ SIGNATURES = {
     "lnasr_split_frames": [_vp, _vp, _i64, _i, _i, _vp],
     "lnasr_mfcc": [_vp, _vp, _i, _vp, _i, _P(MfccCfgStruct), _vp, _vp, _vp, _vp, _vp],
     "lnasr_pad_rows": [_vp, _vp, _vp, _i, _i, _i64, _vp],
+    "lnasr_affine": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i64],
+    "lnasr_affine_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _vp],
+    "lnasr_projection": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64],
+    "lnasr_projection_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64,
+                              _vp, _vp, _vp, _vp],
     "lnasr_comm_unique_id": [_vp],
     "lnasr_comm_init": [_vp, _vp, _i, _i],
     "lnasr_comm_destroy": [_vp],
@@ -270,6 +276,79 @@ def _in(x, dtype):
     return np.ascontiguousarray(x, dtype=dtype)
 
 
+# dtype codes of the feature transforms
+_CODES = {"float64": F64, "float32": F32, "float16": F16, "bfloat16": BF16}
+
+
+class _Arg:
+    """An array handed to a feature transform: a numpy array (or what becomes one), a DeviceArray, or a tensor of another library
+    on the GPU (an object with data_ptr(), shape, dtype, stride() and is_cuda, as torch's).  `obj` keeps it alive."""
+    __slots__ = ("ptr", "shape", "ld", "kind", "obj")
+
+    def __init__(self, ctx, x, name, ndim, like=None, out=False):
+        """like: the _Arg whose type this one must have (None: any of the four; a kind: exactly that)."""
+        if isinstance(x, DeviceArray):
+            if not x.ptr or x.ctx.device != ctx.device:
+                raise LnasrError("%s: a DeviceArray that was freed, or of another device" % name)
+            self.obj, self.ptr, self.shape, self.kind = x, x.ptr, x.shape, x.dtype.name
+            self.ld = x.shape[-1] if ndim > 1 and len(x.shape) == ndim else 1
+        elif getattr(x, "is_cuda", False):
+            if x.get_device() != ctx.device:
+                raise LnasrError("%s lies on device %d, the context on device %d" % (name, x.get_device(), ctx.device))
+            self.obj, self.ptr, self.shape, self.kind = x, x.data_ptr(), tuple(x.shape), str(x.dtype).replace("torch.", "")
+            self.ld = 1
+            if not ctx._tensors_checked:
+                # pointers of another copy of the HIP runtime mean nothing to this one
+                if self.ptr and lib().lnasr_debug_require_device_ptr(self.ptr) != 0:
+                    raise LnasrError("%s: GPU memory this process's HIP runtime does not know: import the library it comes from "
+                                     "before lnasr makes its first call" % name)
+                ctx._tensors_checked = bool(self.ptr)
+            if len(self.shape) == ndim:
+                if ndim == 2:
+                    st = x.stride()
+                    self.ld = st[0] if self.shape[0] > 1 else self.shape[1]
+                    if (self.shape[1] > 1 and st[1] != 1) or self.ld < self.shape[1]:
+                        raise LnasrError("%s: rows must be contiguous, got strides %s" % (name, tuple(st)))
+                elif not x.is_contiguous():
+                    raise LnasrError("%s must be contiguous" % name)
+        else:
+            if out:
+                if not isinstance(x, np.ndarray) or not x.flags.c_contiguous or not x.flags.writeable:
+                    raise LnasrError("%s must be a writable C-contiguous numpy array, a DeviceArray or a tensor" % name)
+            else:
+                x = np.asarray(x)
+                if isinstance(like, str):
+                    x = np.ascontiguousarray(x, dtype=like)
+                else:
+                    kind = like.kind if like is not None and like.kind != "bfloat16" else x.dtype.name
+                    x = np.ascontiguousarray(x, dtype=kind if kind in _CODES else np.float64)
+            self.obj, self.ptr, self.shape, self.kind = x, x.ctypes.data, x.shape, x.dtype.name
+            self.ld = x.shape[-1] if ndim > 1 and x.ndim == ndim else 1
+        if len(self.shape) != ndim:
+            raise ValueError("%s must have %d dimensions, got shape %s" % (name, ndim, tuple(self.shape)))
+        want = like if isinstance(like, str) else like.kind if like is not None else None
+        if want is not None and self.kind != want:
+            raise LnasrError("%s is %s, expected %s" % (name, self.kind, want))
+        if want is None and self.kind not in _CODES:
+            raise LnasrError("%s is %s: feature transforms take float64, float32, float16 and bfloat16" % (name, self.kind))
+
+    def empty(self, ctx, shape, zero):
+        """A new array of this one's library, device and type."""
+        if isinstance(self.obj, DeviceArray):
+            d = DeviceArray(ctx, shape, self.obj.dtype)
+            if zero:
+                check(lib().lnasr_memset(ctx.handle, d.ptr, 0, d.nbytes))
+            return d
+        if isinstance(self.obj, np.ndarray):
+            return np.zeros(shape, dtype=self.obj.dtype)
+        return self.obj.new_zeros(shape) if zero else self.obj.new_empty(shape)
+
+
+def _need(arg, name, shape):
+    if tuple(arg.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(arg.shape)))
+
+
 class Context:
     """One process = one GPU = one Context (one HIP stream)."""
 
@@ -297,6 +376,8 @@ class Context:
         self.model_owner = None       # (id(obj), version) of the model currently uploaded
         self.model_shape = None       # (N, M, D) or (N,)
         self._model_fp = None         # fingerprint of the parameters the device holds (see upload_*)
+        self._tensors_checked = False # a tensor of another library was seen and its memory is known to this HIP runtime
+        self._stream = None           # the caller's stream this context works on (None: its own)
 
     def close(self):
         if self.handle:
@@ -312,6 +393,16 @@ class Context:
     # -- runtime -----------------------------------------------------------------------
     def sync(self):
         check(lib().lnasr_sync(self.handle))
+
+    def use_stream(self, stream=None):
+        """Send this context's further calls to `stream` (a hipStream_t as an int, or an object with `cuda_stream`, as torch's
+        streams have), behind what it was given so far; None: back to its own.  Tensors of another library are produced on a
+        stream of that library: choose that stream here (lnasr_ctx_use_stream)."""
+        if stream is not None and not isinstance(stream, int):
+            stream = stream.cuda_stream
+        if stream != self._stream:
+            check(lib().lnasr_ctx_use_stream(self.handle, stream, 1 if stream is None else 0))
+            self._stream = stream
 
     def device_sync(self):
         """hipDeviceSynchronize on this context's device (every stream drained): the bracket of a timed region."""
@@ -819,6 +910,109 @@ class Context:
         out = self._out(isinstance(packed, DeviceArray), (U, int(pad_rows), W), np.float64)
         check(lib().lnasr_pad_rows(self.handle, _ptr(packed), _ptr(row_offsets), U, W, int(pad_rows), _ptr(out)))
         return out, lens
+
+    # -- feature transforms ------------------------------------------------------------------------
+    # (lnasr/transform.py has what the arguments mean)
+    def _rows(self, x, offsets, slots, groups):
+        """(_Args of x, offsets, slots, number of segments, whether every row is known to belong to a segment)."""
+        x = _Arg(self, x, "x", 2)
+        off = _Arg(self, offsets, "offsets", 1, like="int64")
+        S = off.shape[0] - 1
+        if S < 0:
+            raise ValueError("offsets must hold at least one value")
+        sl = None
+        if slots is not None:
+            sl = _Arg(self, slots, "slots", 1, like="int32")
+            _need(sl, "slots", (S,))
+        elif S != groups:
+            raise ValueError("%d segments of %d groups: without slots there is one segment for each group" % (S, groups))
+        known = isinstance(off.obj, np.ndarray) and (sl is None or isinstance(sl.obj, np.ndarray))
+        return x, off, sl, S, known and off.obj[0] == 0 and off.obj[-1] == x.shape[0]
+
+    def affine(self, x, offsets, w, bias=None, slots=None, out=None):
+        x, off, sl, S, covered = self._rows(x, offsets, slots, w.shape[0])
+        w = _Arg(self, w, "w", 3, like=x)
+        G, O, I = w.shape
+        _need(x, "x", (x.shape[0], I))
+        if bias is not None:
+            bias = _Arg(self, bias, "bias", 2, like=x)
+            _need(bias, "bias", (G, O))
+            if bias.ld != O:
+                raise LnasrError("bias must be contiguous")
+        y = out if out is not None else x.empty(self, (x.shape[0], O), not covered)
+        ya = _Arg(self, y, "out", 2, like=x, out=True)
+        _need(ya, "out", (x.shape[0], O))
+        check(lib().lnasr_affine(self.handle, _CODES[x.kind], x.ptr, x.shape[0], I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr,
+                                 bias and bias.ptr, G, O, ya.ptr, ya.ld))
+        return y
+
+    def _grads(self, x, shapes, want, out, covered):
+        """The arrays that gradients go to: `out` (a dict: exactly those), or new ones for the names in `want`."""
+        given = out is not None
+        names = tuple(out) if given else tuple(want)
+        for k in names:
+            if k not in shapes:
+                raise ValueError("no gradient of %r: choose from %s" % (k, ", ".join(shapes)))
+        res = {k: out[k] if given else x.empty(self, shapes[k], k == "x" and not covered) for k in names}
+        args = {k: _Arg(self, v, "out[%r]" % k, len(shapes[k]), like=x, out=True) for k, v in res.items()}
+        for k, a in args.items():
+            _need(a, "out[%r]" % k, shapes[k])
+            if k != "x" and len(a.shape) == 2 and a.ld != a.shape[1]:
+                raise LnasrError("out[%r] must be contiguous" % k)
+        return res, (lambda k: args[k].ptr if k in args else None), (args["x"].ld if "x" in args else 0)
+
+    def affine_grad(self, x, offsets, w, dy, slots=None, want=("x", "w", "bias"), out=None):
+        x, off, sl, S, covered = self._rows(x, offsets, slots, w.shape[0])
+        w = _Arg(self, w, "w", 3, like=x)
+        G, O, I = w.shape
+        F = x.shape[0]
+        _need(x, "x", (F, I))
+        dy = _Arg(self, dy, "dy", 2, like=x)
+        _need(dy, "dy", (F, O))
+        res, ptr, lddx = self._grads(x, {"x": (F, I), "w": (G, O, I), "bias": (G, O)}, want, out, covered)
+        check(lib().lnasr_affine_grad(self.handle, _CODES[x.kind], x.ptr, F, I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr, G, O,
+                                      dy.ptr, dy.ld, ptr("x"), lddx, ptr("w"), ptr("bias")))
+        return res
+
+    def _adapters(self, x, w, a, b, scale):
+        w = _Arg(self, w, "w", 2, like=x)
+        O, I = w.shape
+        if w.ld != I:
+            raise LnasrError("w must be contiguous")
+        _need(x, "x", (x.shape[0], I))
+        a, b = _Arg(self, a, "a", 3, like=x), _Arg(self, b, "b", 3, like=x)
+        G, R = a.shape[:2]
+        _need(a, "a", (G, R, I))
+        _need(b, "b", (G, O, R))
+        if scale is not None:
+            scale = _Arg(self, scale, "scale", 1, like="float64")
+            _need(scale, "scale", (G,))
+        return w, a, b, scale, I, O, G, R
+
+    def projection(self, x, offsets, w, a, b, bias=None, scale=None, slots=None, out=None):
+        x, off, sl, S, covered = self._rows(x, offsets, slots, a.shape[0])
+        w, a, b, scale, I, O, G, R = self._adapters(x, w, a, b, scale)
+        if bias is not None:
+            bias = _Arg(self, bias, "bias", 1, like=x)
+            _need(bias, "bias", (O,))
+        y = out if out is not None else x.empty(self, (x.shape[0], O), not covered)
+        ya = _Arg(self, y, "out", 2, like=x, out=True)
+        _need(ya, "out", (x.shape[0], O))
+        check(lib().lnasr_projection(self.handle, _CODES[x.kind], x.ptr, x.shape[0], I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr,
+                                     bias and bias.ptr, O, a.ptr, b.ptr, scale and scale.ptr, G, R, ya.ptr, ya.ld))
+        return y
+
+    def projection_grad(self, x, offsets, w, a, b, dy, scale=None, slots=None, want=("x", "a", "b", "w", "bias"), out=None):
+        x, off, sl, S, covered = self._rows(x, offsets, slots, a.shape[0])
+        w, a, b, scale, I, O, G, R = self._adapters(x, w, a, b, scale)
+        F = x.shape[0]
+        dy = _Arg(self, dy, "dy", 2, like=x)
+        _need(dy, "dy", (F, O))
+        res, ptr, lddx = self._grads(x, {"x": (F, I), "a": (G, R, I), "b": (G, O, R), "w": (O, I), "bias": (O,)}, want, out, covered)
+        check(lib().lnasr_projection_grad(self.handle, _CODES[x.kind], x.ptr, F, I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr, O, a.ptr,
+                                          b.ptr, scale and scale.ptr, G, R, dy.ptr, dy.ld, ptr("x"), lddx, ptr("a"), ptr("b"),
+                                          ptr("w"), ptr("bias")))
+        return res
 
     # -- multi-GPU ---------------------------------------------------------------------------------
     def comm_init(self, unique_id, rank, nranks):
