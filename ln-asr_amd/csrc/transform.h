@@ -134,6 +134,57 @@ __device__ __forceinline__ u32x4 load_piece(const T* line, long c, long end) {
     return v;
 }
 
+// Consecutive block numbers go to the eight dies (XCDs) in turn, each with an L2 of its own: give every die a run of
+// neighbouring tiles, so that the tiles that share a matrix or a span of rows share an L2.
+__device__ __forceinline__ unsigned die_order(unsigned id, unsigned total) {
+    const unsigned per = total / 8, rest = total % 8, die = id % 8, at = id / 8;
+    return die * per + min(die, rest) + at;
+}
+
+// 16 bytes a lane from base + offset to LDS at `to` (wave-uniform) + 16 * lane; zeros where offset >= 2^31
+__device__ __forceinline__ void bring_piece(const char* base, unsigned offset, char* to) {
+    const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x80000000u, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
+}
+
+// A tile of C columns whose k is strided, in LDS as lines of k: the run of 16 columns (sizeof(T) pieces) at place p of line k
+// is run p ^ spread(k), so that the lines one fragment read touches (they differ in (lane & 15) >> 2 and lane >> 4 for 16 bit,
+// in lane >> 4 alone for the others) lie in other banks.
+template <typename T, int C>
+__device__ __forceinline__ int spread(int k) {
+    constexpr int RUNS = C / 16;
+    if (sizeof(T) == 2) return ((k & 3) | (k >> 1 & 4)) & (RUNS < 8 ? RUNS - 1 : 7);
+    if (sizeof(T) == 4) return k >> 2 & (RUNS < 4 ? RUNS - 1 : 3);
+    return k >> 1 & (RUNS < 2 ? RUNS - 1 : 1);
+}
+// the wave's fragment of columns c .. c + 15 (c a multiple of 16), half h of the 128 bytes of k
+template <typename T, int C>
+__device__ __forceinline__ u32x4 strided_fragment(const char* tile, int h, int c) {
+    constexpr int SZ = (int)sizeof(T), E = Mat<T>::E;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
+    u32x4 f;
+    if constexpr (SZ == 2) {
+        // each 16 lanes read 4 lines of 16 columns, 8 bytes a lane; the lane gets the 4 k of its column
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds16x4;
+        const int k = 32 * h + 8 * kk + (l15 >> 2);
+        const char* at = tile + k * (C * 2) + (((c / 16) ^ spread<T, C>(k)) << 5) + (l15 & 3) * 8;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(at + 4 * (C * 2)));    // spread(k + 4) == spread(k)
+        __builtin_memcpy(&f, &lo, 8);
+        __builtin_memcpy((char*)&f + 8, &hi, 8);
+    } else {
+        T e[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int k = (4 * h + kk) * E + j;
+            e[j] = *(const T*)(tile + k * (C * SZ) + (((c / 16) ^ spread<T, C>(k)) * 16 + l15) * SZ);
+        }
+        __builtin_memcpy(&f, e, 16);
+    }
+    return f;
+}
+
 // y[r, :] = scale_k * (x[r, :] W_k') + bias_k  for the rows of the segments; W_k' = W_k^T (kn false, W_k [n, k]) or W_k (kn
 // true, W_k [k, n]).  w_stride 0: one W for all rows, tiles of rows then run across segments; with `low` each row also gets
 // p[r, :] L_k' of its segment's group (none where the group is negative).
@@ -162,6 +213,13 @@ struct SumArgs {
     int groups, I, J;
 };
 int transform_sum(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
+// transform_narrow.hip: the same for contiguous rows of up to 64 values
+bool rows_narrow_ok(const RowsArgs& a);
+int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name);
+bool sum_narrow_ok(const SumArgs& a);
+int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
+// out and cols from the sums of the spans of 2^ts rows
+int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const void* parts, const void* col_parts);
 // Sorts the segments by group (stable): *group_off [G + 1], *rowmap [rows].  Without slots both are the segments' own.
 int transform_sort(lnasr_ctx* ctx, const Segments& sg, const int64_t** group_off, const int64_t** rowmap);
 

@@ -1,0 +1,368 @@
+// Feature transforms of up to 64 values a row: MFCC frames (39), spliced and reduced features (40), their gradients.  Such a
+// product is bound by the memory it moves (39 x 39 in fp64: 5 operations a byte), so rows are read and written as the contiguous
+// bytes they are, whatever their width, and the matrix stays in registers.
+#include <algorithm>
+#include <type_traits>
+
+#include "transform.h"
+
+namespace lnasr {
+
+// LDS of one wave is its own: order its writes and reads for the compiler (the hardware keeps the order of a wave's LDS accesses)
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The bytes [0, bytes) from src to the wave's LDS by 16 a lane; HF * 1024 at least `bytes`.  `room` bytes of src may be read.
+template <typename T, int HF>
+struct Chunk {
+    u32x4 v[HF];
+    __device__ __forceinline__ void load(const char* src, int bytes, int64_t room) {
+        const int lane = threadIdx.x & 63;
+        if (room >= (int64_t)((bytes + 15) & ~15)) {
+#pragma unroll
+            for (int i = 0; i < HF; ++i)
+                if ((i * 64 + lane) * 16 < bytes) __builtin_memcpy(&v[i], src + (i * 64 + lane) * 16, 16);
+        } else {                                           // the end of the array
+#pragma unroll
+            for (int i = 0; i < HF; ++i) {
+                const int64_t at = (i * 64 + lane) * 16;
+                v[i] = load_piece((const T*)src, at / (int)sizeof(T), room > 0 ? room / (int)sizeof(T) : 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* lds, int bytes) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < HF; ++i)
+            if ((i * 64 + lane) * 16 < bytes) *(u32x4*)(lds + (i * 64 + lane) * 16) = v[i];
+    }
+};
+
+// ------------------------------------------------------------------------------------------
+// y[r] = scale (W x[r]) + bias: the four waves of a block share a span of rows, each takes 16 at a time.  The next 16 rows are on
+// their way while the current ones multiply.  N <= 16 NF, K sizeof(T) <= 64 HF.
+// ------------------------------------------------------------------------------------------
+template <typename T, int NF, int HF>
+__global__ __launch_bounds__(256) void rows_narrow(RowsArgs a, int ts, int wave_lds) {
+    using M = Mat<T>;
+    using Sum = typename M::Sum;
+    constexpr int SZ = (int)sizeof(T), E = M::E;
+    extern __shared__ __attribute__((aligned(16))) char lds_all[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
+    char* lds = lds_all + wave * wave_lds;
+    int64_t r0, r1;
+    const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, die_order(blockIdx.x, gridDim.x), ts, &r0, &r1);
+    if (s < 0) return;
+    const int slot = seg_slot(a.sg, s);
+    if (slot < 0) return;
+    r0 += wave * 16;
+    if (r0 >= r1) return;
+
+    const int in_bytes = 16 * a.K * SZ, K = a.K, N = a.N;
+    Chunk<T, HF> next;
+    next.load((const char*)a.x + r0 * K * SZ, in_bytes, (a.sg.rows - r0) * K * SZ);
+
+    const T* w = (const T*)a.w + slot * a.w_stride;
+    u32x4 wf[NF][HF];
+#pragma unroll
+    for (int n = 0; n < NF; ++n) {
+        const int c = min(16 * n + l15, N - 1);
+#pragma unroll
+        for (int h = 0; h < HF; ++h) {
+            const int k = (4 * h + kk) * E;
+            if (a.kn) {
+                T e[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = k + j < K ? w[(k + j) * N + c] : (T)0;
+                __builtin_memcpy(&wf[n][h], e, 16);
+            } else {
+                wf[n][h] = load_piece(w + c * K, k, K);
+            }
+        }
+    }
+    Sum bv[NF][4];
+    const T* bias = a.bias ? (const T*)a.bias + slot * a.bias_stride : nullptr;
+#pragma unroll
+    for (int n = 0; n < NF; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int c = 16 * n + M::row(r, kk);
+            bv[n][r] = bias && c < N ? (Sum)bias[c] : (Sum)0;
+        }
+    const Sum scale = a.scale ? (Sum)a.scale[slot] : (Sum)1;
+
+    for (; r0 < r1; r0 += 64) {
+        next.store(lds, in_bytes);
+        wave_lds_order();
+        u32x4 xf[HF];
+#pragma unroll
+        for (int h = 0; h < HF; ++h) {
+            const int k = (4 * h + kk) * E;
+            if ((4 * h + 4) * E <= K) {                    // (the same for every lane)
+                __builtin_memcpy(&xf[h], lds + (l15 * K + k) * SZ, 16);
+            } else {
+                T e[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = k + j < K ? *(const T*)(lds + (l15 * K + k + j) * SZ) : (T)0;
+                __builtin_memcpy(&xf[h], e, 16);
+            }
+        }
+        wave_lds_order();
+        if (r0 + 64 < r1) next.load((const char*)a.x + (r0 + 64) * K * SZ, in_bytes, (a.sg.rows - r0 - 64) * K * SZ);
+#pragma unroll
+        for (int n = 0; n < NF; ++n) {
+            typename M::Acc acc = typename M::Acc{0, 0, 0, 0};
+#pragma unroll
+            for (int h = 0; h < HF; ++h) acc = M::mma(wf[n][h], xf[h], acc);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int c = 16 * n + M::row(r, kk);
+                if (c < N) *(T*)(lds + (l15 * N + c) * SZ) = (T)(acc[r] * scale + bv[n][r]);      // the one rounding of the result
+            }
+        }
+        wave_lds_order();
+        const int out_bytes = (int)min(r1 - r0, (int64_t)16) * N * SZ;
+        char* y = (char*)a.y + r0 * N * SZ;
+        for (int at = lane * 16; at < out_bytes; at += 1024) {
+            if (at + 16 <= out_bytes) {
+                const u32x4 v = *(const u32x4*)(lds + at);
+                __builtin_memcpy(y + at, &v, 16);
+            } else {
+                for (int b = at; b < out_bytes; b += SZ) *(T*)(y + b) = *(const T*)(lds + b);
+            }
+        }
+        wave_lds_order();
+    }
+}
+
+template <typename T, int NF, int HF>
+static int launch_narrow(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
+    // spans: long ones spread the cost of fetching the matrix, but every CU should have a few blocks
+    int ts = 6;
+    while (ts < 10 && (a.sg.rows >> ts) > 8 * ctx->prop.multiProcessorCount) ++ts;
+    const int64_t spans = (a.sg.rows >> ts) + a.sg.S;
+    LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d segments are too many for one call", (long long)a.sg.rows, a.sg.S);
+    const int wave_lds = (16 * std::max(a.K, a.N) * (int)sizeof(T) + 15) / 16 * 16;
+    LN_LAUNCH(ctx, name, (rows_narrow<T, NF, HF>), dim3((unsigned)spans), dim3(256), 4 * wave_lds, a, ts, wave_lds);
+    return 0;
+}
+
+template <typename T, int HF>
+static int narrow_n(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
+    if (a.N <= 16) return launch_narrow<T, 1, HF>(ctx, a, name);
+    if (a.N <= 48) return launch_narrow<T, 3, HF>(ctx, a, name);
+    return launch_narrow<T, 4, HF>(ctx, a, name);
+}
+
+template <typename T>
+static int narrow_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
+    const int bytes = a.K * (int)sizeof(T);
+    if constexpr (sizeof(T) == 8) {
+        if (bytes <= 128) return narrow_n<T, 2>(ctx, a, name);
+        if (bytes <= 320) return narrow_n<T, 5>(ctx, a, name);
+        return narrow_n<T, 8>(ctx, a, name);
+    } else if constexpr (sizeof(T) == 4) {
+        if (bytes <= 64) return narrow_n<T, 1>(ctx, a, name);
+        if (bytes <= 192) return narrow_n<T, 3>(ctx, a, name);
+        return narrow_n<T, 4>(ctx, a, name);
+    } else {
+        if (bytes <= 64) return narrow_n<T, 1>(ctx, a, name);
+        return narrow_n<T, 2>(ctx, a, name);
+    }
+}
+
+bool rows_narrow_ok(const RowsArgs& a) {
+    return a.w_stride && a.K <= 64 && a.N <= 64 && a.ldx == a.K && a.ldy == a.N;
+}
+
+int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name) {
+    switch (dtype) {
+        case LNASR_F64: return narrow_t<double>(ctx, a, name);
+        case LNASR_F32: return narrow_t<float>(ctx, a, name);
+        case LNASR_F16: return narrow_t<_Float16>(ctx, a, name);
+        default: return narrow_t<__bf16>(ctx, a, name);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// out = sum over the rows of a span of a[r]^T b[r], up to 64 x 64: each of the four waves sums its own chunks of R rows (the k of
+// one matrix instruction's piece, or two), whole, and the block adds the four at the end.  The column sums of a come with the
+// product: b has a column of ones behind its last.
+// ------------------------------------------------------------------------------------------
+template <typename T, int IF, int JF, int HA, int HB>
+__global__ __launch_bounds__(256) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts, typename Mat<T>::Sum* col_parts, int wave_lds) {
+    using M = Mat<T>;
+    using Sum = typename M::Sum;
+    constexpr int SZ = (int)sizeof(T), E = M::E, R = SZ == 2 ? 32 : 16, H = R / (4 * E);
+    extern __shared__ __attribute__((aligned(16))) char lds_all[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
+    const int I = a.I, J = a.J, a_bytes = R * I * SZ, b_bytes = R * J * SZ;
+    char* as = lds_all + wave * wave_lds;
+    char* bs = as + (a_bytes + 15) / 16 * 16;
+    const int64_t t = die_order(blockIdx.x, gridDim.x);
+    auto clamped = [&](int g) {
+        const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
+        return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
+    };
+    const int g = wave_search(a.groups, t, [&](int i) { return (clamped(i) >> ts) + i; });
+    if (g < 0) return;
+    const int64_t go = clamped(g), ge = max(go, clamped(g + 1)), span = t - ((go >> ts) + g), q0 = go + (span << ts);
+    if (span > 0 && q0 >= ge) return;
+    const int n = (int)min(ge - q0, (int64_t)1 << ts);
+    const bool whole = go + (1ll << ts) >= ge;
+
+    typename M::Acc acc[IF][JF];
+#pragma unroll
+    for (int i = 0; i < IF; ++i)
+#pragma unroll
+        for (int j = 0; j < JF; ++j) acc[i][j] = typename M::Acc{0, 0, 0, 0};
+
+    Chunk<T, HA> an;
+    Chunk<T, HB> bn;
+    // R rows from place k of the span that lie together, or -1: (wave-uniform)
+    auto run_at = [&](int k) -> int64_t {
+        if (k + R > n) return -1;
+        if (!a.rowmap) return q0 + k;
+        const int64_t lo = a.rowmap[q0 + k], hi = a.rowmap[q0 + k + R - 1];
+        // (a run may wrap out of and back into a segment's rows only if it holds them all in order: the map is a permutation
+        // that keeps the order within a segment, so equal distance alone is not enough -- every lane checks its row)
+        const int64_t mine = a.rowmap[q0 + k + (lane & (R - 1))];
+        const bool fits = hi - lo == R - 1 && mine == lo + (lane & (R - 1));
+        return __all(fits) ? lo : (int64_t)-1;
+    };
+    auto fetch = [&](int64_t row) {
+        an.load((const char*)a.a + row * I * SZ, a_bytes, (a.sg.rows - row) * I * SZ);
+        bn.load((const char*)a.b + row * J * SZ, b_bytes, (a.sg.rows - row) * J * SZ);
+    };
+    int k0 = wave * R;
+    int64_t row = k0 < n ? run_at(k0) : -1;
+    if (row >= 0) fetch(row);
+    for (; k0 < n; k0 += 4 * R) {
+        if (row >= 0) {
+            an.store(as, a_bytes);
+            bn.store(bs, b_bytes);
+        } else {                                           // the span's last rows, or rows that lie apart: one value at a time
+            for (int e = lane; e < R * I; e += 64) {
+                const int k = e / I;
+                const int64_t at = k0 + k < n ? (a.rowmap ? a.rowmap[q0 + k0 + k] : q0 + k0 + k) : -1;
+                *(T*)(as + e * SZ) = at >= 0 ? ((const T*)a.a)[at * I + e - k * I] : (T)0;
+            }
+            for (int e = lane; e < R * J; e += 64) {
+                const int k = e / J;
+                const int64_t at = k0 + k < n ? (a.rowmap ? a.rowmap[q0 + k0 + k] : q0 + k0 + k) : -1;
+                *(T*)(bs + e * SZ) = at >= 0 ? ((const T*)a.b)[at * J + e - k * J] : (T)0;
+            }
+        }
+        wave_lds_order();
+        const int k1 = k0 + 4 * R;
+        if (k1 < n) {
+            row = run_at(k1);
+            if (row >= 0) fetch(row);
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            u32x4 af[IF], bf[JF];
+#pragma unroll
+            for (int i = 0; i < IF; ++i) {
+                T e[E];
+                const int c = min(16 * i + l15, I - 1);
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = *(const T*)(as + (((4 * h + kk) * E + j) * I + c) * SZ);
+                __builtin_memcpy(&af[i], e, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < JF; ++i) {
+                T e[E];
+                const int c = min(16 * i + l15, J - 1);
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = *(const T*)(bs + (((4 * h + kk) * E + j) * J + c) * SZ);
+                if (i == J >> 4)
+#pragma unroll
+                    for (int j = 0; j < E; ++j) e[j] = l15 == (J & 15) ? (T)1 : e[j];
+                __builtin_memcpy(&bf[i], e, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < IF; ++i)
+#pragma unroll
+                for (int j = 0; j < JF; ++j) acc[i][j] = M::mma(af[i], bf[j], acc[i][j]);
+        }
+        wave_lds_order();
+    }
+
+    // the four waves' sums, in their order
+    Sum* sum = (Sum*)lds_all;
+    constexpr int W = 16 * JF;
+    for (int turn = 0; turn < 4; ++turn) {
+        __syncthreads();
+        if (wave == turn) {
+#pragma unroll
+            for (int i = 0; i < IF; ++i)
+#pragma unroll
+                for (int j = 0; j < JF; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = (16 * i + M::row(r, kk)) * W + 16 * j + l15;
+                        sum[at] = turn ? sum[at] + acc[i][j][r] : acc[i][j][r];
+                    }
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < I * J; e += 256) {
+        const Sum v = sum[e / J * W + e % J];
+        if (whole) ((T*)a.out)[(int64_t)g * I * J + e] = (T)v;
+        else parts[t * I * J + e] = v;
+    }
+    if (a.cols)
+        for (int i = threadIdx.x; i < I; i += 256) {
+            const Sum v = sum[i * W + J];
+            if (whole) ((T*)a.cols)[(int64_t)g * I + i] = (T)v;
+            else col_parts[t * I + i] = v;
+        }
+}
+
+template <typename T, int IF, int JF>
+static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
+    using Sum = typename Mat<T>::Sum;
+    constexpr int SZ = (int)sizeof(T), R = SZ == 2 ? 32 : 16;
+    constexpr int HA = R * 16 * IF * SZ / 1024, HB = R * 16 * JF * SZ / 1024;
+    const int64_t size = (int64_t)a.I * a.J + a.I;
+    int ts = 8;
+    while (ts < 40 && ((a.sg.rows >> ts) > 4 * ctx->prop.multiProcessorCount || (a.sg.rows >> ts) * size * (int64_t)sizeof(Sum) > (256ll << 20))) ++ts;
+    const int64_t spans = (a.sg.rows >> ts) + a.groups;
+    LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d groups are too many for one call", (long long)a.sg.rows, a.groups);
+    void* parts = nullptr;
+    const bool split = a.sg.rows > (1ll << ts);
+    if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
+    Sum* cp = (Sum*)parts + spans * a.I * a.J;
+    const int wave_lds = (R * a.I * SZ + 15) / 16 * 16 + (R * a.J * SZ + 15) / 16 * 16;
+    const int lds = std::max(4 * wave_lds, 16 * IF * 16 * JF * (int)sizeof(Sum));
+    LN_LAUNCH(ctx, name, (sum_narrow<T, IF, JF, HA, HB>), dim3((unsigned)spans), dim3(256), lds, a, ts, (Sum*)parts, cp, wave_lds);
+    return split ? transform_join(ctx, a, sizeof(T) == 8 ? LNASR_F64 : sizeof(T) == 4 ? LNASR_F32 : std::is_same<T, _Float16>::value ? LNASR_F16 : LNASR_BF16,
+                                  ts, parts, cp)
+                 : 0;
+}
+
+template <typename T>
+static int sum_narrow_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
+    const int j = a.J + (a.cols ? 1 : 0);
+    if (a.I <= 16) return j <= 48 ? launch_sum_narrow<T, 1, 3>(ctx, a, name) : launch_sum_narrow<T, 1, 4>(ctx, a, name);
+    if (a.I <= 48) return j <= 16 ? launch_sum_narrow<T, 3, 1>(ctx, a, name) : j <= 48 ? launch_sum_narrow<T, 3, 3>(ctx, a, name) : launch_sum_narrow<T, 3, 4>(ctx, a, name);
+    return j <= 16 ? launch_sum_narrow<T, 4, 1>(ctx, a, name) : j <= 48 ? launch_sum_narrow<T, 4, 3>(ctx, a, name) : launch_sum_narrow<T, 4, 4>(ctx, a, name);
+}
+
+bool sum_narrow_ok(const SumArgs& a) {
+    return a.I <= 64 && a.J + (a.cols ? 1 : 0) <= 64 && a.lda == a.I && a.ldb == a.J;
+}
+
+int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name) {
+    switch (dtype) {
+        case LNASR_F64: return sum_narrow_t<double>(ctx, a, name);
+        case LNASR_F32: return sum_narrow_t<float>(ctx, a, name);
+        case LNASR_F16: return sum_narrow_t<_Float16>(ctx, a, name);
+        default: return sum_narrow_t<__bf16>(ctx, a, name);
+    }
+}
+
+}  // namespace lnasr

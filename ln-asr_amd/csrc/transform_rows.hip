@@ -5,19 +5,6 @@
 
 namespace lnasr {
 
-// Consecutive block numbers go to the eight dies (XCDs) in turn, each with an L2 of its own: give every die a run of
-// neighbouring tiles, so that the tiles that share a matrix or a span of rows share an L2.
-__device__ __forceinline__ unsigned die_order(unsigned id, unsigned total) {
-    const unsigned per = total / 8, rest = total % 8, die = id % 8, at = id / 8;
-    return die * per + min(die, rest) + at;
-}
-
-// 16 bytes a lane from base + offset to LDS at `to` (wave-uniform) + 16 * lane; zeros where offset >= 2^31
-__device__ __forceinline__ void bring_piece(const char* base, unsigned offset, char* to) {
-    const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x80000000u, 0x00027000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
-}
-
 // ------------------------------------------------------------------------------------------
 // Tiles of TM rows x TN results, WM x WN waves.  Both operands pass through LDS in steps of 128 bytes of k, double buffered, as
 // 16-byte pieces in the order of the threads that bring them (LDS-DMA, buffer_load ... lds, needs just that).  Which piece a
@@ -61,10 +48,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     }
     const int nrow = (int)(r1 - r0);                                                 // 1 .. TM
 
-    // runs of 16 columns at other places on other lines: the lines that one read touches differ in l15 >> 2 and kk (16 bit) or
-    // in kk alone
-    auto spread = [](int k) { return SZ == 2 ? ((k & 3) | (k >> 1 & 4)) & (LINE / 2 - 1) : SZ == 4 ? k >> 2 & 3 & (LINE / 4 - 1) : k >> 1 & 1 & (LINE / 8 - 1); };
-
     Acc acc[NR][MR];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -84,23 +67,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
                 const int c = wn + 16 * n;
                 if constexpr (!KN) {
                     wf[n] = *(const u32x4*)(ws + (c + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
-                } else if constexpr (SZ == 2) {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s16x4 lds16x4;
-                    const int k = 32 * h + 8 * kk + (l15 >> 2);
-                    const char* at = ws + k * (TN * 2) + (((c / 16) ^ spread(k)) << 5) + (l15 & 3) * 8;
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)at);
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(at + 4 * (TN * 2)));
-                    __builtin_memcpy(&wf[n], &lo, 8);
-                    __builtin_memcpy((char*)&wf[n] + 8, &hi, 8);
                 } else {
-                    T e[E];
-#pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        const int k = (4 * h + kk) * E + j;
-                        e[j] = *(const T*)(ws + k * (TN * SZ) + (((c / 16) ^ spread(k)) * 16 + l15) * SZ);
-                    }
-                    __builtin_memcpy(&wf[n], e, 16);
+                    wf[n] = strided_fragment<T, TN>(ws, h, c);
                 }
             }
 #pragma unroll
@@ -134,7 +102,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             for (int i = 0; i < WI; ++i) {
                 const int q = tid + NT * i;
                 if (KN) {
-                    const int k = q / LINE, c = (q % LINE ^ spread(k) * SZ) * E;
+                    const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
                     wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
                 } else {
                     const int row = q >> 3;
@@ -165,7 +133,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         for (int i = 0; i < WI; ++i) {
             const int q = tid + NT * i;
             if (KN) {
-                const int k = q / LINE, c = (q % LINE ^ spread(k) * SZ) * E;
+                const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
                 wo[i] = n0 + c < a.N ? (unsigned)k * (unsigned)(ldw * SZ) + c * SZ : OUT;
             } else {
                 wo[i] = (unsigned)min(q >> 3, a.N - 1 - n0) * (unsigned)(ldw * SZ) + xk * SZ;
@@ -309,6 +277,7 @@ static int rows_any(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 
 int transform_rows(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name) {
     if (a.sg.rows == 0 || a.sg.S == 0 || a.N == 0) return 0;
+    if (rows_narrow_ok(a)) return transform_rows_narrow(ctx, dtype, a, name);
     switch (dtype) {
         case LNASR_F64: return rows_any<double>(ctx, a, name);
         case LNASR_F32: return rows_any<float>(ctx, a, name);
