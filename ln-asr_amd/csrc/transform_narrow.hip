@@ -14,41 +14,64 @@ __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The bytes [0, bytes) from src to the wave's LDS by 16 a lane; HF * 1024 at least `bytes`.  `room` bytes of src may be read.
+// `bytes` (a multiple of 16, at most 1024 HF) from src to the wave's LDS, 16 a lane; lanes past the end load nothing.  No branches:
+// the wait for the loads can then be told from that for stores that came after them.
 template <typename T, int HF>
 struct Chunk {
     u32x4 v[HF];
-    __device__ __forceinline__ void load(const char* src, int bytes, int64_t room) {
-        const int lane = threadIdx.x & 63;
-        if (room >= (int64_t)((bytes + 15) & ~15)) {
+    __device__ __forceinline__ void load(const char* src, int bytes) {
+        const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, (unsigned)bytes, 0x00027000);
+        const int at = (threadIdx.x & 63) * 16;
 #pragma unroll
-            for (int i = 0; i < HF; ++i)
-                if ((i * 64 + lane) * 16 < bytes) __builtin_memcpy(&v[i], src + (i * 64 + lane) * 16, 16);
-        } else {                                           // the end of the array
-#pragma unroll
-            for (int i = 0; i < HF; ++i) {
-                const int64_t at = (i * 64 + lane) * 16;
-                v[i] = load_piece((const T*)src, at / (int)sizeof(T), room > 0 ? room / (int)sizeof(T) : 0);
-            }
-        }
+        for (int i = 0; i < HF; ++i) v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, at + 1024 * i, 0, 0));
     }
-    __device__ __forceinline__ void store(char* lds, int bytes) const {
-        const int lane = threadIdx.x & 63;
+    // the same where the array ends after `room` bytes
+    __device__ __forceinline__ void load_end(const char* src, int64_t room) {
 #pragma unroll
         for (int i = 0; i < HF; ++i)
-            if ((i * 64 + lane) * 16 < bytes) *(u32x4*)(lds + (i * 64 + lane) * 16) = v[i];
+            v[i] = load_piece((const T*)src, ((threadIdx.x & 63) + 64 * i) * Mat<T>::E, room > 0 ? room / (int)sizeof(T) : 0);
+    }
+    __device__ __forceinline__ void store(char* lds, int bytes) const {
+        const int at = (threadIdx.x & 63) * 16;
+#pragma unroll
+        for (int i = 0; i < HF; ++i)
+            if (at + 1024 * i < bytes) *(u32x4*)(lds + at + 1024 * i) = v[i];
     }
 };
+// values of a small array; 0 where `live` does not hold
+template <typename T>
+struct Words {
+    __amdgpu_buffer_rsrc_t d;
+    __device__ __forceinline__ Words(const T* p, int n) : d(__builtin_amdgcn_make_buffer_rsrc((void*)p, 0, n * (unsigned)sizeof(T), 0x00027000)) {}
+    __device__ __forceinline__ T get(int i, bool live) const {
+        const unsigned at = live ? i * (unsigned)sizeof(T) : 0xffffffffu;
+        if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(d, at, 0, 0));
+        else if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(d, at, 0, 0));
+        else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(d, at, 0, 0));
+    }
+};
+// 16-byte pieces of the wave's LDS to memory, the counterpart of Chunk
+template <int HF>
+__device__ __forceinline__ void put_chunk(char* to, const char* lds, int bytes) {
+    const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)to, 0, (unsigned)bytes, 0x00027000);
+    const int at = (threadIdx.x & 63) * 16;
+    u32x4 v[HF];
+#pragma unroll
+    for (int i = 0; i < HF; ++i) v[i] = *(const u32x4*)(lds + at + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < HF; ++i) __builtin_amdgcn_raw_buffer_store_b128(v[i], d, at + 1024 * i, 0, 0);
+}
 
 // ------------------------------------------------------------------------------------------
 // y[r] = scale (W x[r]) + bias: the four waves of a block share a span of rows, each takes 16 at a time.  The next 16 rows are on
-// their way while the current ones multiply.  N <= 16 NF, K sizeof(T) <= 64 HF.
+// their way while the current ones multiply, and the stores of the last ones are not waited for.  N <= 16 NF, K sizeof(T) <= 64
+// HF; `one` (there is a bias): K + 1 values fit, the bias is a column of W that meets a one behind each row.
 // ------------------------------------------------------------------------------------------
 template <typename T, int NF, int HF>
-__global__ __launch_bounds__(256) void rows_narrow(RowsArgs a, int ts, int wave_lds) {
+__global__ __launch_bounds__(256, NF * HF <= 15 ? 3 : 1) void rows_narrow(RowsArgs a, int ts, int wave_lds) {
     using M = Mat<T>;
     using Sum = typename M::Sum;
-    constexpr int SZ = (int)sizeof(T), E = M::E;
+    constexpr int SZ = (int)sizeof(T), E = M::E, HO = (16 * 16 * NF * SZ + 1023) / 1024;
     extern __shared__ __attribute__((aligned(16))) char lds_all[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
     char* lds = lds_all + wave * wave_lds;
@@ -60,57 +83,55 @@ __global__ __launch_bounds__(256) void rows_narrow(RowsArgs a, int ts, int wave_
     r0 += wave * 16;
     if (r0 >= r1) return;
 
-    const int in_bytes = 16 * a.K * SZ, K = a.K, N = a.N;
+    const int K = a.K, N = a.N, in_bytes = 16 * K * SZ, out_bytes = 16 * N * SZ;
+    const char* x = (const char*)a.x + r0 * K * SZ;
+    char* y = (char*)a.y + r0 * N * SZ;
     Chunk<T, HF> next;
-    next.load((const char*)a.x + r0 * K * SZ, in_bytes, (a.sg.rows - r0) * K * SZ);
+    // (rows past the span may be read, past the array not: its last, uneven rows are loaded when their turn comes)
+    auto fetch = [&](int64_t r) {
+        next.load(x, r < r1 && r + 16 <= a.sg.rows ? in_bytes : 0);
+        x += 64 * K * SZ;
+    };
+    fetch(r0);
 
-    const T* w = (const T*)a.w + slot * a.w_stride;
+    // (32-bit offsets and zeros for what lies outside, without a branch or an address in registers)
+    const Words<T> w((const T*)a.w + slot * a.w_stride, K * N), bias((const T*)a.bias + slot * a.bias_stride, a.bias ? N : 0);
+    const int wc = a.kn ? 1 : K, wk = a.kn ? N : 1;
     u32x4 wf[NF][HF];
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
         const int c = min(16 * n + l15, N - 1);
 #pragma unroll
         for (int h = 0; h < HF; ++h) {
-            const int k = (4 * h + kk) * E;
-            if (a.kn) {
-                T e[E];
+            T e[E];
 #pragma unroll
-                for (int j = 0; j < E; ++j) e[j] = k + j < K ? w[(k + j) * N + c] : (T)0;
-                __builtin_memcpy(&wf[n][h], e, 16);
-            } else {
-                wf[n][h] = load_piece(w + c * K, k, K);
+            for (int j = 0; j < E; ++j) {
+                const int k = (4 * h + kk) * E + j;
+                e[j] = w.get(c * wc + k * wk, k < K);
+                if ((4 * h + 4) * E > K) {                                    // (the same for every lane)
+                    const T b = bias.get(c, k == K);
+                    e[j] = k == K ? b : e[j];
+                }
             }
+            __builtin_memcpy(&wf[n][h], e, 16);
         }
     }
-    Sum bv[NF][4];
-    const T* bias = a.bias ? (const T*)a.bias + slot * a.bias_stride : nullptr;
-#pragma unroll
-    for (int n = 0; n < NF; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int c = 16 * n + M::row(r, kk);
-            bv[n][r] = bias && c < N ? (Sum)bias[c] : (Sum)0;
-        }
     const Sum scale = a.scale ? (Sum)a.scale[slot] : (Sum)1;
 
-    for (; r0 < r1; r0 += 64) {
-        next.store(lds, in_bytes);
-        wave_lds_order();
+    // 16 rows in LDS -> their results in LDS
+    auto multiply = [&]() {
         u32x4 xf[HF];
 #pragma unroll
         for (int h = 0; h < HF; ++h) {
             const int k = (4 * h + kk) * E;
-            if ((4 * h + 4) * E <= K) {                    // (the same for every lane)
-                __builtin_memcpy(&xf[h], lds + (l15 * K + k) * SZ, 16);
-            } else {
-                T e[E];
+            T e[E];
+            __builtin_memcpy(e, lds + (l15 * K + k) * SZ, 16);                // (past a row's end: the next row, or what lies behind)
+            if ((4 * h + 4) * E > K)                                          // (the same for every lane)
 #pragma unroll
-                for (int j = 0; j < E; ++j) e[j] = k + j < K ? *(const T*)(lds + (l15 * K + k + j) * SZ) : (T)0;
-                __builtin_memcpy(&xf[h], e, 16);
-            }
+                for (int j = 0; j < E; ++j) e[j] = k + j < K ? e[j] : k + j == K ? (T)1 : (T)0;
+            __builtin_memcpy(&xf[h], e, 16);
         }
         wave_lds_order();
-        if (r0 + 64 < r1) next.load((const char*)a.x + (r0 + 64) * K * SZ, in_bytes, (a.sg.rows - r0 - 64) * K * SZ);
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
             typename M::Acc acc = typename M::Acc{0, 0, 0, 0};
@@ -119,21 +140,34 @@ __global__ __launch_bounds__(256) void rows_narrow(RowsArgs a, int ts, int wave_
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int c = 16 * n + M::row(r, kk);
-                if (c < N) *(T*)(lds + (l15 * N + c) * SZ) = (T)(acc[r] * scale + bv[n][r]);      // the one rounding of the result
+                if (c < N) *(T*)(lds + (l15 * N + c) * SZ) = (T)(acc[r] * scale);     // the one rounding of the result
             }
         }
         wave_lds_order();
-        const int out_bytes = (int)min(r1 - r0, (int64_t)16) * N * SZ;
-        char* y = (char*)a.y + r0 * N * SZ;
-        for (int at = lane * 16; at < out_bytes; at += 1024) {
-            if (at + 16 <= out_bytes) {
+    };
+    for (; r0 + 16 <= r1; r0 += 64) {
+        next.store(lds, in_bytes);
+        wave_lds_order();
+        fetch(r0 + 64);
+        multiply();
+        put_chunk<HO>(y, lds, out_bytes);
+        y += 64 * N * SZ;
+        wave_lds_order();
+    }
+    if (r0 < r1) {                                                            // the span's last rows
+        if (r0 + 16 > a.sg.rows) next.load_end(x - 64 * K * SZ, (a.sg.rows - r0) * K * SZ);
+        next.store(lds, in_bytes);
+        wave_lds_order();
+        multiply();
+        const int bytes = (int)(r1 - r0) * N * SZ;
+        for (int at = lane * 16; at < bytes; at += 1024) {
+            if (at + 16 <= bytes) {
                 const u32x4 v = *(const u32x4*)(lds + at);
                 __builtin_memcpy(y + at, &v, 16);
             } else {
-                for (int b = at; b < out_bytes; b += SZ) *(T*)(y + b) = *(const T*)(lds + b);
+                for (int b = at; b < bytes; b += SZ) *(T*)(y + b) = *(const T*)(lds + b);
             }
         }
-        wave_lds_order();
     }
 }
 
@@ -144,7 +178,8 @@ static int launch_narrow(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     while (ts < 10 && (a.sg.rows >> ts) > 8 * ctx->prop.multiProcessorCount) ++ts;
     const int64_t spans = (a.sg.rows >> ts) + a.sg.S;
     LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d segments are too many for one call", (long long)a.sg.rows, a.sg.S);
-    const int wave_lds = (16 * std::max(a.K, a.N) * (int)sizeof(T) + 15) / 16 * 16;
+    // (a fragment's read may run 64 bytes past the last row, put_chunk's up to the end of its last kilobyte)
+    const int wave_lds = std::max(16 * a.K * (int)sizeof(T) + 64, (16 * 16 * NF * (int)sizeof(T) + 1023) / 1024 * 1024);
     LN_LAUNCH(ctx, name, (rows_narrow<T, NF, HF>), dim3((unsigned)spans), dim3(256), 4 * wave_lds, a, ts, wave_lds);
     return 0;
 }
@@ -158,7 +193,7 @@ static int narrow_n(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 
 template <typename T>
 static int narrow_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
-    const int bytes = a.K * (int)sizeof(T);
+    const int bytes = (a.K + (a.bias ? 1 : 0)) * (int)sizeof(T);
     if constexpr (sizeof(T) == 8) {
         if (bytes <= 128) return narrow_n<T, 2>(ctx, a, name);
         if (bytes <= 320) return narrow_n<T, 5>(ctx, a, name);
@@ -174,7 +209,7 @@ static int narrow_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 }
 
 bool rows_narrow_ok(const RowsArgs& a) {
-    return a.w_stride && a.K <= 64 && a.N <= 64 && a.ldx == a.K && a.ldy == a.N;
+    return a.w_stride && a.K + (a.bias ? 1 : 0) <= 64 && a.N <= 64 && a.ldx == a.K && a.ldy == a.N;
 }
 
 int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name) {
@@ -192,7 +227,7 @@ int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const ch
 // product: b has a column of ones behind its last.
 // ------------------------------------------------------------------------------------------
 template <typename T, int IF, int JF, int HA, int HB>
-__global__ __launch_bounds__(256) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts, typename Mat<T>::Sum* col_parts, int wave_lds) {
+__global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts, typename Mat<T>::Sum* col_parts, int wave_lds) {
     using M = Mat<T>;
     using Sum = typename M::Sum;
     constexpr int SZ = (int)sizeof(T), E = M::E, R = SZ == 2 ? 32 : 16, H = R / (4 * E);
@@ -232,9 +267,9 @@ __global__ __launch_bounds__(256) void sum_narrow(SumArgs a, int ts, typename Ma
         const bool fits = hi - lo == R - 1 && mine == lo + (lane & (R - 1));
         return __all(fits) ? lo : (int64_t)-1;
     };
-    auto fetch = [&](int64_t row) {
-        an.load((const char*)a.a + row * I * SZ, a_bytes, (a.sg.rows - row) * I * SZ);
-        bn.load((const char*)a.b + row * J * SZ, b_bytes, (a.sg.rows - row) * J * SZ);
+    auto fetch = [&](int64_t row) {                        // (R rows of the array: nothing past its end)
+        an.load((const char*)a.a + row * I * SZ, a_bytes);
+        bn.load((const char*)a.b + row * J * SZ, b_bytes);
     };
     int k0 = wave * R;
     int64_t row = k0 < n ? run_at(k0) : -1;
