@@ -153,6 +153,7 @@ __device__ __forceinline__ void bring_piece(const char* base, unsigned offset, c
 template <typename T, int C>
 __device__ __forceinline__ int spread(int k) {
     constexpr int RUNS = C / 16;
+    if ((RUNS & (RUNS - 1)) != 0) return 0;
     if (sizeof(T) == 2) return ((k & 3) | (k >> 1 & 4)) & (RUNS < 8 ? RUNS - 1 : 7);
     if (sizeof(T) == 4) return k >> 2 & (RUNS < 4 ? RUNS - 1 : 3);
     return k >> 1 & (RUNS < 2 ? RUNS - 1 : 1);

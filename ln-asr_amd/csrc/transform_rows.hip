@@ -5,38 +5,196 @@
 
 namespace lnasr {
 
+// acc[n][m] += p L_k' for the rows row0 + 16 m + (lane & 15) < row1 and the columns c0 + 16 n .., segment by segment with the
+// adapter of each (those numbered `turn` modulo `turns`).  64 segments are looked up at a time, a lane each; fragments come straight
+// from memory: for segments of a few rows every adapter is read once and there is nothing to share.
+template <typename T, bool KN, int MR, int NR>
+__device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, int64_t row1, int c0, int turn, int turns,
+                                             typename Mat<T>::Acc (&acc)[NR][MR]) {
+    using M = Mat<T>;
+    constexpr int E = M::E;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
+    if (row0 >= row1) return;
+    const int last = (int)(row1 - 1 - row0);
+    const T* p = (const T*)a.p + row0 * a.ldp;
+    int count = 0;
+    for (int s = max(0, wave_search(a.sg.S, row0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; s += 64) {
+        const int mine = min(s + lane, a.sg.S - 1);
+        const int64_t lo = seg_off(a.sg, mine), hi = seg_off(a.sg, mine + 1);
+        const int slot = seg_slot(a.sg, mine);
+        const int from = (int)(max(lo, row0) - row0), to = (int)max((int64_t)0, min(hi, row1) - row0);     // (from may lie past `last`)
+        for (uint64_t todo = __ballot(s + lane < a.sg.S && lo < row1 && from < to && slot >= 0); todo; todo &= todo - 1) {
+            if (count++ % turns != turn) continue;
+            const int b = __builtin_ctzll(todo), f = __builtin_amdgcn_readlane(from, b), t = __builtin_amdgcn_readlane(to, b);
+            const T* low = (const T*)a.low + __builtin_amdgcn_readlane(slot, b) * a.low_stride;
+            for (int k0 = 0; k0 < a.R; k0 += 4 * E) {
+                const int k = k0 + kk * E;
+                u32x4 wf[NR];
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    const int c = min(c0 + 16 * n + l15, a.N - 1);
+                    if (KN) {
+                        T e[E];
+#pragma unroll
+                        for (int j = 0; j < E; ++j) e[j] = k + j < a.R ? low[(int64_t)(k + j) * a.N + c] : (T)0;
+                        __builtin_memcpy(&wf[n], e, 16);
+                    } else {
+                        wf[n] = load_piece(low + (int64_t)c * a.R, k, a.R);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < MR; ++m) {
+                    if (t <= 16 * m || f >= 16 * m + 16) continue;
+                    const int row = 16 * m + l15;
+                    const u32x4 pf = load_piece(p + (int64_t)min(row, last) * a.ldp, k, a.R);
+                    const bool in = row >= f && row < t;
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        // chosen, not masked by a product with zero: another row's adapter may hold a NaN
+                        const typename M::Acc d = M::mma(wf[n], pf, acc[n][m]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
+                    }
+                }
+            }
+        }
+        if (seg_off(a.sg, min(s + 64, a.sg.S)) >= row1) break;
+    }
+}
+
+// Writes acc (times scale, plus bias) to the rows row0 + 16 m + (lane & 15) < row1, columns c0 + 16 n ..
+template <typename T, int MR, int NR>
+__device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_t row1, int c0, typename Mat<T>::Sum scale, const T* bias,
+                                         const typename Mat<T>::Acc (&acc)[NR][MR]) {
+    using Sum = typename Mat<T>::Sum;
+    constexpr int SZ = (int)sizeof(T);
+    // four results of a row lie together, but for fp64 (whose instruction spreads them over the rows of its tile)
+    constexpr bool RUN = SZ != 8;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int c = c0 + 16 * n + (RUN ? 4 * kk : kk);
+        Sum bv[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bv[r] = bias && c + (RUN ? r : 4 * r) < a.N ? (Sum)bias[c + (RUN ? r : 4 * r)] : (Sum)0;
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            const int64_t row = row0 + 16 * m + l15;
+            if (row >= row1) continue;
+            T* y = (T*)a.y + row * a.ldy + c;
+            T v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = (T)(acc[n][m][r] * scale + bv[r]);     // the one rounding of the result
+            if (RUN && c + 4 <= a.N) {
+                __builtin_memcpy(y, v, 4 * SZ);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (c + (RUN ? r : 4 * r) < a.N) y[RUN ? r : 4 * r] = v[r];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// A few rows: 16 MR rows x 16 results a block, its eight waves divide k between them.  Bound by the latency of memory and, with many
+// groups, by the matrices read once: fragments go from memory to registers, many at a time, and meet in LDS at the end.
+// ------------------------------------------------------------------------------------------
+template <typename T, bool KN, int MR, int LOW>
+__global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, int ts) {
+    using M = Mat<T>;
+    using Acc = typename M::Acc;
+    constexpr int E = M::E, WAVES = 8, DEEP = MR == 1 ? 8 : MR == 2 ? 4 : 2;
+    __shared__ Acc part[WAVES - 1][MR][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
+    const int c0 = (int)(blockIdx.x % tiles_n) * 16;
+    int64_t r0, r1;
+    int slot = 0;
+    if (LOW == 0) {
+        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, blockIdx.x / tiles_n, ts, &r0, &r1);
+        if (s < 0) return;
+        slot = seg_slot(a.sg, s);
+        if (slot < 0) return;
+    } else {
+        r0 = seg_off(a.sg, 0) + (int64_t)(blockIdx.x / tiles_n) * (16 * MR);
+        r1 = min(seg_off(a.sg, a.sg.S), r0 + 16 * MR);
+        if (r0 >= r1) return;
+    }
+    const T* w = (const T*)a.w + (LOW ? 0 : slot * a.w_stride);
+    const T* x[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) x[m] = (const T*)a.x + min(r0 + 16 * m + l15, r1 - 1) * a.ldx;
+    const int c = min(c0 + l15, a.N - 1);
+    Acc acc[1][MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[0][m] = Acc{0, 0, 0, 0};
+    for (int k0 = wave * (4 * E * DEEP); k0 < a.K; k0 += WAVES * 4 * E * DEEP) {
+        u32x4 wf[DEEP], xf[DEEP][MR];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int k = k0 + (4 * d + kk) * E;
+            if (KN) {
+                T e[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = k + j < a.K ? w[(int64_t)(k + j) * a.N + c] : (T)0;
+                __builtin_memcpy(&wf[d], e, 16);
+            } else {
+                wf[d] = load_piece(w + (int64_t)c * a.K, k, a.K);
+            }
+#pragma unroll
+            for (int m = 0; m < MR; ++m) xf[d][m] = load_piece(x[m], k, a.K);
+        }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+            for (int m = 0; m < MR; ++m) acc[0][m] = M::mma(wf[d], xf[d][m], acc[0][m]);
+    }
+    if (LOW) add_adapters<T, KN, MR, 1>(a, r0, r1, c0, wave, WAVES, acc);
+    if (wave) {
+#pragma unroll
+        for (int m = 0; m < MR; ++m) part[wave - 1][m][lane] = acc[0][m];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < WAVES - 1; ++i)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) acc[0][m] += part[i][m][lane];
+    const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
+    put_tile<T, MR, 1>(a, r0, r1, c0, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc);
+}
+
 // ------------------------------------------------------------------------------------------
 // Tiles of TM rows x TN results, WM x WN waves.  Both operands pass through LDS in steps of 128 bytes of k, double buffered, as
-// 16-byte pieces in the order of the threads that bring them (LDS-DMA, buffer_load ... lds, needs just that).  Which piece a
-// thread brings is chosen so that the reads of a fragment spread over the banks:
+// 16-byte pieces in the order of the threads that bring them (LDS-DMA, buffer_load ... lds, needs just that; its addresses need
+// no alignment, so rows of 351 values take it too).  Which piece a thread brings is chosen so that the reads of a fragment spread
+// over the banks:
 //   k contiguous (x, and w [n, k]): rows of 8 pieces; place p of row r holds piece p ^ (r & 7)
-//   k strided (w [k, n]): lines of k; a fragment's 16 columns are sizeof(T) pieces, and the run of 16 columns at place p of line k
-//     is run p ^ spread(k).  16 bit: ds_read_b64_tr_b16 turns 4 k x 16 columns on the way to the registers.
-// DMA: every operand is aligned to 16 bytes and as wide as whole pieces; otherwise the pieces travel through registers, loaded a
-// step ahead.  The low-rank product is short and always takes the registers.
-// LOW: 0 none; 1 tiles are spans of one segment, whose adapter joins in; 2 tiles of rows that lie together, the adapters of
-// every segment they meet join in one after the other (short segments: a span of a few rows would waste its tile).
+//   k strided (w [k, n]): lines of k (spread, strided_fragment)
+// The first `full` steps go by LDS-DMA, the rest -- a last step that ends inside a piece -- through registers.
+// LOW: 0 none; 1 tiles are spans of one segment, whose adapter joins in; 2 tiles of rows that lie together (short segments: a
+// span of a few rows would waste its tile).
 // ------------------------------------------------------------------------------------------
-template <typename T, int TM, int TN, int WM, int WN, bool KN, bool DMA, int LOW>
-__global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigned tiles_n, int ts) {
+template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW>
+__global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigned tiles_n, int ts, int full) {
     using M = Mat<T>;
     using Acc = typename M::Acc;
     constexpr int SZ = (int)sizeof(T), E = M::E, KB = 128 / SZ, NT = 64 * WM * WN, MR = TM / WM / 16, NR = TN / WN / 16;
     constexpr int XB = TM * 128, WB = TN * 128, XI = TM * 8 / NT, WI = (TN * 8 + NT - 1) / NT;
     constexpr int LINE = TN * SZ / 16;                                                // pieces of a line of w [k, n]
-    static_assert(TM * 8 % NT == 0 && (TN * 8 % NT == 0 || (NT % (TN * 8) == 0)), "whole waves of pieces");
+    static_assert(TM * 8 % NT == 0 && TN * 8 % 64 == 0, "whole waves of pieces");
     __shared__ __attribute__((aligned(1024))) char lds[2 * (XB + WB)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
-    const bool brings_w = TN * 8 % NT == 0 || tid < TN * 8;                           // uniform over a wave
     const unsigned id = die_order(blockIdx.x, gridDim.x);
     const int n0 = (int)(id % tiles_n) * TN;
     const int64_t t = id / tiles_n;
+    auto brings_w = [&](int i) { return TN * 8 % NT == 0 || wave * 64 + NT * i < TN * 8; };
 
     int64_t r0, r1;
-    int slot = 0, s = 0;
+    int slot = 0;
     if (LOW != 2) {
-        s = find_span(a.sg.off, a.sg.S, a.sg.rows, t, ts, &r0, &r1);
+        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, t, ts, &r0, &r1);
         if (s < 0) return;
         slot = seg_slot(a.sg, s);
         if (slot < 0 && LOW == 0) return;
@@ -54,9 +212,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 #pragma unroll
         for (int m = 0; m < MR; ++m) acc[n][m] = Acc{0, 0, 0, 0};
 
-    // acc += X W' over the 128 bytes of k in buffer buf; with SEL only in the columns (rows of x) for which pred says so
-    auto multiply = [&](int buf, auto sel, const bool* pred) {
-        constexpr bool SEL = decltype(sel)::value;
+    // acc += X W' over the 128 bytes of k in buffer buf
+    auto multiply = [&](int buf) {
         const char* xs = lds + buf * (XB + WB);
         const char* ws = xs + XB;
 #pragma unroll
@@ -65,209 +222,154 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 const int c = wn + 16 * n;
-                if constexpr (!KN) {
-                    wf[n] = *(const u32x4*)(ws + (c + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
-                } else {
-                    wf[n] = strided_fragment<T, TN>(ws, h, c);
-                }
+                if constexpr (KN) wf[n] = strided_fragment<T, TN>(ws, h, c);
+                else wf[n] = *(const u32x4*)(ws + (c + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
             }
 #pragma unroll
             for (int m = 0; m < MR; ++m) xf[m] = *(const u32x4*)(xs + (wm + 16 * m + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int m = 0; m < MR; ++m) {
-                    const Acc d = M::mma(wf[n], xf[m], acc[n][m]);
-                    if (SEL) {
-                        // chosen, not masked by a product with zero: another row's adapter may hold a NaN
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[n][m][r] = pred[m] ? d[r] : acc[n][m][r];
-                    } else {
-                        acc[n][m] = d;
-                    }
-                }
+                for (int m = 0; m < MR; ++m) acc[n][m] = M::mma(wf[n], xf[m], acc[n][m]);
         }
     };
 
-    // through registers
-    u32x4 xr[XI], wr[WI];
-    auto load = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen) {
+    // one step through registers: what lies past klen (or, in a line of w, past N) is 0
+    auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen) {
+        u32x4 xr[XI], wr[WI];
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             const int q = tid + NT * i, row = q >> 3;
             xr[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ row) & 7) * E, klen);
         }
-        if (brings_w)
 #pragma unroll
-            for (int i = 0; i < WI; ++i) {
-                const int q = tid + NT * i;
-                if (KN) {
-                    const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
-                    wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
-                } else {
-                    const int row = q >> 3;
-                    wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
-                }
+        for (int i = 0; i < WI; ++i) {
+            if (!brings_w(i)) break;
+            const int q = tid + NT * i;
+            if (KN) {
+                const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
+                wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
+            } else {
+                const int row = q >> 3;
+                wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
             }
-    };
-    auto store = [&](int buf) {
-        char* xs = lds + buf * (XB + WB);
+        }
 #pragma unroll
-        for (int i = 0; i < XI; ++i) *(u32x4*)(xs + (tid + NT * i) * 16) = xr[i];
-        if (brings_w)
+        for (int i = 0; i < XI; ++i) *(u32x4*)(lds + (tid + NT * i) * 16) = xr[i];
 #pragma unroll
-            for (int i = 0; i < WI; ++i) *(u32x4*)(xs + XB + (tid + NT * i) * 16) = wr[i];
+        for (int i = 0; i < WI; ++i)
+            if (brings_w(i)) *(u32x4*)(lds + XB + (tid + NT * i) * 16) = wr[i];
+        __syncthreads();
+        multiply(0);
+        __syncthreads();
     };
 
     const T* x = (const T*)a.x + r0 * a.ldx;
     const T* w = (const T*)a.w + (LOW ? 0 : slot * a.w_stride);
     const int64_t ldw = KN ? a.N : a.K;
-    if constexpr (DMA) {
-        // offsets of this lane's pieces from the tile's first; out of range (the hardware then writes zeros) where k or n ends
-        constexpr unsigned OUT = 0xffffffffu;
+    if (full > 0) {
+        // offsets of this lane's pieces from the step's first; out of range (nothing is read, LDS gets zeros) past the last column
         unsigned xo[XI], wo[WI];
-        const int xk = ((tid ^ tid >> 3) & 7) * E;                                    // k of the lane's pieces in a step
+        const int xk = ((tid ^ tid >> 3) & 7) * 16;
 #pragma unroll
-        for (int i = 0; i < XI; ++i) xo[i] = (unsigned)min((tid + NT * i) >> 3, nrow - 1) * (unsigned)(a.ldx * SZ) + xk * SZ;
+        for (int i = 0; i < XI; ++i) xo[i] = (unsigned)min((tid + NT * i) >> 3, nrow - 1) * (unsigned)(a.ldx * SZ) + xk;
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
             const int q = tid + NT * i;
             if (KN) {
                 const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
-                wo[i] = n0 + c < a.N ? (unsigned)k * (unsigned)(ldw * SZ) + c * SZ : OUT;
+                wo[i] = n0 + c < a.N ? (unsigned)k * (unsigned)(ldw * SZ) + c * SZ : 0xffffffffu;
             } else {
-                wo[i] = (unsigned)min(q >> 3, a.N - 1 - n0) * (unsigned)(ldw * SZ) + xk * SZ;
+                wo[i] = (unsigned)min(q >> 3, a.N - 1 - n0) * (unsigned)(ldw * SZ) + xk;
             }
         }
         const char* xb = (const char*)x;
         const char* wb = (const char*)(KN ? w + n0 : w + (int64_t)n0 * ldw);
-        auto bring = [&](int buf, int left) {
+        auto bring = [&](int buf) {
             char* xs = lds + buf * (XB + WB);
-            const bool tail = left < KB;
 #pragma unroll
-            for (int i = 0; i < XI; ++i)
-                bring_piece(xb, tail && xk >= left ? OUT : xo[i], xs + (wave * 64 + NT * i) * 16);
-            if (brings_w)
+            for (int i = 0; i < XI; ++i) bring_piece(xb, xo[i], xs + (wave * 64 + NT * i) * 16);
 #pragma unroll
-                for (int i = 0; i < WI; ++i)
-                    bring_piece(wb, tail && (KN ? (tid + NT * i) / LINE : xk) >= left ? OUT : wo[i], xs + XB + (wave * 64 + NT * i) * 16);
+            for (int i = 0; i < WI; ++i)
+                if (brings_w(i)) bring_piece(wb, wo[i], xs + XB + (wave * 64 + NT * i) * 16);
             xb += KB * SZ;
             wb += KN ? KB * ldw * SZ : KB * SZ;
         };
-        bring(0, a.K);
+        bring(0);
         __syncthreads();
-        int buf = 0;
-        for (int left = a.K; left > 0; left -= KB, buf ^= 1) {
-            if (left > KB) bring(buf ^ 1, left - KB);
-            multiply(buf, std::false_type{}, nullptr);
-            __syncthreads();
-        }
-    } else {
-        load(x, a.ldx, w, ldw, 0, a.K);
-        store(0);
-        __syncthreads();
-        int buf = 0;
-        for (int k0 = 0; k0 < a.K; k0 += KB, buf ^= 1) {
-            const bool more = k0 + KB < a.K;
-            if (more) load(x, a.ldx, w, ldw, k0 + KB, a.K);
-            multiply(buf, std::false_type{}, nullptr);
-            if (more) store(buf ^ 1);
+        for (int i = 0; i < full; ++i) {
+            if (i + 1 < full) bring((i + 1) & 1);
+            multiply(i & 1);
             __syncthreads();
         }
     }
+    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K);
 
-    auto adapter = [&](int k, auto sel, const bool* pred) {
-        const T* p = (const T*)a.p + r0 * a.ldp;
-        const T* low = (const T*)a.low + k * a.low_stride;
-        for (int k0 = 0; k0 < a.R; k0 += KB) {
-            load(p, a.ldp, low, KN ? a.N : a.R, k0, a.R);
-            store(0);
-            __syncthreads();
-            multiply(0, sel, pred);
-            __syncthreads();
-        }
-    };
-    if (LOW == 1 && slot >= 0) adapter(slot, std::false_type{}, nullptr);
-    if (LOW == 2) {
-        for (s = max(0, wave_search(a.sg.S, r0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; ++s) {
-            const int64_t lo = seg_off(a.sg, s), hi = seg_off(a.sg, s + 1);
-            if (lo >= r1) break;
-            const int k = seg_slot(a.sg, s);
-            if (hi <= r0 || lo >= hi || k < 0) continue;
-            bool pred[MR];
-#pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                const int64_t r = r0 + wm + 16 * m + l15;
-                pred[m] = r >= lo && r < hi;
-            }
-            adapter(k, std::true_type{}, pred);
-        }
+    if (LOW == 1 && slot >= 0) {
+        const T* low = (const T*)a.low + slot * a.low_stride;
+        for (int k0 = 0; k0 < a.R; k0 += KB) step((const T*)a.p + r0 * a.ldp, a.ldp, low, KN ? a.N : a.R, k0, a.R);
     }
+    if (LOW == 2) add_adapters<T, KN, MR, NR>(a, r0 + wm, r1, n0 + wn, 0, 1, acc);
 
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
-    const T* bias = a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr;
-    // four results of a row lie together, but for fp64 (whose instruction spreads them over the rows of its tile)
-    constexpr bool RUN = SZ != 8;
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        const int c0 = n0 + wn + 16 * n + (RUN ? 4 * kk : kk);
-        typename M::Sum bv[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) bv[r] = bias && c0 + (RUN ? r : 4 * r) < a.N ? (typename M::Sum)bias[c0 + (RUN ? r : 4 * r)] : (typename M::Sum)0;
-#pragma unroll
-        for (int m = 0; m < MR; ++m) {
-            const int row = wm + 16 * m + l15;
-            if (row >= nrow) continue;
-            T* y = (T*)a.y + (r0 + row) * a.ldy + c0;
-            T v[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(acc[n][m][r] * scale + bv[r]);     // the one rounding of the result
-            if (RUN && c0 + 4 <= a.N) {
-                __builtin_memcpy(y, v, 4 * SZ);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c0 + (RUN ? r : 4 * r) < a.N) y[RUN ? r : 4 * r] = v[r];
-            }
-        }
-    }
+    put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc);
 }
+
+constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
 template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW>
 static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
-    constexpr int ts = TM == 256 ? 8 : TM == 128 ? 7 : 6;
-    static_assert(TM == 1 << ts, "tile heights");
+    static_assert(TM == 1 << log2_of(TM), "tile heights");
+    constexpr int KB = 128 / (int)sizeof(T), E = Mat<T>::E;
     const int64_t tiles_n = (a.N + TN - 1) / TN, tiles_m = LOW != 2 ? a.sg.rows / TM + a.sg.S : (a.sg.rows + TM - 1) / TM;
     LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
-    // 16-byte pieces throughout, and a tile's offsets within 31 bits
-    const int64_t e = 16 / sizeof(T), ldw = KN ? a.N : a.K;
-    const bool dma = ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.K % e == 0 && (!KN || a.N % e == 0) && a.ldx % e == 0 &&
-                     a.ldx * TM * (int64_t)sizeof(T) < (1ll << 31) && ldw * std::max(TN, 64) * (int64_t)sizeof(T) < (1ll << 31);
-    const dim3 grid((unsigned)(tiles_n * tiles_m)), block(64 * WM * WN);
-    if (dma) LN_LAUNCH(ctx, name, (rows_tile<T, TM, TN, WM, WN, KN, true, LOW>), grid, block, 0, a, (unsigned)tiles_n, ts);
-    else LN_LAUNCH(ctx, name, (rows_tile<T, TM, TN, WM, WN, KN, false, LOW>), grid, block, 0, a, (unsigned)tiles_n, ts);
+    // Steps for the LDS-DMA: whole ones; not the last line of w [k, n] where a piece would run past its end (elsewhere it runs
+    // into the next line); none where a tile's offsets pass 31 bits
+    const int64_t ldw = KN ? a.N : a.K;
+    int full = KN && a.N % E ? (a.K - 1) / KB : a.K / KB;
+    if (a.ldx * TM * (int64_t)sizeof(T) >= (1ll << 31) || ldw * std::max(TN, KB) * (int64_t)sizeof(T) >= (1ll << 31)) full = 0;
+    LN_LAUNCH(ctx, name, (rows_tile<T, TM, TN, WM, WN, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(64 * WM * WN), 0, a,
+              (unsigned)tiles_n, log2_of(TM), full);
+    return 0;
+}
+
+template <typename T, bool KN, int MR, int LOW>
+static int launch_few(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
+    const int64_t tiles_n = (a.N + 15) / 16, tiles_m = LOW == 0 ? a.sg.rows / (16 * MR) + a.sg.S : (a.sg.rows + 16 * MR - 1) / (16 * MR);
+    LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
+    LN_LAUNCH(ctx, name, (rows_few<T, KN, MR, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_n, log2_of(16 * MR));
     return 0;
 }
 
 template <typename T, bool KN, int LOW>
 static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
-    if (a.N <= 32) return launch_tile<T, 128, 32, 4, 1, KN, LOW>(ctx, a, name);
-    if (a.N <= 64) return launch_tile<T, 128, 64, 4, 1, KN, LOW>(ctx, a, name);
-    if constexpr (sizeof(T) == 2) {
-        if (a.sg.rows / 256 * (a.N / 256) >= 256) return launch_tile<T, 256, 256, 2, 4, KN, LOW>(ctx, a, name);
-        return launch_tile<T, 128, 128, 2, 2, KN, LOW>(ctx, a, name);
-    } else if constexpr (sizeof(T) == 4) {
-        return launch_tile<T, 128, 128, 2, 2, KN, LOW>(ctx, a, name);
-    } else {
-        return launch_tile<T, 128, 128, 2, 4, KN, LOW>(ctx, a, name);
+    const int64_t cus = ctx->prop.multiProcessorCount, rows = a.sg.rows;
+    if constexpr (LOW != 2) {
+        if (a.N <= 16) return launch_tile<T, 128, 16, 4, 1, KN, LOW>(ctx, a, name);
+        if (a.N <= 32) return launch_tile<T, 128, 32, 4, 1, KN, LOW>(ctx, a, name);
+        if (a.N <= 48) return launch_tile<T, 128, 48, 4, 1, KN, LOW>(ctx, a, name);
+        if (a.N <= 64) return launch_tile<T, 128, 64, 4, 1, KN, LOW>(ctx, a, name);
+        if constexpr (sizeof(T) == 2)
+            if (rows / 256 * (a.N / 256) >= cus) return launch_tile<T, 256, 256, 2, 4, KN, LOW>(ctx, a, name);
+        constexpr int WN = sizeof(T) == 8 ? 4 : 2;
+        if ((rows / 128 + a.sg.S) * ((a.N + 127) / 128) >= 4 * cus) return launch_tile<T, 128, 128, 2, WN, KN, LOW>(ctx, a, name);
     }
+    return launch_tile<T, 64, 64, 2, 2, KN, LOW>(ctx, a, name);
 }
 
 template <typename T, bool KN>
 static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
-    if (a.w_stride) return rows_t<T, KN, 0>(ctx, a, name);
-    if (a.sg.rows / a.sg.S >= 64) return rows_t<T, KN, 1>(ctx, a, name);
-    return launch_tile<T, 64, 64, 2, 2, KN, 2>(ctx, a, name);
+    const int64_t cus = ctx->prop.multiProcessorCount, rows = a.sg.rows, mean = rows / a.sg.S;
+    if (a.w_stride) {
+        if (mean <= 16) return launch_few<T, KN, 1, 0>(ctx, a, name);
+        if (mean <= 32) return launch_few<T, KN, 2, 0>(ctx, a, name);
+        return rows_t<T, KN, 0>(ctx, a, name);
+    }
+    if (rows <= 16) return launch_few<T, KN, 1, 2>(ctx, a, name);
+    if (rows <= 32) return launch_few<T, KN, 2, 2>(ctx, a, name);
+    if (rows * a.N <= 64 * 16 * 2 * cus) return launch_few<T, KN, 4, 2>(ctx, a, name);
+    if (mean >= 64) return rows_t<T, KN, 1>(ctx, a, name);
+    return rows_t<T, KN, 2>(ctx, a, name);
 }
 
 template <typename T>
