@@ -134,6 +134,12 @@ __device__ __forceinline__ u32x4 load_piece(const T* line, long c, long end) {
     return v;
 }
 
+// LDS of one wave is its own: order its writes and reads for the compiler (the hardware keeps the order of a wave's LDS accesses)
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Consecutive block numbers go to the eight dies (XCDs) in turn, each with an L2 of its own: give every die a run of
 // neighbouring tiles, so that the tiles that share a matrix or a span of rows share an L2.
 __device__ __forceinline__ unsigned die_order(unsigned id, unsigned total) {

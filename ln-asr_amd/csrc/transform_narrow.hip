@@ -8,12 +8,6 @@
 
 namespace lnasr {
 
-// LDS of one wave is its own: order its writes and reads for the compiler (the hardware keeps the order of a wave's LDS accesses)
-__device__ __forceinline__ void wave_lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // `bytes` (a multiple of 16, at most 1024 HF) from src to the wave's LDS, 16 a lane; lanes past the end load nothing.  No branches:
 // the wait for the loads can then be told from that for stores that came after them.
 template <typename T, int HF>

@@ -62,37 +62,58 @@ __device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, in
     }
 }
 
-// Writes acc (times scale, plus bias) to the rows row0 + 16 m + (lane & 15) < row1, columns c0 + 16 n ..
+// Writes acc (times scale, plus bias) to the rows row0 + 16 m + (lane & 15) < row1, columns c0 + 16 n ..  Sixteen rows at a time pass
+// through `scratch` (the wave's own put_scratch bytes of LDS), so that a row's results leave as whole runs of 16-byte pieces: as the
+// matrix instruction leaves them, 32 bytes of a row at a time, twice the bytes went out to memory.
+template <typename T, int NR>
+constexpr int put_scratch() {
+    return 16 * (NR * 16 * (int)sizeof(T) + 16);
+}
 template <typename T, int MR, int NR>
 __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_t row1, int c0, typename Mat<T>::Sum scale, const T* bias,
-                                         const typename Mat<T>::Acc (&acc)[NR][MR]) {
-    using Sum = typename Mat<T>::Sum;
-    constexpr int SZ = (int)sizeof(T);
-    // four results of a row lie together, but for fp64 (whose instruction spreads them over the rows of its tile)
-    constexpr bool RUN = SZ != 8;
+                                         const typename Mat<T>::Acc (&acc)[NR][MR], char* scratch) {
+    using M = Mat<T>;
+    using Sum = typename M::Sum;
+    constexpr int SZ = (int)sizeof(T), E = M::E, PITCH = NR * 16 * SZ + 16, PER = NR * SZ;       // bytes, pieces of a row
     const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
+    Sum bv[NR][4];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        const int c = c0 + 16 * n + (RUN ? 4 * kk : kk);
-        Sum bv[4];
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bv[r] = bias && c + (RUN ? r : 4 * r) < a.N ? (Sum)bias[c + (RUN ? r : 4 * r)] : (Sum)0;
+        for (int r = 0; r < 4; ++r) {
+            const int c = c0 + 16 * n + M::row(r, kk);
+            bv[n][r] = bias && c < a.N ? (Sum)bias[c] : (Sum)0;
+        }
 #pragma unroll
-        for (int m = 0; m < MR; ++m) {
-            const int64_t row = row0 + 16 * m + l15;
-            if (row >= row1) continue;
-            T* y = (T*)a.y + row * a.ldy + c;
+    for (int m = 0; m < MR; ++m) {
+        if (row0 + 16 * m >= row1) break;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
             T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(acc[n][m][r] * scale + bv[r]);     // the one rounding of the result
-            if (RUN && c + 4 <= a.N) {
-                __builtin_memcpy(y, v, 4 * SZ);
+            for (int r = 0; r < 4; ++r) v[r] = (T)(acc[n][m][r] * scale + bv[n][r]);             // the one rounding of the result
+            if constexpr (SZ != 8) {
+                __builtin_memcpy(scratch + l15 * PITCH + (16 * n + 4 * kk) * SZ, v, 4 * SZ);
             } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c + (RUN ? r : 4 * r) < a.N) y[RUN ? r : 4 * r] = v[r];
+                for (int r = 0; r < 4; ++r) *(T*)(scratch + l15 * PITCH + (16 * n + M::row(r, kk)) * SZ) = v[r];
             }
         }
+        wave_lds_order();
+#pragma unroll
+        for (int i = 0; i < (16 * PER + 63) / 64; ++i) {
+            const int q = lane + 64 * i, row = q / PER, c = c0 + q % PER * E;
+            if (q >= 16 * PER || row0 + 16 * m + row >= row1 || c >= a.N) continue;
+            const char* from = scratch + row * PITCH + q % PER * 16;
+            T* y = (T*)a.y + (row0 + 16 * m + row) * a.ldy + c;
+            if (c + E <= a.N) {
+                const u32x4 v = *(const u32x4*)from;
+                __builtin_memcpy(y, &v, 16);
+            } else {
+                for (int j = 0; j < a.N - c; ++j) y[j] = *(const T*)(from + j * SZ);
+            }
+        }
+        wave_lds_order();
     }
 }
 
@@ -106,6 +127,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
     using Acc = typename M::Acc;
     constexpr int E = M::E, WAVES = 8, DEEP = MR == 1 ? 8 : MR == 2 ? 4 : 2;
     __shared__ Acc part[WAVES - 1][MR][64];
+    __shared__ __attribute__((aligned(16))) char scratch[put_scratch<T, 1>()];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
     const int c0 = (int)(blockIdx.x % tiles_n) * 16;
     int64_t r0, r1;
@@ -161,7 +183,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 #pragma unroll
         for (int m = 0; m < MR; ++m) acc[0][m] += part[i][m][lane];
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
-    put_tile<T, MR, 1>(a, r0, r1, c0, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc);
+    put_tile<T, MR, 1>(a, r0, r1, c0, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc, scratch);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -172,8 +194,9 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 //   k contiguous (x, and w [n, k]): rows of 8 pieces; place p of row r holds piece p ^ (r & 7)
 //   k strided (w [k, n]): lines of k (spread, strided_fragment)
 // The first `full` steps go by LDS-DMA, the rest -- a last step that ends inside a piece -- through registers.
-// LOW: 0 none; 1 tiles are spans of one segment, whose adapter joins in; 2 tiles of rows that lie together (short segments: a
-// span of a few rows would waste its tile).
+// LOW: 0 tiles are spans of one segment, with its matrix.  One matrix for all rows, tiles of rows that lie together, and the
+// adapters of the segments that a tile meets join in: 1 through LDS, a step for each; 2 straight from memory (add_adapters), for
+// segments shorter than a tile.
 // ------------------------------------------------------------------------------------------
 template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW>
 __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigned tiles_n, int ts, int full) {
@@ -184,6 +207,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     constexpr int LINE = TN * SZ / 16;                                                // pieces of a line of w [k, n]
     static_assert(TM * 8 % NT == 0 && TN * 8 % 64 == 0, "whole waves of pieces");
     __shared__ __attribute__((aligned(1024))) char lds[2 * (XB + WB)];
+    static_assert(WM * WN * put_scratch<T, NR>() <= 2 * (XB + WB), "put_tile's rows");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
     const unsigned id = die_order(blockIdx.x, gridDim.x);
@@ -193,11 +217,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 
     int64_t r0, r1;
     int slot = 0;
-    if (LOW != 2) {
+    if (LOW == 0) {
         const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, t, ts, &r0, &r1);
         if (s < 0) return;
         slot = seg_slot(a.sg, s);
-        if (slot < 0 && LOW == 0) return;
+        if (slot < 0) return;
     } else {
         r0 = seg_off(a.sg, 0) + t * TM;
         r1 = seg_off(a.sg, a.sg.S);
@@ -212,8 +236,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 #pragma unroll
         for (int m = 0; m < MR; ++m) acc[n][m] = Acc{0, 0, 0, 0};
 
-    // acc += X W' over the 128 bytes of k in buffer buf
-    auto multiply = [&](int buf) {
+    // acc += X W' over the 128 bytes of k in buffer buf; with SOME only for the rows from .. to - 1 of the wave's
+    auto multiply = [&](int buf, auto some, int from, int to) {
+        constexpr bool SOME = decltype(some)::value;
         const char* xs = lds + buf * (XB + WB);
         const char* ws = xs + XB;
 #pragma unroll
@@ -227,15 +252,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             }
 #pragma unroll
             for (int m = 0; m < MR; ++m) xf[m] = *(const u32x4*)(xs + (wm + 16 * m + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
+            if constexpr (!SOME) {
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
+                for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int m = 0; m < MR; ++m) acc[n][m] = M::mma(wf[n], xf[m], acc[n][m]);
+                    for (int m = 0; m < MR; ++m) acc[n][m] = M::mma(wf[n], xf[m], acc[n][m]);
+            } else
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                if (to <= 16 * m || from >= 16 * m + 16) continue;
+                if (from > 16 * m || to < 16 * m + 16) {
+                    // chosen, not masked by a product with zero: another row's adapter may hold a NaN
+                    const bool in = 16 * m + l15 >= from && 16 * m + l15 < to;
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        const Acc d = M::mma(wf[n], xf[m], acc[n][m]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) acc[n][m] = M::mma(wf[n], xf[m], acc[n][m]);
+                }
+            }
         }
     };
 
     // one step through registers: what lies past klen (or, in a line of w, past N) is 0
-    auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen) {
+    auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen, auto some, int from, int to) {
         u32x4 xr[XI], wr[WI];
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
@@ -260,7 +304,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         for (int i = 0; i < WI; ++i)
             if (brings_w(i)) *(u32x4*)(lds + XB + (tid + NT * i) * 16) = wr[i];
         __syncthreads();
-        multiply(0);
+        multiply(0, some, from, to);
         __syncthreads();
     };
 
@@ -299,20 +343,224 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         __syncthreads();
         for (int i = 0; i < full; ++i) {
             if (i + 1 < full) bring((i + 1) & 1);
-            multiply(i & 1);
+            multiply(i & 1, std::false_type{}, 0, 0);
             __syncthreads();
         }
     }
-    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K);
+    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, std::false_type{}, 0, 0);
 
-    if (LOW == 1 && slot >= 0) {
-        const T* low = (const T*)a.low + slot * a.low_stride;
-        for (int k0 = 0; k0 < a.R; k0 += KB) step((const T*)a.p + r0 * a.ldp, a.ldp, low, KN ? a.N : a.R, k0, a.R);
+    if (LOW == 1) {
+        const T* p = (const T*)a.p + r0 * a.ldp;
+        for (int s = max(0, wave_search(a.sg.S, r0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; ++s) {
+            const int64_t lo = seg_off(a.sg, s), hi = seg_off(a.sg, s + 1);
+            if (lo >= r1) break;
+            const int k = seg_slot(a.sg, s);
+            if (hi <= r0 || lo >= hi || k < 0) continue;
+            const T* low = (const T*)a.low + k * a.low_stride;
+            const int from = lo > r0 ? (int)(lo - r0) - wm : 0, to = hi < r1 ? (int)(hi - r0) - wm : TM;
+            for (int k0 = 0; k0 < a.R; k0 += KB) step(p, a.ldp, low, KN ? a.N : a.R, k0, a.R, std::true_type{}, from, to);
+        }
     }
     if (LOW == 2) add_adapters<T, KN, MR, NR>(a, r0 + wm, r1, n0 + wn, 0, 1, acc);
 
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
-    put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc);
+    put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
+                        lds + wave * put_scratch<T, NR>());
+}
+
+// ------------------------------------------------------------------------------------------
+// The same for 16-bit types and wide matrices: 256 x 256 results, eight waves of 128 x 64, steps of 32 k through four LDS buffers.
+// While a step multiplies, the fragments of the next one are read (a register set each), the one after that has arrived or is
+// about to, and the third is being asked for: the matrix cores, the LDS and the memory each work a step apart, with one barrier
+// a step and a wait that counts (only the newest four requests may be out).  With a step's reads before its products instead
+// (rows_tile at this size) the two took turns: 638 us against XX us for 65,536 x 2048 x 2048.
+// Rows of 64 bytes, four to a turn of the banks: place p of row r holds piece p ^ (-(r / 4) & 3).  A 16-byte read serves lanes 0 - 3,
+// 12 - 15, 20 - 23, 24 - 27 together, then 4 - 11, 16 - 19, 28 - 31 and so on: all sixteen rows, the middle eight of the next piece.
+// ------------------------------------------------------------------------------------------
+template <typename T, bool KN, int LOW>
+__global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_n, int ts, int full) {
+    using M = Mat<T>;
+    using Acc = typename M::Acc;
+    constexpr int SZ = 2, E = 8, KB = 32, NT = 512, MR = 8, NR = 4, TM = 256, TN = 256, HALF = TM * KB * SZ, LINE = TN * SZ / 16;
+    static_assert(sizeof(T) == 2, "16-bit types");
+    // (four variables, not one array: the compiler then knows that reading one does not wait for what is brought into another)
+    __shared__ __attribute__((aligned(1024))) char b0[2 * HALF], b1[2 * HALF], b2[2 * HALF], b3[2 * HALF];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
+    const int wm = wave / 4 * 128, wn = wave % 4 * 64;
+    const unsigned id = die_order(blockIdx.x, gridDim.x);
+    const int n0 = (int)(id % tiles_n) * TN;
+    const int64_t t = id / tiles_n;
+    int64_t r0, r1;
+    int slot = 0;
+    if (LOW == 0) {
+        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, t, ts, &r0, &r1);
+        if (s < 0) return;
+        slot = seg_slot(a.sg, s);
+        if (slot < 0) return;
+    } else {
+        r0 = seg_off(a.sg, 0) + t * TM;
+        r1 = seg_off(a.sg, a.sg.S);
+        if (r1 > r0 + TM) r1 = r0 + TM;
+        if (r0 >= r1) return;
+    }
+    const int nrow = (int)(r1 - r0);
+
+    Acc acc[NR][MR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) acc[n][m] = Acc{0, 0, 0, 0};
+    struct Frags {
+        u32x4 x[MR], w[NR];
+    };
+    auto read = [&](const char* buf, Frags& f) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const int c = wn + 16 * n;
+            if constexpr (KN) f.w[n] = strided_fragment<T, TN>(buf + HALF, 0, c);
+            else f.w[n] = *(const u32x4*)(buf + HALF + (c + l15) * 64 + ((kk ^ (-(l15 >> 2) & 3)) << 4));
+        }
+#pragma unroll
+        for (int m = 0; m < MR; ++m) f.x[m] = *(const u32x4*)(buf + (wm + 16 * m + l15) * 64 + ((kk ^ (-(l15 >> 2) & 3)) << 4));
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int m = 0; m < MR; ++m) acc[n][m] = M::mma(f.w[n], f.x[m], acc[n][m]);
+    };
+    // rows from .. to - 1 of the wave's only
+    auto multiply_some = [&](const Frags& f, int from, int to) {
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            if (to <= 16 * m || from >= 16 * m + 16) continue;
+            if (from > 16 * m || to < 16 * m + 16) {
+                // chosen, not masked by a product with zero: another row's adapter may hold a NaN
+                const bool in = 16 * m + l15 >= from && 16 * m + l15 < to;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    const Acc d = M::mma(f.w[n], f.x[m], acc[n][m]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NR; ++n) acc[n][m] = M::mma(f.w[n], f.x[m], acc[n][m]);
+            }
+        }
+    };
+    const T* x = (const T*)a.x + r0 * a.ldx;
+    const T* w = (const T*)a.w + (LOW ? 0 : slot * a.w_stride);
+    const int64_t ldw = KN ? a.N : a.K;
+    if (full > 0) {
+        unsigned xo[2], wo[2];
+        const int xk = ((tid ^ -(tid >> 4)) & 3) * 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) xo[i] = (unsigned)min((tid + NT * i) >> 2, nrow - 1) * (unsigned)(a.ldx * SZ) + xk;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int q = tid + NT * i;
+            if (KN) {
+                const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
+                wo[i] = n0 + c < a.N ? (unsigned)k * (unsigned)(ldw * SZ) + c * SZ : 0xffffffffu;
+            } else {
+                wo[i] = (unsigned)min(q >> 2, a.N - 1 - n0) * (unsigned)(ldw * SZ) + xk;
+            }
+        }
+        const char* xb = (const char*)x;
+        const char* wb = (const char*)(KN ? w + n0 : w + (int64_t)n0 * ldw);
+        auto bring = [&](char* buf) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) bring_piece(xb, xo[i], buf + (wave * 64 + NT * i) * 16);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) bring_piece(wb, wo[i], buf + HALF + (wave * 64 + NT * i) * 16);
+            xb += KB * SZ;
+            wb += KN ? KB * ldw * SZ : KB * SZ;
+        };
+        // s_waitcnt vmcnt(n), the other counters free
+        constexpr int VM0 = 0x0f70, VM4 = 0x0f74, VM8 = 0x0f78;
+        bring(b0);
+        if (full > 1) bring(b1);
+        if (full > 2) bring(b2);
+        if (full > 2) __builtin_amdgcn_s_waitcnt(VM8);
+        else if (full > 1) __builtin_amdgcn_s_waitcnt(VM4);
+        else __builtin_amdgcn_s_waitcnt(VM0);
+        __builtin_amdgcn_s_barrier();
+        Frags f0, f1;
+        read(b0, f0);
+        // at the barrier the step after this one has arrived for every wave, and every wave is done reading the buffer it frees
+        auto run = [&](Frags& now, Frags& next, const char* arrived, char* free) {
+            __builtin_amdgcn_s_waitcnt(VM4);
+            __builtin_amdgcn_s_barrier();
+            bring(free);
+            read(arrived, next);
+            multiply(now);
+        };
+        auto turn = [&](int i, Frags& now, Frags& next, const char* arrived, char* free) {
+            if (i + 2 < full) __builtin_amdgcn_s_waitcnt(VM4);
+            else __builtin_amdgcn_s_waitcnt(VM0);
+            __builtin_amdgcn_s_barrier();
+            if (i + 3 < full) bring(free);
+            if (i + 1 < full) read(arrived, next);
+            multiply(now);
+        };
+        int i = 0;
+        for (; i + 6 < full; i += 4) {                                                // (no branches: the waits can be told apart)
+            run(f0, f1, b1, b3);
+            run(f1, f0, b2, b0);
+            run(f0, f1, b3, b1);
+            run(f1, f0, b0, b2);
+        }
+        for (; i < full; i += 4) {
+            turn(i, f0, f1, b1, b3);
+            if (i + 1 < full) turn(i + 1, f1, f0, b2, b0);
+            if (i + 2 < full) turn(i + 2, f0, f1, b3, b1);
+            if (i + 3 < full) turn(i + 3, f1, f0, b0, b2);
+        }
+        __syncthreads();
+    }
+    // one step through registers: what lies past klen (or, in a line of w, past N) is 0
+    auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen, bool some, int from, int to) {
+        u32x4 xr[2], wr[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int q = tid + NT * i, row = q >> 2;
+            xr[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ -(row >> 2)) & 3) * E, klen);
+            if (KN) {
+                const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
+                wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
+            } else {
+                wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ -(row >> 2)) & 3) * E, klen);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            *(u32x4*)(b0 + (tid + NT * i) * 16) = xr[i];
+            *(u32x4*)(b0 + HALF + (tid + NT * i) * 16) = wr[i];
+        }
+        __syncthreads();
+        Frags f;
+        read(b0, f);
+        if (some) multiply_some(f, from, to);
+        else multiply(f);
+        __syncthreads();
+    };
+    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, false, 0, 0);
+    if (LOW == 1) {
+        const T* p = (const T*)a.p + r0 * a.ldp;
+        for (int s = max(0, wave_search(a.sg.S, r0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; ++s) {
+            const int64_t lo = seg_off(a.sg, s), hi = seg_off(a.sg, s + 1);
+            if (lo >= r1) break;
+            const int k = seg_slot(a.sg, s);
+            if (hi <= r0 || lo >= hi || k < 0) continue;
+            const T* low = (const T*)a.low + k * a.low_stride;
+            const int from = lo > r0 ? (int)(lo - r0) - wm : 0, to = hi < r1 ? (int)(hi - r0) - wm : TM;
+            for (int k0 = 0; k0 < a.R; k0 += KB) step(p, a.ldp, low, KN ? a.N : a.R, k0, a.R, true, from, to);
+        }
+    }
+    const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
+    put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
+                        (wave < 4 ? b0 : b1) + wave % 4 * put_scratch<T, NR>());
 }
 
 constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
@@ -321,7 +569,7 @@ template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW>
 static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     static_assert(TM == 1 << log2_of(TM), "tile heights");
     constexpr int KB = 128 / (int)sizeof(T), E = Mat<T>::E;
-    const int64_t tiles_n = (a.N + TN - 1) / TN, tiles_m = LOW != 2 ? a.sg.rows / TM + a.sg.S : (a.sg.rows + TM - 1) / TM;
+    const int64_t tiles_n = (a.N + TN - 1) / TN, tiles_m = LOW == 0 ? a.sg.rows / TM + a.sg.S : (a.sg.rows + TM - 1) / TM;
     LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
     // Steps for the LDS-DMA: whole ones; not the last line of w [k, n] where a piece would run past its end (elsewhere it runs
     // into the next line); none where a tile's offsets pass 31 bits
@@ -330,6 +578,16 @@ static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     if (a.ldx * TM * (int64_t)sizeof(T) >= (1ll << 31) || ldw * std::max(TN, KB) * (int64_t)sizeof(T) >= (1ll << 31)) full = 0;
     LN_LAUNCH(ctx, name, (rows_tile<T, TM, TN, WM, WN, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(64 * WM * WN), 0, a,
               (unsigned)tiles_n, log2_of(TM), full);
+    return 0;
+}
+
+template <typename T, bool KN, int LOW>
+static int launch_deep(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
+    const int64_t tiles_n = (a.N + 255) / 256, tiles_m = LOW == 0 ? a.sg.rows / 256 + a.sg.S : (a.sg.rows + 255) / 256;
+    LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
+    int full = KN && a.N % 8 ? (a.K - 1) / 32 : a.K / 32;                             // as in launch_tile
+    if (a.ldx * 512 >= (1ll << 31) || (KN ? a.N : a.K) * 512ll >= (1ll << 31)) full = 0;
+    LN_LAUNCH(ctx, name, (rows_deep<T, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_n, 8, full);
     return 0;
 }
 
@@ -350,7 +608,7 @@ static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         if (a.N <= 48) return launch_tile<T, 128, 48, 4, 1, KN, LOW>(ctx, a, name);
         if (a.N <= 64) return launch_tile<T, 128, 64, 4, 1, KN, LOW>(ctx, a, name);
         if constexpr (sizeof(T) == 2)
-            if (rows / 256 * (a.N / 256) >= cus) return launch_tile<T, 256, 256, 2, 4, KN, LOW>(ctx, a, name);
+            if (rows / 256 * (a.N / 256) >= cus) return launch_deep<T, KN, LOW>(ctx, a, name);
         constexpr int WN = sizeof(T) == 8 ? 4 : 2;
         if ((rows / 128 + a.sg.S) * ((a.N + 127) / 128) >= 4 * cus) return launch_tile<T, 128, 128, 2, WN, KN, LOW>(ctx, a, name);
     }
