@@ -147,6 +147,13 @@ __device__ __forceinline__ unsigned die_order(unsigned id, unsigned total) {
     return die * per + min(die, rest) + at;
 }
 
+// Tile number -> (m, n): eight tiles of n beside each other before the next of m, so that the tiles a die works on at a time share
+// rows and columns about evenly
+__device__ __forceinline__ void tile_order(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned* m, unsigned* n) {
+    const unsigned group = id / (8 * tiles_m), wide = min(8u, tiles_n - 8 * group), at = id - group * 8 * tiles_m;
+    *m = at / wide;
+    *n = 8 * group + at % wide;
+}
 // 16 bytes a lane from base + offset to LDS at `to` (wave-uniform) + 16 * lane; zeros where offset >= 2^31
 __device__ __forceinline__ void bring_piece(const char* base, unsigned offset, char* to) {
     const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x80000000u, 0x00027000);

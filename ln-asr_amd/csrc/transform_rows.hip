@@ -369,36 +369,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 }
 
 // ------------------------------------------------------------------------------------------
-// The same for 16-bit types and wide matrices: 256 x 256 results, eight waves of 128 x 64, steps of 32 k through four LDS buffers.
-// While a step multiplies, the fragments of the next one are read (a register set each), the one after that has arrived or is
-// about to, and the third is being asked for: the matrix cores, the LDS and the memory each work a step apart, with one barrier
-// a step and a wait that counts (only the newest four requests may be out).  With a step's reads before its products instead
-// (rows_tile at this size) the two took turns: 638 us against XX us for 65,536 x 2048 x 2048.
-// Rows of 64 bytes, four to a turn of the banks: place p of row r holds piece p ^ (-(r / 4) & 3).  A 16-byte read serves lanes 0 - 3,
-// 12 - 15, 20 - 23, 24 - 27 together, then 4 - 11, 16 - 19, 28 - 31 and so on: all sixteen rows, the middle eight of the next piece.
+// The same for 16-bit types and wide matrices: 256 x 256 results, eight waves of 128 x 64, steps of 64 k through a ring of five LDS
+// buffers of 32 KB (x and w of a step take two).  While half a step multiplies, the fragments of the next half are read; w of the
+// step after next and x of the one behind it are asked for in the middle of each step, where its own buffers fall free: the matrix
+// cores, the LDS and the memory each work ahead of one another, with one barrier a step and a wait that counts (the newest four
+// requests, x of the step after next, may be out).
 // ------------------------------------------------------------------------------------------
 template <typename T, bool KN, int LOW>
-__global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_n, int ts, int full) {
+__global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m, unsigned tiles_n, int full) {
     using M = Mat<T>;
     using Acc = typename M::Acc;
-    constexpr int SZ = 2, E = 8, KB = 32, NT = 512, MR = 8, NR = 4, TM = 256, TN = 256, HALF = TM * KB * SZ, LINE = TN * SZ / 16;
+    constexpr int SZ = 2, E = 8, KB = 64, NT = 512, MR = 8, NR = 4, TM = 256, TN = 256, LINE = TN * SZ / 16;
     static_assert(sizeof(T) == 2, "16-bit types");
-    // (four variables, not one array: the compiler then knows that reading one does not wait for what is brought into another)
-    __shared__ __attribute__((aligned(1024))) char b0[2 * HALF], b1[2 * HALF], b2[2 * HALF], b3[2 * HALF];
+    // (five variables, not one array: the compiler then knows that reading one does not wait for what is brought into another)
+    __shared__ __attribute__((aligned(1024))) char u0[TM * 128], u1[TM * 128], u2[TM * 128], u3[TM * 128], u4[TM * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / 4 * 128, wn = wave % 4 * 64;
-    const unsigned id = die_order(blockIdx.x, gridDim.x);
-    const int n0 = (int)(id % tiles_n) * TN;
-    const int64_t t = id / tiles_n;
+    unsigned tm, tn;
+    tile_order(die_order(blockIdx.x, gridDim.x), tiles_m, tiles_n, &tm, &tn);
+    const int n0 = (int)tn * TN;
     int64_t r0, r1;
     int slot = 0;
     if (LOW == 0) {
-        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, t, ts, &r0, &r1);
+        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, tm, 8, &r0, &r1);
         if (s < 0) return;
         slot = seg_slot(a.sg, s);
         if (slot < 0) return;
     } else {
-        r0 = seg_off(a.sg, 0) + t * TM;
+        r0 = seg_off(a.sg, 0) + (int64_t)tm * TM;
         r1 = seg_off(a.sg, a.sg.S);
         if (r1 > r0 + TM) r1 = r0 + TM;
         if (r0 >= r1) return;
@@ -413,21 +411,22 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_n
     struct Frags {
         u32x4 x[MR], w[NR];
     };
-    auto read = [&](const char* buf, Frags& f) {
+    auto read = [&](const char* xs, const char* ws, int h, Frags& f) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const int c = wn + 16 * n;
-            if constexpr (KN) f.w[n] = strided_fragment<T, TN>(buf + HALF, 0, c);
-            else f.w[n] = *(const u32x4*)(buf + HALF + (c + l15) * 64 + ((kk ^ (-(l15 >> 2) & 3)) << 4));
+            if constexpr (KN) f.w[n] = strided_fragment<T, TN>(ws, h, c);
+            else f.w[n] = *(const u32x4*)(ws + (c + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
         }
 #pragma unroll
-        for (int m = 0; m < MR; ++m) f.x[m] = *(const u32x4*)(buf + (wm + 16 * m + l15) * 64 + ((kk ^ (-(l15 >> 2) & 3)) << 4));
+        for (int m = 0; m < MR; ++m) f.x[m] = *(const u32x4*)(xs + (wm + 16 * m + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
     };
+    // (a fragment of x meets its four of w and is done with: the next one can take its registers)
     auto multiply = [&](const Frags& f) {
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
+        for (int m = 0; m < MR; ++m)
 #pragma unroll
-            for (int m = 0; m < MR; ++m) acc[n][m] = M::mma(f.w[n], f.x[m], acc[n][m]);
+            for (int n = 0; n < NR; ++n) acc[n][m] = M::mma(f.w[n], f.x[m], acc[n][m]);
     };
     // rows from .. to - 1 of the wave's only
     auto multiply_some = [&](const Frags& f, int from, int to) {
@@ -453,96 +452,136 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_n
     const T* w = (const T*)a.w + (LOW ? 0 : slot * a.w_stride);
     const int64_t ldw = KN ? a.N : a.K;
     if (full > 0) {
-        unsigned xo[2], wo[2];
-        const int xk = ((tid ^ -(tid >> 4)) & 3) * 16;
+        unsigned xo[4], wo[4];
+        const int xk = ((tid ^ tid >> 3) & 7) * 16;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) xo[i] = (unsigned)min((tid + NT * i) >> 2, nrow - 1) * (unsigned)(a.ldx * SZ) + xk;
+        for (int i = 0; i < 4; ++i) xo[i] = (unsigned)min((tid + NT * i) >> 3, nrow - 1) * (unsigned)(a.ldx * SZ) + xk;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const int q = tid + NT * i;
             if (KN) {
                 const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
                 wo[i] = n0 + c < a.N ? (unsigned)k * (unsigned)(ldw * SZ) + c * SZ : 0xffffffffu;
             } else {
-                wo[i] = (unsigned)min(q >> 2, a.N - 1 - n0) * (unsigned)(ldw * SZ) + xk;
+                wo[i] = (unsigned)min(q >> 3, a.N - 1 - n0) * (unsigned)(ldw * SZ) + xk;
             }
         }
         const char* xb = (const char*)x;
         const char* wb = (const char*)(KN ? w + n0 : w + (int64_t)n0 * ldw);
-        auto bring = [&](char* buf) {
+        auto bring_x = [&](char* u) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) bring_piece(xb, xo[i], buf + (wave * 64 + NT * i) * 16);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) bring_piece(wb, wo[i], buf + HALF + (wave * 64 + NT * i) * 16);
+            for (int i = 0; i < 4; ++i) bring_piece(xb, xo[i], u + (wave * 64 + NT * i) * 16);
             xb += KB * SZ;
+        };
+        auto bring_w = [&](char* u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bring_piece(wb, wo[i], u + (wave * 64 + NT * i) * 16);
             wb += KN ? KB * ldw * SZ : KB * SZ;
         };
-        // s_waitcnt vmcnt(n), the other counters free
-        constexpr int VM0 = 0x0f70, VM4 = 0x0f74, VM8 = 0x0f78;
-        bring(b0);
-        if (full > 1) bring(b1);
-        if (full > 2) bring(b2);
-        if (full > 2) __builtin_amdgcn_s_waitcnt(VM8);
-        else if (full > 1) __builtin_amdgcn_s_waitcnt(VM4);
-        else __builtin_amdgcn_s_waitcnt(VM0);
+        constexpr int VM0 = 0x0f70, VM4 = 0x0f74;                                     // s_waitcnt vmcnt(n), the other counters free
+        bring_x(u0);
+        bring_w(u1);
+        if (full > 1) {
+            bring_x(u2);
+            bring_w(u3);
+        }
+        if (full > 2) bring_x(u4);
+        __builtin_amdgcn_s_waitcnt(VM0);
         __builtin_amdgcn_s_barrier();
         Frags f0, f1;
-        read(b0, f0);
-        // at the barrier the step after this one has arrived for every wave, and every wave is done reading the buffer it frees
-        auto run = [&](Frags& now, Frags& next, const char* arrived, char* free) {
-            __builtin_amdgcn_s_waitcnt(VM4);
+        read(u0, u1, 0, f0);
+        // One step: its x and w in xs, ws; the next one's in xn, wn.  At the barrier the next step has arrived for every wave, and
+        // every wave has read all of this one, whose buffers take w of the step after next and x of the one behind.
+        auto run = [&](char* xs, char* ws, const char* xn, const char* wn_) {
+            auto interleave = [&]() {                                                 // a read behind every two or three products
+                if constexpr (KN) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            read(xs, ws, 1, f1);
+            multiply(f0);
+            interleave();
+            __builtin_amdgcn_s_waitcnt(VM4 & 0xf0ff);                                 // vmcnt(4) lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
-            bring(free);
-            read(arrived, next);
-            multiply(now);
+            __builtin_amdgcn_sched_barrier(0);
+            bring_w(xs);
+            bring_x(ws);
+            read(xn, wn_, 0, f0);
+            multiply(f1);
+            __builtin_amdgcn_sched_group_barrier(0x020, 8, 0);
+            interleave();
         };
-        auto turn = [&](int i, Frags& now, Frags& next, const char* arrived, char* free) {
-            if (i + 2 < full) __builtin_amdgcn_s_waitcnt(VM4);
-            else __builtin_amdgcn_s_waitcnt(VM0);
+        auto turn = [&](int s, char* xs, char* ws, const char* xn, const char* wn_) {
+            read(xs, ws, 1, f1);
+            multiply(f0);
+            __builtin_amdgcn_s_waitcnt(VM0 & 0xf0ff);
             __builtin_amdgcn_s_barrier();
-            if (i + 3 < full) bring(free);
-            if (i + 1 < full) read(arrived, next);
-            multiply(now);
+            if (s + 2 < full) bring_w(xs);
+            if (s + 3 < full) bring_x(ws);
+            if (s + 1 < full) read(xn, wn_, 0, f0);
+            multiply(f1);
         };
-        int i = 0;
-        for (; i + 6 < full; i += 4) {                                                // (no branches: the waits can be told apart)
-            run(f0, f1, b1, b3);
-            run(f1, f0, b2, b0);
-            run(f0, f1, b3, b1);
-            run(f1, f0, b0, b2);
+        int s = 0;
+        for (; s + 8 <= full; s += 5) {
+            run(u0, u1, u2, u3);
+            run(u2, u3, u4, u0);
+            run(u4, u0, u1, u2);
+            run(u1, u2, u3, u4);
+            run(u3, u4, u0, u1);
         }
-        for (; i < full; i += 4) {
-            turn(i, f0, f1, b1, b3);
-            if (i + 1 < full) turn(i + 1, f1, f0, b2, b0);
-            if (i + 2 < full) turn(i + 2, f0, f1, b3, b1);
-            if (i + 3 < full) turn(i + 3, f1, f0, b0, b2);
+        for (; s < full; s += 5) {
+            turn(s, u0, u1, u2, u3);
+            if (s + 1 < full) turn(s + 1, u2, u3, u4, u0);
+            if (s + 2 < full) turn(s + 2, u4, u0, u1, u2);
+            if (s + 3 < full) turn(s + 3, u1, u2, u3, u4);
+            if (s + 4 < full) turn(s + 4, u3, u4, u0, u1);
         }
         __syncthreads();
     }
     // one step through registers: what lies past klen (or, in a line of w, past N) is 0
     auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen, bool some, int from, int to) {
-        u32x4 xr[2], wr[2];
+        u32x4 xr[4], wr[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int q = tid + NT * i, row = q >> 2;
-            xr[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ -(row >> 2)) & 3) * E, klen);
+        for (int i = 0; i < 4; ++i) {
+            const int q = tid + NT * i, row = q >> 3;
+            xr[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ row) & 7) * E, klen);
             if (KN) {
                 const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
                 wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
             } else {
-                wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ -(row >> 2)) & 3) * E, klen);
+                wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            *(u32x4*)(b0 + (tid + NT * i) * 16) = xr[i];
-            *(u32x4*)(b0 + HALF + (tid + NT * i) * 16) = wr[i];
+        for (int i = 0; i < 4; ++i) {
+            *(u32x4*)(u0 + (tid + NT * i) * 16) = xr[i];
+            *(u32x4*)(u1 + (tid + NT * i) * 16) = wr[i];
         }
         __syncthreads();
-        Frags f;
-        read(b0, f);
-        if (some) multiply_some(f, from, to);
-        else multiply(f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h && klen - k0 <= KB / 2) break;
+            Frags f;
+            read(u0, u1, h, f);
+            if (some) multiply_some(f, from, to);
+            else multiply(f);
+        }
         __syncthreads();
     };
     for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, false, 0, 0);
@@ -560,7 +599,7 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_n
     }
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
     put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
-                        (wave < 4 ? b0 : b1) + wave % 4 * put_scratch<T, NR>());
+                        (wave < 4 ? u0 : u1) + wave % 4 * put_scratch<T, NR>());
 }
 
 constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
@@ -585,9 +624,9 @@ template <typename T, bool KN, int LOW>
 static int launch_deep(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t tiles_n = (a.N + 255) / 256, tiles_m = LOW == 0 ? a.sg.rows / 256 + a.sg.S : (a.sg.rows + 255) / 256;
     LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
-    int full = KN && a.N % 8 ? (a.K - 1) / 32 : a.K / 32;                             // as in launch_tile
+    int full = KN && a.N % 8 ? (a.K - 1) / 64 : a.K / 64;                             // as in launch_tile
     if (a.ldx * 512 >= (1ll << 31) || (KN ? a.N : a.K) * 512ll >= (1ll << 31)) full = 0;
-    LN_LAUNCH(ctx, name, (rows_deep<T, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_n, 8, full);
+    LN_LAUNCH(ctx, name, (rows_deep<T, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_m, (unsigned)tiles_n, full);
     return 0;
 }
 
