@@ -11,6 +11,7 @@ typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // One 16 x 16 block of a product by the matrix cores.  Every type moves in pieces of 16 bytes: lane l of the wave holds, for
@@ -182,11 +183,10 @@ __device__ __forceinline__ u32x4 strided_fragment(const char* tile, int h, int c
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4 lds16x4;
         const int k = 32 * h + 8 * kk + (l15 >> 2);
-        const char* at = tile + k * (C * 2) + (((c / 16) ^ spread<T, C>(k)) << 5) + (l15 & 3) * 8;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)at);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(at + 4 * (C * 2)));    // spread(k + 4) == spread(k)
-        __builtin_memcpy(&f, &lo, 8);
-        __builtin_memcpy((char*)&f + 8, &hi, 8);
+        const int at = k * (C * 2) + (((c / 16) ^ spread<T, C>(k)) << 5) + (l15 & 3) * 8;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(tile + at)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(tile + (at + 4 * (C * 2)))));    // spread(k + 4) == spread(k)
+        f = u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
         T e[E];
 #pragma unroll
@@ -221,6 +221,8 @@ struct SumArgs {
     const int64_t* group_off;   // group g: places group_off[g * group_step] .. group_off[(g + 1) * group_step] of `rowmap`
     int64_t group_step;         // 1; S: all segments as one group
     const int64_t* rowmap;      // row at each place of the sorted order, or null: the rows as they lie
+    const int64_t* place;       // [S + 1] (with rowmap) places of the sorted segments' rows
+    const int* ord;             // [S] the sorted segments
     const void *a, *b;
     void *out, *cols;
     int64_t lda, ldb;
@@ -234,8 +236,8 @@ bool sum_narrow_ok(const SumArgs& a);
 int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
 // out and cols from the sums of the spans of 2^ts rows
 int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const void* parts, const void* col_parts);
-// Sorts the segments by group (stable): *group_off [G + 1], *rowmap [rows].  Without slots both are the segments' own.
-int transform_sort(lnasr_ctx* ctx, const Segments& sg, const int64_t** group_off, const int64_t** rowmap);
+// Sorts the segments by group (stable): group_off, rowmap, place, ord of a.  Without slots the rows are sorted as they lie.
+int transform_sort(lnasr_ctx* ctx, SumArgs* a);
 
 // Workspace `i` of the feature transforms with room for `bytes`
 int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out);

@@ -99,6 +99,56 @@ __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes
     for (int g = last + 1 + tid; g <= sg.G; g += kSortNT) group_off[g] = total;
 }
 
+// The same for up to 1024 segments in one kernel with the rows' places: every block finds all of them -- thread i counts the segments
+// that come before segment i (a smaller group, or the same and earlier) and their rows -- and writes the rows of some.
+__global__ __launch_bounds__(kSortNT) void sort_few_segments(Segments sg, int* ord, int64_t* place, int64_t* group_off, int64_t* rowmap) {
+    __shared__ int keys[kSortNT];
+    __shared__ int64_t lens[kSortNT], first[kSortNT], at[kSortNT];
+    const int tid = threadIdx.x;
+    int k = sg.G;
+    int64_t len = 0, from = 0;
+    if (tid < sg.S) {
+        from = seg_off(sg, tid);
+        k = seg_slot(sg, tid);
+        if (k < 0) k = sg.G;
+        len = k < sg.G ? max((int64_t)0, seg_off(sg, tid + 1) - from) : 0;
+    }
+    keys[tid] = k;
+    lens[tid] = len;
+    first[tid] = from;
+    __syncthreads();
+    int64_t before = 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < sg.S; ++j) {
+        const bool first = keys[j] < k || (keys[j] == k && j < tid);
+        before += first ? lens[j] : 0;
+        rank += first ? 1 : 0;
+    }
+    before = min(before, sg.rows);
+    at[tid] = before;
+    if (blockIdx.x == 0) {
+        __shared__ int sorted[kSortNT];
+        if (tid < sg.S) {
+            ord[rank] = tid;
+            place[rank] = before;
+            sorted[rank] = k;
+            if (rank == sg.S - 1) place[sg.S] = min(before + len, sg.rows);
+        }
+        __syncthreads();
+        // a group begins where the first segment of it, or of a later one, lies; those behind the last segment's, at the end
+        if (tid < sg.S) {
+            for (int g = rank ? sorted[rank - 1] + 1 : 0; g <= k; ++g) group_off[g] = before;
+            if (rank == sg.S - 1)
+                for (int g = k + 1; g <= sg.G; ++g) group_off[g] = min(before + len, sg.rows);
+        }
+    }
+    __syncthreads();
+    for (int s = blockIdx.x * 4 + (tid >> 8); s < sg.S; s += gridDim.x * 4)
+        for (int64_t i = tid & 255; i < lens[s]; i += 256)
+            if (at[s] + i < sg.rows) rowmap[at[s] + i] = first[s] + i;
+}
+
 // the row at each place of the sorted order
 __global__ __launch_bounds__(256) void map_rows(Segments sg, const int* ord, const int64_t* place, int64_t* rowmap) {
     const int64_t q0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64, total = place[sg.S];
@@ -112,10 +162,12 @@ __global__ __launch_bounds__(256) void map_rows(Segments sg, const int* ord, con
     rowmap[q] = row < sg.rows ? row : sg.rows - 1;
 }
 
-int transform_sort(lnasr_ctx* ctx, const Segments& sg, const int64_t** group_off, const int64_t** rowmap) {
+int transform_sort(lnasr_ctx* ctx, SumArgs* a) {
+    const Segments& sg = a->sg;
+    a->rowmap = a->place = nullptr;
+    a->ord = nullptr;
     if (!sg.slots) {
-        *group_off = sg.off;
-        *rowmap = nullptr;
+        a->group_off = sg.off;
         return 0;
     }
     void* p;
@@ -124,54 +176,104 @@ int transform_sort(lnasr_ctx* ctx, const Segments& sg, const int64_t** group_off
     int64_t* place = map + sg.rows;
     int64_t* goff = place + sg.S + 1;
     int* ord0 = (int*)(goff + sg.G + 1);
+    a->group_off = goff;
+    a->rowmap = map;
+    a->place = place;
+    a->ord = ord0;
+    if (sg.S <= kSortNT) {
+        LN_LAUNCH(ctx, "sort_few_segments", sort_few_segments, dim3((unsigned)std::min((sg.S + 3) / 4, 64)), dim3(kSortNT), 0, sg, ord0, place, goff,
+                  map);
+        return 0;
+    }
     int passes = 1;
     while (passes < 4 && (sg.G >> (8 * passes)) > 0) ++passes;
     LN_LAUNCH(ctx, "sort_segments", sort_segments, dim3(1), dim3(kSortNT), 0, sg, passes, ord0, ord0 + sg.S, place, goff);
     LN_LAUNCH(ctx, "map_rows", map_rows, dim3((unsigned)((sg.rows + 255) / 256)), dim3(256), 0, sg, ord0, place, map);
-    *group_off = goff;
-    *rowmap = map;
     return 0;
+}
+
+// Span t of 2^ts places of the sorted rows: its group, first place and rows; false: nothing to do.  (A group without rows has one
+// span without rows, to be written as zeros.)
+__device__ __forceinline__ bool sum_span(const SumArgs& a, int64_t t, int ts, int* group, int64_t* q0, int* n, bool* whole) {
+    auto clamped = [&](int g) {
+        const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
+        return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
+    };
+    const int g = wave_search(a.groups, t, [&](int i) { return (clamped(i) >> ts) + i; });
+    if (g < 0) return false;
+    const int64_t go = clamped(g), ge = max(go, clamped(g + 1)), span = t - ((go >> ts) + g);
+    *group = g;
+    *q0 = go + (span << ts);
+    if (span > 0 && *q0 >= ge) return false;
+    *n = (int)min(ge - *q0, (int64_t)1 << ts);
+    *whole = go + (1ll << ts) >= ge;
+    return true;
+}
+// Of up to 64 spans the t-th longest: blocks start in the order of their numbers, and the longest ones are to start first
+__device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int64_t t, int ts) {
+    const int lane = threadIdx.x & 63;
+    int64_t n = -1;                           // rows of span `lane`, -1: none such
+    for (int g = 0; g < a.groups; ++g) {
+        auto at = [&](int i) {
+            const int64_t o = a.sg.S ? a.group_off[i * a.group_step] : 0;
+            return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
+        };
+        const int64_t go = at(g), ge = at(g + 1), q = go + ((lane - ((go >> ts) + g)) << ts);
+        if (lane >= (go >> ts) + g) n = q < ge ? min(ge - q, (int64_t)1 << ts) : 0;
+    }
+    int rank = 0;
+    for (int j = 0; j < spans; ++j) {
+        const int64_t other = __shfl(n, j);
+        rank += other > n || (other == n && j < lane) ? 1 : 0;
+    }
+    const uint64_t mine = __ballot(lane < spans && rank == (int)t);
+    return mine ? __builtin_ctzll(mine) : t;
+}
+// The rows that lie together from place q of the sorted rows on, at most up to place end: calls each(first row, rows) run by run
+template <typename F>
+__device__ __forceinline__ void each_run(const SumArgs& a, int64_t q, int64_t end, F each) {
+    int i = a.rowmap ? max(0, wave_search(a.sg.S, q, [&](int j) { return a.place[j]; })) : 0;
+    while (q < end) {                                     // (one call of `each`: it is a kernel's whole loop)
+        int64_t row = q, to = end;
+        if (a.rowmap) {
+            while (i < a.sg.S && a.place[i + 1] <= q) ++i;
+            if (i >= a.sg.S) return;
+            to = min(a.place[i + 1], end);
+            row = seg_off(a.sg, a.ord[i]) + (q - a.place[i]);
+        }
+        each(row, (int)(to - q));
+        q = to;
+    }
 }
 
 // ------------------------------------------------------------------------------------------
 // Tiles of TI x TJ results of one group, WI x WJ waves, summed over a span of the group's rows.  The rows are the k of the product,
-// strided for both operands: they lie in LDS as lines (strided_fragment).  FROM: 0 through registers; where both operands are made
-// of whole aligned 16-byte pieces by LDS-DMA, 1 from rows that lie together (a running base, fixed offsets), 2 from the rows
-// that rowmap names.  A group with one span is written at once, the others leave sums of 32
+// strided for both operands: they lie in LDS as lines (strided_fragment).  TOGETHER: rows that lie together (a segment's) come by
+// LDS-DMA step by step, the last and uneven one through registers; otherwise -- segments of a few rows -- all of them through
+// registers, row by row as rowmap says, loaded a step ahead.  A group with one span is written at once, the others leave sums of 32
 // bits or more per span, which join_parts adds in the order of the spans.
 // ------------------------------------------------------------------------------------------
-__device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
-
-__device__ __forceinline__ void bring_from(const char* from, char* to) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-}
-
-template <typename T, int TI, int TJ, int WI, int WJ, int FROM>
+template <typename T, int TI, int TJ, int WI, int WJ, bool TOGETHER>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned tiles_i, unsigned tiles_j, int ts, typename Mat<T>::Sum* parts,
                                                             typename Mat<T>::Sum* col_parts) {
     using M = Mat<T>;
     using Acc = typename M::Acc;
     constexpr int SZ = (int)sizeof(T), E = M::E, KB = 128 / SZ, NT = 64 * WI * WJ, IR = TI / WI / 16, JR = TJ / WJ / 16;
     constexpr int AL = TI * SZ / 16, BL = TJ * SZ / 16;                               // pieces of a line
-    constexpr int AP = TI * 8 / NT, BP = TJ * 8 / NT;
-    static_assert(TI * 8 % NT == 0 && TJ * 8 % NT == 0, "whole waves of pieces");
+    constexpr int AP = (TI * 8 + NT - 1) / NT, BP = (TJ * 8 + NT - 1) / NT;
+    static_assert(TI * 8 % 64 == 0 && TJ * 8 % 64 == 0, "whole waves of pieces");
     __shared__ __attribute__((aligned(1024))) char lds[2 * (TI + TJ) * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wi = wave / WJ * (TI / WI), wj = wave % WJ * (TJ / WJ);
     const unsigned tiles = tiles_i * tiles_j, id = die_order(blockIdx.x, gridDim.x);
     const int i0 = (int)(id % tiles / tiles_j) * TI, j0 = (int)(id % tiles_j) * TJ;
     const int64_t t = id / tiles;
-    // (a span without rows still has its group: a group without rows is written as zeros)
-    auto clamped = [&](int g) {
-        const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
-        return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
-    };
-    const int g = wave_search(a.groups, t, [&](int i) { return (clamped(i) >> ts) + i; });
-    if (g < 0) return;
-    const int64_t go = clamped(g), ge = max(go, clamped(g + 1)), span = t - ((go >> ts) + g), q0 = go + (span << ts);
-    if (span > 0 && q0 >= ge) return;
-    const int n = (int)min(ge - q0, (int64_t)1 << ts);                                // rows of the span
-    const bool whole = go + (1ll << ts) >= ge;
+    auto brings_a = [&](int i) { return TI * 8 % NT == 0 || wave * 64 + NT * i < TI * 8; };
+    auto brings_b = [&](int i) { return TJ * 8 % NT == 0 || wave * 64 + NT * i < TJ * 8; };
+    int g, n;
+    int64_t q0;
+    bool whole;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
 
     Acc acc[IR][JR], col[IR];
 #pragma unroll
@@ -188,7 +290,6 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
         for (int j = 0; j < E; ++j) e[j] = (T)1;
         __builtin_memcpy(&ones, e, 16);
     }
-    auto row_of = [&](int k) { return a.rowmap ? a.rowmap[q0 + k] : q0 + k; };
     auto multiply = [&](int buf) {
         const char* as = lds + buf * (TI + TJ) * 128;
         const char* bs = as + TI * 128;
@@ -208,96 +309,90 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
                 for (int i = 0; i < IR; ++i) col[i] = M::mma(af[i], ones, col[i]);
         }
     };
-    if constexpr (FROM == 1) {
-        constexpr unsigned OUT = 0xffffffffu;
+    // a step through registers: row(k) of its k-th place, for k < left; zeros for the others and past the last column
+    u32x4 ar[AP], br[BP];
+    auto load = [&](int left, auto row) {
+#pragma unroll
+        for (int i = 0; i < AP; ++i) {
+            const int q = tid + NT * i, k = q / AL, c = i0 + (q % AL ^ spread<T, TI>(k) * SZ) * E;
+            if (brings_a(i)) ar[i] = k < left ? load_piece((const T*)a.a + row(k) * a.lda, c, a.I) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < BP; ++i) {
+            const int q = tid + NT * i, k = q / BL, c = j0 + (q % BL ^ spread<T, TJ>(k) * SZ) * E;
+            if (brings_b(i)) br[i] = k < left ? load_piece((const T*)a.b + row(k) * a.ldb, c, a.J) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto store = [&](int buf) {
+        char* as = lds + buf * (TI + TJ) * 128;
+#pragma unroll
+        for (int i = 0; i < AP; ++i)
+            if (brings_a(i)) *(u32x4*)(as + (tid + NT * i) * 16) = ar[i];
+#pragma unroll
+        for (int i = 0; i < BP; ++i)
+            if (brings_b(i)) *(u32x4*)(as + TI * 128 + (tid + NT * i) * 16) = br[i];
+    };
+    if constexpr (TOGETHER) {
+        // offsets of this lane's pieces from the step's first; out of range (nothing is read, LDS gets zeros) past the last column.
+        // A piece that runs past the last column takes what lies behind it, which no result sees; of a run's last row that may be
+        // the array's end, so then the last step goes through registers even if it is a whole one.
         unsigned ao[AP], bo[BP];
 #pragma unroll
         for (int i = 0; i < AP; ++i) {
             const int q = tid + NT * i, k = q / AL, c = (q % AL ^ spread<T, TI>(k) * SZ) * E;
-            ao[i] = i0 + c < a.I ? (unsigned)k * (unsigned)(a.lda * SZ) + c * SZ : OUT;
+            ao[i] = i0 + c < a.I ? (unsigned)k * (unsigned)(a.lda * SZ) + c * SZ : 0xffffffffu;
         }
 #pragma unroll
         for (int i = 0; i < BP; ++i) {
             const int q = tid + NT * i, k = q / BL, c = (q % BL ^ spread<T, TJ>(k) * SZ) * E;
-            bo[i] = j0 + c < a.J ? (unsigned)k * (unsigned)(a.ldb * SZ) + c * SZ : OUT;
+            bo[i] = j0 + c < a.J ? (unsigned)k * (unsigned)(a.ldb * SZ) + c * SZ : 0xffffffffu;
         }
-        const char* ab = (const char*)((const T*)a.a + q0 * a.lda + i0);
-        const char* bb = (const char*)((const T*)a.b + q0 * a.ldb + j0);
-        auto bring = [&](int buf, int left) {
-            char* as = lds + buf * (TI + TJ) * 128;
-            const bool tail = left < KB;
+        const int uneven = a.I % E || a.J % E ? 1 : 0;
+        each_run(a, q0, q0 + n, [&](int64_t row0, int rows) {
+            const int full = (rows - uneven) / KB;
+            const char* ab = (const char*)((const T*)a.a + row0 * a.lda + i0);
+            const char* bb = (const char*)((const T*)a.b + row0 * a.ldb + j0);
+            auto bring = [&](int buf) {
+                char* as = lds + buf * (TI + TJ) * 128;
 #pragma unroll
-            for (int i = 0; i < AP; ++i) bring_piece(ab, tail && (tid + NT * i) / AL >= left ? OUT : ao[i], as + (wave * 64 + NT * i) * 16);
+                for (int i = 0; i < AP; ++i)
+                    if (brings_a(i)) bring_piece(ab, ao[i], as + (wave * 64 + NT * i) * 16);
 #pragma unroll
-            for (int i = 0; i < BP; ++i)
-                bring_piece(bb, tail && (tid + NT * i) / BL >= left ? OUT : bo[i], as + TI * 128 + (wave * 64 + NT * i) * 16);
-            ab += KB * a.lda * SZ;
-            bb += KB * a.ldb * SZ;
-        };
-        if (n > 0) bring(0, n);
-        __syncthreads();
-        int buf = 0;
-        for (int left = n; left > 0; left -= KB, buf ^= 1) {
-            if (left > KB) bring(buf ^ 1, left - KB);
-            multiply(buf);
+                for (int i = 0; i < BP; ++i)
+                    if (brings_b(i)) bring_piece(bb, bo[i], as + TI * 128 + (wave * 64 + NT * i) * 16);
+                ab += KB * a.lda * SZ;
+                bb += KB * a.ldb * SZ;
+            };
+            if (full > 0) bring(0);
+            const int rest = rows - full * KB;
+            auto load_rest = [&]() { load(rest, [&](int k) { return row0 + full * KB + k; }); };
+            constexpr bool EARLY = TI * TJ < 256 * 256;                               // (registers)
+            if (EARLY && rest > 0) load_rest();
             __syncthreads();
-        }
-    } else if constexpr (FROM == 2) {
-        // columns past the end and rows past the span come from a piece of zeros
-        auto bring = [&](int buf, int k0) {
-            char* as = lds + buf * (TI + TJ) * 128;
-#pragma unroll
-            for (int i = 0; i < AP; ++i) {
-                const int q = tid + NT * i, k = q / AL, c = i0 + (q % AL ^ spread<T, TI>(k) * SZ) * E;
-                const bool live = k0 + k < n && c < a.I;
-                bring_from(live ? (const char*)((const T*)a.a + row_of(k0 + k) * a.lda + c) : (const char*)&kZeroPiece, as + (wave * 64 + NT * i) * 16);
+            for (int i = 0; i < full; ++i) {
+                if (i + 1 < full) bring((i + 1) & 1);
+                multiply(i & 1);
+                __syncthreads();
             }
-#pragma unroll
-            for (int i = 0; i < BP; ++i) {
-                const int q = tid + NT * i, k = q / BL, c = j0 + (q % BL ^ spread<T, TJ>(k) * SZ) * E;
-                const bool live = k0 + k < n && c < a.J;
-                bring_from(live ? (const char*)((const T*)a.b + row_of(k0 + k) * a.ldb + c) : (const char*)&kZeroPiece,
-                           as + TI * 128 + (wave * 64 + NT * i) * 16);
+            if (rest > 0) {
+                if (!EARLY) load_rest();
+                store(0);
+                __syncthreads();
+                multiply(0);
+                __syncthreads();
             }
-        };
-        if (n > 0) bring(0, 0);
-        __syncthreads();
-        int buf = 0;
-        for (int k0 = 0; k0 < n; k0 += KB, buf ^= 1) {
-            if (k0 + KB < n) bring(buf ^ 1, k0 + KB);
-            multiply(buf);
-            __syncthreads();
-        }
+        });
     } else {
-        u32x4 ar[AP], br[BP];
-        auto load = [&](int k0) {
-#pragma unroll
-            for (int i = 0; i < AP; ++i) {
-                const int q = tid + NT * i, k = q / AL, c = i0 + (q % AL ^ spread<T, TI>(k) * SZ) * E;
-                ar[i] = k0 + k < n ? load_piece((const T*)a.a + row_of(k0 + k) * a.lda, c, a.I) : u32x4{0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int i = 0; i < BP; ++i) {
-                const int q = tid + NT * i, k = q / BL, c = j0 + (q % BL ^ spread<T, TJ>(k) * SZ) * E;
-                br[i] = k0 + k < n ? load_piece((const T*)a.b + row_of(k0 + k) * a.ldb, c, a.J) : u32x4{0, 0, 0, 0};
-            }
-        };
-        auto store = [&](int buf) {
-            char* as = lds + buf * (TI + TJ) * 128;
-#pragma unroll
-            for (int i = 0; i < AP; ++i) *(u32x4*)(as + (tid + NT * i) * 16) = ar[i];
-#pragma unroll
-            for (int i = 0; i < BP; ++i) *(u32x4*)(as + TI * 128 + (tid + NT * i) * 16) = br[i];
-        };
+        auto fetch = [&](int k0) { load(n - k0, [&](int k) { return a.rowmap ? a.rowmap[q0 + k0 + k] : q0 + k0 + k; }); };
         if (n > 0) {
-            load(0);
+            fetch(0);
             store(0);
         }
         __syncthreads();
         int buf = 0;
         for (int k0 = 0; k0 < n; k0 += KB, buf ^= 1) {
             const bool more = k0 + KB < n;
-            if (more) load(k0 + KB);
+            if (more) fetch(k0 + KB);
             multiply(buf);
             if (more) store(buf ^ 1);
             __syncthreads();
@@ -321,6 +416,204 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
                 else col_parts[t * a.I + ii] = col[i][r];
             }
         }
+}
+
+// ------------------------------------------------------------------------------------------
+// The same for 16-bit types and wide matrices whose segments are long: 256 x 256 results, eight waves of 128 x 64, steps of 64 rows
+// between two pairs of LDS buffers.  While half a step multiplies, the fragments of the next half are read; in the middle of a step
+// its own buffers fall free and the step after next is asked for.
+// Both operands are strided: which rows the lanes of a fragment hold is free as long as both do alike, so lanes 16 kk .. take rows
+// 4 kk .. 4 kk + 3 and 16 more.  Lines of 512 bytes, two to a kilobyte that a wave brings, each kilobyte 64 bytes further on and the
+// odd line's runs of 16 columns swapped in pairs: the eight lines that one read touches lie in other banks, and the reads need two
+// addresses instead of eight (registers).
+// ------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, unsigned tiles_j, int ts, float* parts) {
+    using M = Mat<T>;
+    using Acc = typename M::Acc;
+    constexpr int E = 8, KB = 64, NT = 512, IR = 8, JR = 4, TI = 256, TJ = 256, CHUNK = 1024 + 64, UNIT = 32 * CHUNK;
+    static_assert(sizeof(T) == 2, "16-bit types");
+    // (four variables, not one array: the compiler then knows that reading one does not wait for what is brought into another)
+    __shared__ __attribute__((aligned(64))) char a0[UNIT], b0[UNIT], a1[UNIT], b1[UNIT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
+    const int wi = wave / 4 * 128, wj = wave % 4 * 64;
+    // (not in die_order: neighbouring blocks are tiles of one span, spread over the dies so that all of them start with the longest)
+    const unsigned tiles = tiles_i * tiles_j, id = blockIdx.x;
+    const int i0 = (int)(id % tiles / tiles_j) * TI, j0 = (int)(id % tiles_j) * TJ;
+    const unsigned spans = gridDim.x / tiles;
+    const int64_t t = spans <= 64 ? longest_span(a, spans, id / tiles, ts) : id / tiles;
+    int g, n;
+    int64_t q0;
+    bool whole;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
+
+    Acc acc[IR][JR];
+#pragma unroll
+    for (int i = 0; i < IR; ++i)
+#pragma unroll
+        for (int j = 0; j < JR; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+    struct Frags {
+        u32x4 a[IR], b[JR];
+    };
+    // line k of a unit: chunk k / 2; run r of 16 columns of an odd line lies at r ^ 1
+    auto fragment = [&](const char* unit, int h, int c) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds16x4;
+        const int j = l15 >> 2;                           // lines 32 h + 4 kk + j and 16 further
+        const int at = (2 * kk + (j >> 1)) * CHUNK + (j & 1) * 512 + (((c / 16) ^ (j & 1)) << 5) + (l15 & 3) * 8 + 16 * h * CHUNK;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(unit + at)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(unit + (at + 8 * CHUNK))));
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    auto read = [&](const char* as, const char* bs, int h, Frags& f) {
+#pragma unroll
+        for (int j = 0; j < JR; ++j) f.b[j] = fragment(bs, h, wj + 16 * j);
+#pragma unroll
+        for (int i = 0; i < IR; ++i) f.a[i] = fragment(as, h, wi + 16 * i);
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+        for (int i = 0; i < IR; ++i)
+#pragma unroll
+            for (int j = 0; j < JR; ++j) acc[i][j] = M::mma(f.a[i], f.b[j], acc[i][j]);
+    };
+    unsigned ao[4], bo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int q = tid + NT * i, k = q / 32, c = (q % 32 ^ (k & 1) * 2) * E;      // the piece at this place
+        ao[i] = i0 + c < a.I ? (unsigned)k * (unsigned)(a.lda * 2) + c * 2 : 0xffffffffu;
+        bo[i] = j0 + c < a.J ? (unsigned)k * (unsigned)(a.ldb * 2) + c * 2 : 0xffffffffu;
+    }
+    const int uneven = a.I % E || a.J % E ? 1 : 0;        // as in sum_tile
+    each_run(a, q0, q0 + n, [&](int64_t row0, int rows) {
+        const int full = (rows - uneven) / KB;
+        const char* ab = (const char*)((const T*)a.a + row0 * a.lda + i0);
+        const char* bb = (const char*)((const T*)a.b + row0 * a.ldb + j0);
+        auto bring = [&](char* as, char* bs) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bring_piece(ab, ao[i], as + (wave + 8 * i) * CHUNK);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bring_piece(bb, bo[i], bs + (wave + 8 * i) * CHUNK);
+            ab += KB * a.lda * 2;
+            bb += KB * a.ldb * 2;
+        };
+        constexpr int VM0 = 0x0f70;                       // s_waitcnt vmcnt(0), the other counters free
+        Frags f0, f1;
+        if (full > 0) {
+            bring(a0, b0);
+            if (full > 1) bring(a1, b1);
+            __builtin_amdgcn_s_waitcnt(VM0);
+            __builtin_amdgcn_s_barrier();
+            read(a0, b0, 0, f0);
+            auto interleave = [&]() {                     // a read behind every product, then the other products
+#pragma unroll
+                for (int j = 0; j < 24; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // One step from as, bs; the next one in an, bn.  At the barrier the next step has arrived for every wave, and every wave
+            // has read all of this one.
+            auto run = [&](char* as, char* bs, const char* an, const char* bn) {
+                read(as, bs, 1, f1);
+                multiply(f0);
+                interleave();
+                __builtin_amdgcn_s_waitcnt(VM0 & 0xf0ff);
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                bring(as, bs);
+                read(an, bn, 0, f0);
+                multiply(f1);
+                __builtin_amdgcn_sched_group_barrier(0x020, 8, 0);
+                interleave();
+            };
+            auto turn = [&](int s, char* as, char* bs, const char* an, const char* bn) {
+                read(as, bs, 1, f1);
+                multiply(f0);
+                __builtin_amdgcn_s_waitcnt(VM0 & 0xf0ff);
+                __builtin_amdgcn_s_barrier();
+                if (s + 2 < full) bring(as, bs);
+                if (s + 1 < full) read(an, bn, 0, f0);
+                multiply(f1);
+            };
+            int s = 0;
+            for (; s + 4 <= full; s += 2) {
+                run(a0, b0, a1, b1);
+                run(a1, b1, a0, b0);
+            }
+            for (; s < full; s += 2) {
+                turn(s, a0, b0, a1, b1);
+                if (s + 1 < full) turn(s + 1, a1, b1, a0, b0);
+            }
+            __syncthreads();
+        }
+        const int rest = rows - full * KB;
+        if (rest > 0) {                                   // a last, uneven step through registers
+            const int64_t r = row0 + full * KB;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int q = tid + NT * i, k = q / 32, c = (q % 32 ^ (k & 1) * 2) * E, at = (wave + 8 * i) * CHUNK + lane * 16;
+                *(u32x4*)(a0 + at) = k < rest ? load_piece((const T*)a.a + (r + k) * a.lda, i0 + c, a.I) : u32x4{0, 0, 0, 0};
+                *(u32x4*)(b0 + at) = k < rest ? load_piece((const T*)a.b + (r + k) * a.ldb, j0 + c, a.J) : u32x4{0, 0, 0, 0};
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                read(a0, b0, h, f0);
+                multiply(f0);
+            }
+            __syncthreads();
+        }
+    });
+#pragma unroll
+    for (int i = 0; i < IR; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int ii = i0 + wi + 16 * i + M::row(r, kk);
+            if (ii >= a.I) continue;
+#pragma unroll
+            for (int j = 0; j < JR; ++j) {
+                const int jj = j0 + wj + 16 * j + l15;
+                if (jj >= a.J) continue;
+                if (whole) ((T*)a.out)[((int64_t)g * a.I + ii) * a.J + jj] = (T)acc[i][j][r];
+                else parts[(t * a.I + ii) * a.J + jj] = acc[i][j][r];
+            }
+        }
+}
+
+// Column sums of a beside sum_deep: cols[k, i] = sum of a[r, i], a span and 512 columns a block, eight of them a thread; the rows of the
+// span go to the four waves in turn, which meet in LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int ts, float* col_parts) {
+    __shared__ float part[3][64][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)(blockIdx.x % tiles) * 512 + lane * 8;
+    const int64_t t = blockIdx.x / tiles;
+    int g, n;
+    int64_t q0;
+    bool whole;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+    for (int k = wave; k < n; k += 4) {
+        const u32x4 v = load_piece((const T*)a.a + (a.rowmap ? a.rowmap[q0 + k] : q0 + k) * a.lda, c, a.I);
+        T e[8];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += (float)e[j];
+    }
+    if (wave)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[wave - 1][lane][j] = sum[j];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v = sum[j] + part[0][lane][j] + part[1][lane][j] + part[2][lane][j];
+        if (c + j >= a.I) continue;
+        if (whole) ((T*)a.cols)[(int64_t)g * a.I + c + j] = (T)v;
+        else col_parts[t * a.I + c + j] = v;
+    }
 }
 
 template <typename T>
@@ -367,18 +660,24 @@ int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const vo
     }
 }
 
+// Length of a span, as a power of two: a span's sums are written and read once more (8 or 16 bytes each) beside its 2 x 2^ts products
+// of each, so long ones, but no fewer blocks than the CUs hold at a time (`want`).  Where the groups give that many by themselves,
+// only one far over the mean is cut.  Never more sums than 256 MB beside one for each group.
+static int span_length(const SumArgs& a, int64_t tiles, int64_t want, size_t sum_size) {
+    const int64_t size = (int64_t)a.I * a.J + a.I;
+    int ts = 8;
+    while (ts < 40 && (a.sg.rows >> ts) * tiles > want) ++ts;
+    if (a.groups * tiles >= want) ++ts;
+    while (ts < 40 && (a.sg.rows >> ts) * size * (int64_t)sum_size > (256ll << 20)) ++ts;
+    return ts;
+}
+
 template <typename T, int TI, int TJ, int WI, int WJ>
 static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     using Sum = typename Mat<T>::Sum;
-    const int64_t ti = (a.I + TI - 1) / TI, tj = (a.J + TJ - 1) / TJ, size = (int64_t)a.I * a.J + a.I, e = 16 / sizeof(T);
-    const bool dma = ((uintptr_t)a.a | (uintptr_t)a.b) % 16 == 0 && a.I % e == 0 && a.J % e == 0 && a.lda % e == 0 && a.ldb % e == 0;
-    // A span's sums are written and read once more (8 or 16 bytes each) beside its 2 x 2^ts products of each: long spans, but
-    // no fewer blocks than the CUs hold at a time (one of 256 x 256, two of 128 x 128, four of 64 x 64).  Where the groups give that many by themselves, only one far over the mean is cut.
-    const int64_t want = (TI >= 256 ? 2 : TI >= 128 ? 4 : 8) * ctx->prop.multiProcessorCount;
-    int ts = 8;
-    while (ts < 40 && (a.sg.rows >> ts) * ti * tj > want) ++ts;
-    if (a.groups * ti * tj >= want) ++ts;
-    while (ts < 40 && (a.sg.rows >> ts) * size * (int64_t)sizeof(Sum) > (256ll << 20)) ++ts;
+    constexpr int KB = 128 / (int)sizeof(T), HOLDS = std::min(8, (160 << 10) / (2 * (TI + TJ) * 128));
+    const int64_t ti = (a.I + TI - 1) / TI, tj = (a.J + TJ - 1) / TJ, size = (int64_t)a.I * a.J + a.I;
+    const int ts = span_length(a, ti * tj, (int64_t)HOLDS * ctx->prop.multiProcessorCount, sizeof(Sum));
     const int64_t spans = (a.sg.rows >> ts) + a.groups;
     LN_REQUIRE(spans * ti * tj < (1ll << 31), "%lld rows in %d groups of %d x %d sums are too many for one call", (long long)a.sg.rows,
                a.groups, a.I, a.J);
@@ -387,26 +686,50 @@ static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
     Sum* cp = (Sum*)parts + spans * a.I * a.J;
     const dim3 grid((unsigned)(spans * ti * tj)), block(64 * WI * WJ);
-    if (dma && !a.rowmap && std::max(a.lda, a.ldb) * 64 * (int64_t)sizeof(T) < (1ll << 31))
-        LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, 1>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
-    else if (dma) LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, 2>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
-    else LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, 0>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
-    if (split) return join_t<T>(ctx, a, ts, (const Sum*)parts, (const Sum*)cp);
+    // runs of a few steps at least are worth starting the LDS-DMA for
+    const bool together = (!a.rowmap || a.sg.rows / a.sg.S >= 4 * KB) && std::max(a.lda, a.ldb) * KB * (int64_t)sizeof(T) < (1ll << 31);
+    if (together) LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, true>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
+    else LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, false>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
+    return split ? join_t<T>(ctx, a, ts, parts, cp) : 0;
+}
+
+template <typename T>
+static int launch_sum_deep(lnasr_ctx* ctx, SumArgs a, const char* name) {
+    const int64_t ti = (a.I + 255) / 256, tj = (a.J + 255) / 256;
+    void* const cols = a.cols;
+    for (int pass = 0; pass < (cols ? 2 : 1); ++pass) {
+        // the product, then the column sums: with spans of their own, one after the other in the same workspace
+        if (pass) a.J = 0;
+        a.cols = pass ? cols : nullptr;
+        const int64_t tiles = pass ? (a.I + 511) / 512 : ti * tj, size = (int64_t)a.I * a.J + a.I;
+        const int ts = span_length(a, tiles, (pass ? 4 : 1) * ctx->prop.multiProcessorCount, 4);
+        const int64_t spans = (a.sg.rows >> ts) + a.groups;
+        LN_REQUIRE(spans * tiles < (1ll << 31), "%lld rows in %d groups of %d x %d sums are too many for one call", (long long)a.sg.rows,
+                   a.groups, a.I, a.J);
+        void* parts = nullptr;
+        const bool split = a.sg.rows > (1ll << ts);
+        if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * 4, &parts));
+        float* cp = (float*)parts + spans * a.I * a.J;
+        if (pass) LN_LAUNCH(ctx, "sum_cols", (sum_cols<T>), dim3((unsigned)(spans * tiles)), dim3(256), 0, a, (unsigned)tiles, ts, cp);
+        else LN_LAUNCH(ctx, name, (sum_deep<T>), dim3((unsigned)(spans * tiles)), dim3(512), 0, a, (unsigned)ti, (unsigned)tj, ts, (float*)parts);
+        if (split) LN_TRY(join_t<T>(ctx, a, ts, parts, cp));
+    }
     return 0;
 }
 
 template <typename T>
 static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
+    if (a.I <= 16) return launch_sum<T, 16, 128, 1, 4>(ctx, a, name);
+    if (a.J <= 16) return launch_sum<T, 128, 16, 4, 1>(ctx, a, name);
+    if (a.I <= 32) return launch_sum<T, 32, 128, 1, 4>(ctx, a, name);
+    if (a.J <= 32) return launch_sum<T, 128, 32, 4, 1>(ctx, a, name);
     if constexpr (sizeof(T) == 2) {
-        if ((int64_t)(a.I / 256) * (a.J / 256) * a.groups >= 128) return launch_sum<T, 256, 256, 2, 4>(ctx, a, name);
+        if ((int64_t)(a.I / 256) * (a.J / 256) * std::max<int64_t>(a.groups, a.sg.rows >> 11) >= 128 && (!a.rowmap || a.sg.rows / a.sg.S >= 512) &&
+            std::max(a.lda, a.ldb) * 128 < (1ll << 31))
+            return launch_sum_deep<T>(ctx, a, name);
         if (a.I > 64 && a.J > 64) return launch_sum<T, 128, 128, 2, 2>(ctx, a, name);
-        return launch_sum<T, 64, 64, 2, 2>(ctx, a, name);
-    } else if constexpr (sizeof(T) == 4) {
-        if (a.I > 64 && a.J > 64) return launch_sum<T, 128, 128, 2, 2>(ctx, a, name);
-        return launch_sum<T, 64, 64, 2, 2>(ctx, a, name);
-    } else {
-        return launch_sum<T, 64, 64, 2, 2>(ctx, a, name);
     }
+    return launch_sum<T, 64, 64, 2, 2>(ctx, a, name);
 }
 
 int transform_sum(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name) {

@@ -638,18 +638,28 @@ static int launch_few(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     return 0;
 }
 
+template <typename T, int TN, bool KN, int LOW>
+static int rows_thin(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
+    // (128 rows a tile; 64 where that leaves the CUs short of blocks)
+    if (a.sg.rows / 128 + a.sg.S >= 4 * ctx->prop.multiProcessorCount) return launch_tile<T, 128, TN, 4, 1, KN, LOW>(ctx, a, name);
+    return launch_tile<T, 64, TN, 4, 1, KN, LOW>(ctx, a, name);
+}
+
 template <typename T, bool KN, int LOW>
 static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t cus = ctx->prop.multiProcessorCount, rows = a.sg.rows;
     if constexpr (LOW != 2) {
-        if (a.N <= 16) return launch_tile<T, 128, 16, 4, 1, KN, LOW>(ctx, a, name);
-        if (a.N <= 32) return launch_tile<T, 128, 32, 4, 1, KN, LOW>(ctx, a, name);
-        if (a.N <= 48) return launch_tile<T, 128, 48, 4, 1, KN, LOW>(ctx, a, name);
-        if (a.N <= 64) return launch_tile<T, 128, 64, 4, 1, KN, LOW>(ctx, a, name);
-        if constexpr (sizeof(T) == 2)
+        if (a.N <= 16) return rows_thin<T, 16, KN, LOW>(ctx, a, name);
+        if (a.N <= 32) return rows_thin<T, 32, KN, LOW>(ctx, a, name);
+        if (a.N <= 48) return rows_thin<T, 48, KN, LOW>(ctx, a, name);
+        // 16 bits: the larger the tile the less it asks of the memory for its products (us, 64 x 64 / 128 x 128 / 256 x 256: 65,536 x
+        // 2048 x 2048 1185 / 800 / 599; 16,384 x 1024 x 1024 65 / 57 / 46), as long as there is one for every CU.  32 and 64 bits
+        // have time for that: 64 x 64 leaves the least over at the ends (f32 120,011 x 351 x 128 105 against 142 us, f64 16,384 x
+        // 1024 x 1024 609 against 640; f32 65,536 x 1024 x 1024 1169 against 1165).
+        if constexpr (sizeof(T) == 2) {
             if (rows / 256 * (a.N / 256) >= cus) return launch_deep<T, KN, LOW>(ctx, a, name);
-        constexpr int WN = sizeof(T) == 8 ? 4 : 2;
-        if ((rows / 128 + a.sg.S) * ((a.N + 127) / 128) >= 4 * cus) return launch_tile<T, 128, 128, 2, WN, KN, LOW>(ctx, a, name);
+            if ((rows / 128 + a.sg.S / 2) * ((a.N + 127) / 128) >= 2 * cus) return launch_tile<T, 128, 128, 2, 2, KN, LOW>(ctx, a, name);
+        }
     }
     return launch_tile<T, 64, 64, 2, 2, KN, LOW>(ctx, a, name);
 }
