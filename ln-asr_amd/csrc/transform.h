@@ -218,16 +218,50 @@ int transform_rows(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* nam
 // written, zeros where it has no rows.
 struct SumArgs {
     Segments sg;
-    const int64_t* group_off;   // group g: places group_off[g * group_step] .. group_off[(g + 1) * group_step] of `rowmap`
+    const int64_t* group_off;   // group g: places group_off[g * group_step] .. group_off[(g + 1) * group_step] of the sorted rows
     int64_t group_step;         // 1; S: all segments as one group
-    const int64_t* rowmap;      // row at each place of the sorted order, or null: the rows as they lie
-    const int64_t* place;       // [S + 1] (with rowmap) places of the sorted segments' rows
-    const int* ord;             // [S] the sorted segments
+    const int* ord;             // [S] the segments in the order of their groups, or null: the rows as they lie
+    const int64_t* place;       // [S + 1] (with ord) places of the sorted segments' rows
+    const int64_t* rowmap;      // (with ord, if the segments are short) the row at each place
     const void *a, *b;
     void *out, *cols;
     int64_t lda, ldb;
     int groups, I, J;
 };
+// Span t of 2^ts places of the sorted rows: its group, first place and rows; false: nothing to do.  (A group without rows has one
+// span without rows, to be written as zeros.)
+__device__ __forceinline__ bool sum_span(const SumArgs& a, int64_t t, int ts, int* group, int64_t* q0, int* n, bool* whole) {
+    auto clamped = [&](int g) {
+        const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
+        return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
+    };
+    const int g = wave_search(a.groups, t, [&](int i) { return (clamped(i) >> ts) + i; });
+    if (g < 0) return false;
+    const int64_t go = clamped(g), ge = max(go, clamped(g + 1)), span = t - ((go >> ts) + g);
+    *group = g;
+    *q0 = go + (span << ts);
+    if (span > 0 && *q0 >= ge) return false;
+    *n = (int)min(ge - *q0, (int64_t)1 << ts);
+    *whole = go + (1ll << ts) >= ge;
+    return true;
+}
+// The rows that lie together from place q of the sorted rows on, at most up to place end: calls each(first row, rows) run by run
+template <typename F>
+__device__ __forceinline__ void each_run(const SumArgs& a, int64_t q, int64_t end, F each) {
+    int i = a.place ? max(0, wave_search(a.sg.S, q, [&](int j) { return a.place[j]; })) : 0;
+    while (q < end) {                                     // (one call of `each`: it is a kernel's whole loop)
+        int64_t row = q, to = end;
+        if (a.place) {
+            while (i < a.sg.S && a.place[i + 1] <= q) ++i;
+            if (i >= a.sg.S) return;
+            to = min(a.place[i + 1], end);
+            row = seg_off(a.sg, a.ord[i]) + (q - a.place[i]);
+        }
+        each(row, (int)(to - q));
+        q = to;
+    }
+}
+
 int transform_sum(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
 // transform_narrow.hip: the same for contiguous rows of up to 64 values
 bool rows_narrow_ok(const RowsArgs& a);
@@ -236,8 +270,8 @@ bool sum_narrow_ok(const SumArgs& a);
 int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
 // out and cols from the sums of the spans of 2^ts rows
 int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const void* parts, const void* col_parts);
-// Sorts the segments by group (stable): group_off, rowmap, place, ord of a.  Without slots the rows are sorted as they lie.
-int transform_sort(lnasr_ctx* ctx, SumArgs* a);
+// Sorts the segments by group (stable): group_off, ord, place, rowmap of a.  Without slots the rows are sorted as they lie.
+int transform_sort(lnasr_ctx* ctx, int dtype, SumArgs* a);
 
 // Workspace `i` of the feature transforms with room for `bytes`
 int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out);

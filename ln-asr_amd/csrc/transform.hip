@@ -258,7 +258,7 @@ int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, in
         a.sg = sg;
         a.group_step = 1;
         a.groups = G;
-        LN_TRY(transform_sort(ctx, &a));
+        LN_TRY(transform_sort(ctx, dtype, &a));
         a.a = d_dy;
         a.lda = lddy;
         a.I = dout;
@@ -415,7 +415,7 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
     if (d_da || d_db) {
         t.group_step = 1;
         t.groups = G;
-        if (S > 0) LN_TRY(transform_sort(ctx, &t));
+        if (S > 0) LN_TRY(transform_sort(ctx, dtype, &t));
     }
     if (d_da) {
         t.a = dp;

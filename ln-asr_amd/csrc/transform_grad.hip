@@ -14,7 +14,7 @@ constexpr int kSortNT = 1024;
 __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes, int* ord0, int* ord1, int64_t* place,
                                                          int64_t* group_off) {
     __shared__ int base[256], cnt[kSortNT / 64][256];
-    __shared__ int64_t part[kSortNT], carry;
+    __shared__ int64_t part[kSortNT / 64], carry;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     auto key = [&](int s) {
         const int k = seg_slot(sg, s);
@@ -28,12 +28,21 @@ __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes
         __syncthreads();
         for (int i = tid; i < sg.S; i += kSortNT) atomicAdd(&base[key(in[i]) >> (8 * p) & 255], 1);
         __syncthreads();
-        if (tid == 0)
-            for (int d = 0, sum = 0; d < 256; ++d) {
-                const int c = base[d];
-                base[d] = sum;
-                sum += c;
+        if (wave == 0) {                                  // running sum, four digits a lane
+            int c[4], sum = 0;
+            for (int e = 0; e < 4; ++e) c[e] = base[4 * lane + e];
+            const int mine = c[0] + c[1] + c[2] + c[3];
+            sum = mine;
+            for (int d = 1; d < 64; d *= 2) {
+                const int v = __shfl_up(sum, d);
+                sum += lane >= d ? v : 0;
             }
+            sum -= mine;
+            for (int e = 0; e < 4; ++e) {
+                base[4 * lane + e] = sum;
+                sum += c[e];
+            }
+        }
         for (int c0 = 0; c0 < sg.S; c0 += kSortNT) {
             for (int i = tid; i < kSortNT / 64 * 256; i += kSortNT) cnt[i >> 8][i & 255] = 0;
             __syncthreads();
@@ -74,15 +83,16 @@ __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes
         const int s = live ? in[i] : 0, k = live ? key(s) : sg.G;
         int64_t len = live && k < sg.G ? seg_off(sg, s + 1) - seg_off(sg, s) : 0;
         if (len < 0) len = 0;
-        part[tid] = len;
-        __syncthreads();
-        for (int d = 1; d < kSortNT; d *= 2) {
-            const int64_t v = tid >= d ? part[tid - d] : 0;
-            __syncthreads();
-            part[tid] += v;
-            __syncthreads();
+        // running sum of a wave by shuffles, of the waves by the last lanes' sums
+        int64_t sum = len;
+        for (int d = 1; d < 64; d *= 2) {
+            const int64_t v = __shfl_up(sum, d);
+            sum += lane >= d ? v : 0;
         }
-        const int64_t at = min(carry + part[tid] - len, sg.rows);
+        if (lane == 63) part[wave] = sum;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) sum += part[w];
+        const int64_t at = min(carry + sum - len, sg.rows);
         if (live) {
             place[i] = at;
             if (in != ord0) ord0[i] = s;
@@ -90,63 +100,13 @@ __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes
             for (int g = before + 1; g <= k; ++g) group_off[g] = at;
         }
         __syncthreads();
-        if (tid == kSortNT - 1) carry += part[tid];
+        if (tid == kSortNT - 1) carry += sum;
         __syncthreads();
     }
     const int64_t total = min(carry, sg.rows);
     if (tid == 0) place[sg.S] = total;
     const int last = key(in[sg.S - 1]);
     for (int g = last + 1 + tid; g <= sg.G; g += kSortNT) group_off[g] = total;
-}
-
-// The same for up to 1024 segments in one kernel with the rows' places: every block finds all of them -- thread i counts the segments
-// that come before segment i (a smaller group, or the same and earlier) and their rows -- and writes the rows of some.
-__global__ __launch_bounds__(kSortNT) void sort_few_segments(Segments sg, int* ord, int64_t* place, int64_t* group_off, int64_t* rowmap) {
-    __shared__ int keys[kSortNT];
-    __shared__ int64_t lens[kSortNT], first[kSortNT], at[kSortNT];
-    const int tid = threadIdx.x;
-    int k = sg.G;
-    int64_t len = 0, from = 0;
-    if (tid < sg.S) {
-        from = seg_off(sg, tid);
-        k = seg_slot(sg, tid);
-        if (k < 0) k = sg.G;
-        len = k < sg.G ? max((int64_t)0, seg_off(sg, tid + 1) - from) : 0;
-    }
-    keys[tid] = k;
-    lens[tid] = len;
-    first[tid] = from;
-    __syncthreads();
-    int64_t before = 0;
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < sg.S; ++j) {
-        const bool first = keys[j] < k || (keys[j] == k && j < tid);
-        before += first ? lens[j] : 0;
-        rank += first ? 1 : 0;
-    }
-    before = min(before, sg.rows);
-    at[tid] = before;
-    if (blockIdx.x == 0) {
-        __shared__ int sorted[kSortNT];
-        if (tid < sg.S) {
-            ord[rank] = tid;
-            place[rank] = before;
-            sorted[rank] = k;
-            if (rank == sg.S - 1) place[sg.S] = min(before + len, sg.rows);
-        }
-        __syncthreads();
-        // a group begins where the first segment of it, or of a later one, lies; those behind the last segment's, at the end
-        if (tid < sg.S) {
-            for (int g = rank ? sorted[rank - 1] + 1 : 0; g <= k; ++g) group_off[g] = before;
-            if (rank == sg.S - 1)
-                for (int g = k + 1; g <= sg.G; ++g) group_off[g] = min(before + len, sg.rows);
-        }
-    }
-    __syncthreads();
-    for (int s = blockIdx.x * 4 + (tid >> 8); s < sg.S; s += gridDim.x * 4)
-        for (int64_t i = tid & 255; i < lens[s]; i += 256)
-            if (at[s] + i < sg.rows) rowmap[at[s] + i] = first[s] + i;
 }
 
 // the row at each place of the sorted order
@@ -162,7 +122,10 @@ __global__ __launch_bounds__(256) void map_rows(Segments sg, const int* ord, con
     rowmap[q] = row < sg.rows ? row : sg.rows - 1;
 }
 
-int transform_sort(lnasr_ctx* ctx, SumArgs* a) {
+// Segments long enough for their rows to be taken run by run: four steps of 128 bytes' worth of rows
+static bool rows_together(const Segments& sg, int dtype) { return sg.rows / sg.S >= 4 * 128 / (int64_t)transform_size(dtype); }
+
+int transform_sort(lnasr_ctx* ctx, int dtype, SumArgs* a) {
     const Segments& sg = a->sg;
     a->rowmap = a->place = nullptr;
     a->ord = nullptr;
@@ -177,38 +140,17 @@ int transform_sort(lnasr_ctx* ctx, SumArgs* a) {
     int64_t* goff = place + sg.S + 1;
     int* ord0 = (int*)(goff + sg.G + 1);
     a->group_off = goff;
-    a->rowmap = map;
+    const bool mapped = !rows_together(sg, dtype);
+    if (mapped) a->rowmap = map;
     a->place = place;
     a->ord = ord0;
-    if (sg.S <= kSortNT) {
-        LN_LAUNCH(ctx, "sort_few_segments", sort_few_segments, dim3((unsigned)std::min((sg.S + 3) / 4, 64)), dim3(kSortNT), 0, sg, ord0, place, goff,
-                  map);
-        return 0;
-    }
     int passes = 1;
     while (passes < 4 && (sg.G >> (8 * passes)) > 0) ++passes;
     LN_LAUNCH(ctx, "sort_segments", sort_segments, dim3(1), dim3(kSortNT), 0, sg, passes, ord0, ord0 + sg.S, place, goff);
-    LN_LAUNCH(ctx, "map_rows", map_rows, dim3((unsigned)((sg.rows + 255) / 256)), dim3(256), 0, sg, ord0, place, map);
+    if (mapped) LN_LAUNCH(ctx, "map_rows", map_rows, dim3((unsigned)((sg.rows + 255) / 256)), dim3(256), 0, sg, ord0, place, map);
     return 0;
 }
 
-// Span t of 2^ts places of the sorted rows: its group, first place and rows; false: nothing to do.  (A group without rows has one
-// span without rows, to be written as zeros.)
-__device__ __forceinline__ bool sum_span(const SumArgs& a, int64_t t, int ts, int* group, int64_t* q0, int* n, bool* whole) {
-    auto clamped = [&](int g) {
-        const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
-        return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
-    };
-    const int g = wave_search(a.groups, t, [&](int i) { return (clamped(i) >> ts) + i; });
-    if (g < 0) return false;
-    const int64_t go = clamped(g), ge = max(go, clamped(g + 1)), span = t - ((go >> ts) + g);
-    *group = g;
-    *q0 = go + (span << ts);
-    if (span > 0 && *q0 >= ge) return false;
-    *n = (int)min(ge - *q0, (int64_t)1 << ts);
-    *whole = go + (1ll << ts) >= ge;
-    return true;
-}
 // Of up to 64 spans the t-th longest: blocks start in the order of their numbers, and the longest ones are to start first
 __device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int64_t t, int ts) {
     const int lane = threadIdx.x & 63;
@@ -229,23 +171,6 @@ __device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int
     const uint64_t mine = __ballot(lane < spans && rank == (int)t);
     return mine ? __builtin_ctzll(mine) : t;
 }
-// The rows that lie together from place q of the sorted rows on, at most up to place end: calls each(first row, rows) run by run
-template <typename F>
-__device__ __forceinline__ void each_run(const SumArgs& a, int64_t q, int64_t end, F each) {
-    int i = a.rowmap ? max(0, wave_search(a.sg.S, q, [&](int j) { return a.place[j]; })) : 0;
-    while (q < end) {                                     // (one call of `each`: it is a kernel's whole loop)
-        int64_t row = q, to = end;
-        if (a.rowmap) {
-            while (i < a.sg.S && a.place[i + 1] <= q) ++i;
-            if (i >= a.sg.S) return;
-            to = min(a.place[i + 1], end);
-            row = seg_off(a.sg, a.ord[i]) + (q - a.place[i]);
-        }
-        each(row, (int)(to - q));
-        q = to;
-    }
-}
-
 // ------------------------------------------------------------------------------------------
 // Tiles of TI x TJ results of one group, WI x WJ waves, summed over a span of the group's rows.  The rows are the k of the product,
 // strided for both operands: they lie in LDS as lines (strided_fragment).  TOGETHER: rows that lie together (a segment's) come by
@@ -594,14 +519,16 @@ __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int t
     bool whole;
     if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
     float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-    for (int k = wave; k < n; k += 4) {
-        const u32x4 v = load_piece((const T*)a.a + (a.rowmap ? a.rowmap[q0 + k] : q0 + k) * a.lda, c, a.I);
-        T e[8];
-        __builtin_memcpy(e, &v, 16);
+    each_run(a, q0, q0 + n, [&](int64_t row0, int rows) {
+#pragma unroll 8
+        for (int k = wave; k < rows; k += 4) {
+            const u32x4 v = load_piece((const T*)a.a + (row0 + k) * a.lda, c, a.I);
+            T e[8];
+            __builtin_memcpy(e, &v, 16);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += (float)e[j];
-    }
+            for (int j = 0; j < 8; ++j) sum[j] += (float)e[j];
+        }
+    });
     if (wave)
 #pragma unroll
         for (int j = 0; j < 8; ++j) part[wave - 1][lane][j] = sum[j];
@@ -686,8 +613,8 @@ static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
     Sum* cp = (Sum*)parts + spans * a.I * a.J;
     const dim3 grid((unsigned)(spans * ti * tj)), block(64 * WI * WJ);
-    // runs of a few steps at least are worth starting the LDS-DMA for
-    const bool together = (!a.rowmap || a.sg.rows / a.sg.S >= 4 * KB) && std::max(a.lda, a.ldb) * KB * (int64_t)sizeof(T) < (1ll << 31);
+    // (with rowmap the segments are short: rows_together)
+    const bool together = !a.rowmap && std::max(a.lda, a.ldb) * KB * (int64_t)sizeof(T) < (1ll << 31);
     if (together) LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, true>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
     else LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, false>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
     return split ? join_t<T>(ctx, a, ts, parts, cp) : 0;
@@ -724,7 +651,7 @@ static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     if (a.I <= 32) return launch_sum<T, 32, 128, 1, 4>(ctx, a, name);
     if (a.J <= 32) return launch_sum<T, 128, 32, 4, 1>(ctx, a, name);
     if constexpr (sizeof(T) == 2) {
-        if ((int64_t)(a.I / 256) * (a.J / 256) * std::max<int64_t>(a.groups, a.sg.rows >> 11) >= 128 && (!a.rowmap || a.sg.rows / a.sg.S >= 512) &&
+        if ((int64_t)(a.I / 256) * (a.J / 256) * std::max<int64_t>(a.groups, a.sg.rows >> 11) >= 128 && (!a.place || a.sg.rows / a.sg.S >= 512) &&
             std::max(a.lda, a.ldb) * 128 < (1ll << 31))
             return launch_sum_deep<T>(ctx, a, name);
         if (a.I > 64 && a.J > 64) return launch_sum<T, 128, 128, 2, 2>(ctx, a, name);

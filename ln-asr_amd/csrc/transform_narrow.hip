@@ -231,16 +231,10 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
     char* as = lds_all + wave * wave_lds;
     char* bs = as + (a_bytes + 15) / 16 * 16;
     const int64_t t = die_order(blockIdx.x, gridDim.x);
-    auto clamped = [&](int g) {
-        const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
-        return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
-    };
-    const int g = wave_search(a.groups, t, [&](int i) { return (clamped(i) >> ts) + i; });
-    if (g < 0) return;
-    const int64_t go = clamped(g), ge = max(go, clamped(g + 1)), span = t - ((go >> ts) + g), q0 = go + (span << ts);
-    if (span > 0 && q0 >= ge) return;
-    const int n = (int)min(ge - q0, (int64_t)1 << ts);
-    const bool whole = go + (1ll << ts) >= ge;
+    int g, n;
+    int64_t q0;
+    bool whole;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
 
     typename M::Acc acc[IF][JF];
 #pragma unroll
@@ -250,16 +244,19 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
 
     Chunk<T, HA> an;
     Chunk<T, HB> bn;
-    // R rows from place k of the span that lie together, or -1: (wave-uniform)
+    // the segment (of the sorted ones) of the place looked at last, and of the one after that
+    int seg = a.place ? max(0, wave_search(a.sg.S, q0, [&](int j) { return a.place[j]; })) : 0;
+    auto row_at = [&](int64_t q, int i) -> int64_t {
+        if (!a.place) return q;
+        while (i + 1 < a.sg.S && a.place[i + 1] <= q) ++i;
+        return seg_off(a.sg, a.ord[i]) + min(q, a.place[i + 1]) - a.place[i];
+    };
+    // first of the R rows from place k of the span on, -1 if they do not lie together (the same for every lane)
     auto run_at = [&](int k) -> int64_t {
         if (k + R > n) return -1;
-        if (!a.rowmap) return q0 + k;
-        const int64_t lo = a.rowmap[q0 + k], hi = a.rowmap[q0 + k + R - 1];
-        // (a run may wrap out of and back into a segment's rows only if it holds them all in order: the map is a permutation
-        // that keeps the order within a segment, so equal distance alone is not enough -- every lane checks its row)
-        const int64_t mine = a.rowmap[q0 + k + (lane & (R - 1))];
-        const bool fits = hi - lo == R - 1 && mine == lo + (lane & (R - 1));
-        return __all(fits) ? lo : (int64_t)-1;
+        if (!a.place) return q0 + k;
+        while (seg + 1 < a.sg.S && a.place[seg + 1] <= q0 + k) ++seg;
+        return q0 + k + R <= a.place[seg + 1] ? seg_off(a.sg, a.ord[seg]) + q0 + k - a.place[seg] : (int64_t)-1;
     };
     auto fetch = [&](int64_t row) {                        // (R rows of the array: nothing past its end)
         an.load((const char*)a.a + row * I * SZ, a_bytes);
@@ -267,6 +264,7 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
     };
     int k0 = wave * R;
     int64_t row = k0 < n ? run_at(k0) : -1;
+    int here = seg;
     if (row >= 0) fetch(row);
     for (; k0 < n; k0 += 4 * R) {
         if (row >= 0) {
@@ -275,12 +273,12 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
         } else {                                           // the span's last rows, or rows that lie apart: one value at a time
             for (int e = lane; e < R * I; e += 64) {
                 const int k = e / I;
-                const int64_t at = k0 + k < n ? (a.rowmap ? a.rowmap[q0 + k0 + k] : q0 + k0 + k) : -1;
+                const int64_t at = k0 + k < n ? row_at(q0 + k0 + k, here) : -1;
                 *(T*)(as + e * SZ) = at >= 0 ? ((const T*)a.a)[at * I + e - k * I] : (T)0;
             }
             for (int e = lane; e < R * J; e += 64) {
                 const int k = e / J;
-                const int64_t at = k0 + k < n ? (a.rowmap ? a.rowmap[q0 + k0 + k] : q0 + k0 + k) : -1;
+                const int64_t at = k0 + k < n ? row_at(q0 + k0 + k, here) : -1;
                 *(T*)(bs + e * SZ) = at >= 0 ? ((const T*)a.b)[at * J + e - k * J] : (T)0;
             }
         }
@@ -288,6 +286,7 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
         const int k1 = k0 + 4 * R;
         if (k1 < n) {
             row = run_at(k1);
+            here = seg;
             if (row >= 0) fetch(row);
         }
 #pragma unroll
