@@ -25,10 +25,10 @@ struct Mat<double> {
     using Acc = f64x4;
     using Sum = double;
     static constexpr int E = 2;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+    static constexpr int PARTS = 2;
+    static __device__ __forceinline__ Acc part(u32x4 a, u32x4 b, Acc c, int j) {
         const f64x2 x = __builtin_bit_cast(f64x2, a), y = __builtin_bit_cast(f64x2, b);
-        c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[0], y[0], c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f64_16x16x4f64(x[1], y[1], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f64_16x16x4f64(x[j], y[j], c, 0, 0, 0);
     }
     static __device__ __forceinline__ int row(int r, int kk) { return 4 * r + kk; }
 };
@@ -37,11 +37,10 @@ struct Mat<float> {
     using Acc = f32x4;
     using Sum = float;
     static constexpr int E = 4;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+    static constexpr int PARTS = 4;
+    static __device__ __forceinline__ Acc part(u32x4 a, u32x4 b, Acc c, int j) {
         const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-        return c;
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
     }
     static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
 };
@@ -50,7 +49,8 @@ struct Mat<_Float16> {
     using Acc = f32x4;
     using Sum = float;
     static constexpr int E = 8;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ Acc part(u32x4 a, u32x4 b, Acc c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
@@ -60,11 +60,29 @@ struct Mat<__bf16> {
     using Acc = f32x4;
     using Sum = float;
     static constexpr int E = 8;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ Acc part(u32x4 a, u32x4 b, Acc c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
 };
+
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::Acc mma(u32x4 a, u32x4 b, typename Mat<T>::Acc c) {
+#pragma unroll
+    for (int j = 0; j < Mat<T>::PARTS; ++j) c = Mat<T>::part(a, b, c, j);
+    return c;
+}
+// acc[i][j] += a[i] b[j]: the instructions of one piece in turns over all of acc, so that none waits for the one before
+template <typename T, int I, int J>
+__device__ __forceinline__ void mma_all(const u32x4 (&a)[I], const u32x4 (&b)[J], typename Mat<T>::Acc (&acc)[I][J]) {
+#pragma unroll
+    for (int p = 0; p < Mat<T>::PARTS; ++p)
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[i][j] = Mat<T>::part(a[i], b[j], acc[i][j], p);
+}
 
 // Segments of rows.  offsets may come from device memory that the host has not looked at: every value is brought into
 // [0, rows] before it is used, so that an offset out of order gives meaningless numbers but no access out of range.

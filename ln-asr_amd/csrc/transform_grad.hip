@@ -225,13 +225,10 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
             for (int i = 0; i < IR; ++i) af[i] = strided_fragment<T, TI>(as, h, wi + 16 * i);
 #pragma unroll
             for (int j = 0; j < JR; ++j) bf[j] = strided_fragment<T, TJ>(bs, h, wj + 16 * j);
-#pragma unroll
-            for (int i = 0; i < IR; ++i)
-#pragma unroll
-                for (int j = 0; j < JR; ++j) acc[i][j] = M::mma(af[i], bf[j], acc[i][j]);
+            mma_all<T>(af, bf, acc);
             if (want_col)
 #pragma unroll
-                for (int i = 0; i < IR; ++i) col[i] = M::mma(af[i], ones, col[i]);
+                for (int i = 0; i < IR; ++i) col[i] = mma<T>(af[i], ones, col[i]);
         }
     };
     // a step through registers: row(k) of its k-th place, for k < left; zeros for the others and past the last column
@@ -400,7 +397,7 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
 #pragma unroll
         for (int i = 0; i < IR; ++i)
 #pragma unroll
-            for (int j = 0; j < JR; ++j) acc[i][j] = M::mma(f.a[i], f.b[j], acc[i][j]);
+            for (int j = 0; j < JR; ++j) acc[i][j] = mma<T>(f.a[i], f.b[j], acc[i][j]);
     };
     unsigned ao[4], bo[4];
 #pragma unroll

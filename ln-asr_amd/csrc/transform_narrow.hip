@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, NF * HF <= 15 ? 3 : 1) void rows_narrow(RowsAr
         for (int n = 0; n < NF; ++n) {
             typename M::Acc acc = typename M::Acc{0, 0, 0, 0};
 #pragma unroll
-            for (int h = 0; h < HF; ++h) acc = M::mma(wf[n][h], xf[h], acc);
+            for (int h = 0; h < HF; ++h) acc = mma<T>(wf[n][h], xf[h], acc);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int c = 16 * n + M::row(r, kk);
@@ -311,10 +311,7 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
                     for (int j = 0; j < E; ++j) e[j] = l15 == (J & 15) ? (T)1 : e[j];
                 __builtin_memcpy(&bf[i], e, 16);
             }
-#pragma unroll
-            for (int i = 0; i < IF; ++i)
-#pragma unroll
-                for (int j = 0; j < JF; ++j) acc[i][j] = M::mma(af[i], bf[j], acc[i][j]);
+            mma_all<T>(af, bf, acc);
         }
         wave_lds_order();
     }

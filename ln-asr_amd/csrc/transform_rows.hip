@@ -51,7 +51,7 @@ __device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, in
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
                         // chosen, not masked by a product with zero: another row's adapter may hold a NaN
-                        const typename M::Acc d = M::mma(wf[n], pf, acc[n][m]);
+                        const typename M::Acc d = mma<T>(wf[n], pf, acc[n][m]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
                     }
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 #pragma unroll
         for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-            for (int m = 0; m < MR; ++m) acc[0][m] = M::mma(wf[d], xf[d][m], acc[0][m]);
+            for (int m = 0; m < MR; ++m) acc[0][m] = mma<T>(wf[d], xf[d][m], acc[0][m]);
     }
     if (LOW) add_adapters<T, KN, MR, 1>(a, r0, r1, c0, wave, WAVES, acc);
     if (wave) {
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 }
 
 // ------------------------------------------------------------------------------------------
-// Tiles of TM rows x TN results, WM x WN waves.  Both operands pass through LDS in steps of 128 bytes of k, double buffered, as
+// Tiles of TM rows x TN results, WM x WN waves.  Both operands pass through LDS in steps of 128 bytes of k, two steps ahead, as
 // 16-byte pieces in the order of the threads that bring them (LDS-DMA, buffer_load ... lds, needs just that; its addresses need
 // no alignment, so rows of 351 values take it too).  Which piece a thread brings is chosen so that the reads of a fragment spread
 // over the banks:
@@ -206,8 +206,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     constexpr int XB = TM * 128, WB = TN * 128, XI = TM * 8 / NT, WI = (TN * 8 + NT - 1) / NT;
     constexpr int LINE = TN * SZ / 16;                                                // pieces of a line of w [k, n]
     static_assert(TM * 8 % NT == 0 && TN * 8 % 64 == 0, "whole waves of pieces");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (XB + WB)];
-    static_assert(WM * WN * put_scratch<T, NR>() <= 2 * (XB + WB), "put_tile's rows");
+    // (three variables, not one array: the compiler then knows that reading one does not wait for what is brought into another)
+    __shared__ __attribute__((aligned(1024))) char l0[XB + WB], l1[XB + WB], l2[XB + WB];
+    constexpr int PUTS = (XB + WB) / put_scratch<T, NR>();                            // put_tile's rows: waves a buffer has room for
+    static_assert(3 * PUTS >= WM * WN && PUTS > 0, "put_tile's rows");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
     const unsigned id = die_order(blockIdx.x, gridDim.x);
@@ -236,10 +238,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 #pragma unroll
         for (int m = 0; m < MR; ++m) acc[n][m] = Acc{0, 0, 0, 0};
 
-    // acc += X W' over the 128 bytes of k in buffer buf; with SOME only for the rows from .. to - 1 of the wave's
-    auto multiply = [&](int buf, auto some, int from, int to) {
+    // acc += X W' over the 128 bytes of k in a buffer; with SOME only for the rows from .. to - 1 of the wave's
+    auto multiply = [&](const char* xs, auto some, int from, int to) {
         constexpr bool SOME = decltype(some)::value;
-        const char* xs = lds + buf * (XB + WB);
         const char* ws = xs + XB;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -252,12 +253,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             }
 #pragma unroll
             for (int m = 0; m < MR; ++m) xf[m] = *(const u32x4*)(xs + (wm + 16 * m + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
-            if constexpr (!SOME) {
-#pragma unroll
-                for (int n = 0; n < NR; ++n)
-#pragma unroll
-                    for (int m = 0; m < MR; ++m) acc[n][m] = M::mma(wf[n], xf[m], acc[n][m]);
-            } else
+            if constexpr (!SOME) mma_all<T>(wf, xf, acc);
+            else
 #pragma unroll
             for (int m = 0; m < MR; ++m) {
                 if (to <= 16 * m || from >= 16 * m + 16) continue;
@@ -266,13 +263,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
                     const bool in = 16 * m + l15 >= from && 16 * m + l15 < to;
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
-                        const Acc d = M::mma(wf[n], xf[m], acc[n][m]);
+                        const Acc d = mma<T>(wf[n], xf[m], acc[n][m]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
                     }
                 } else {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) acc[n][m] = M::mma(wf[n], xf[m], acc[n][m]);
+                    for (int n = 0; n < NR; ++n) acc[n][m] = mma<T>(wf[n], xf[m], acc[n][m]);
                 }
             }
         }
@@ -299,12 +296,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             }
         }
 #pragma unroll
-        for (int i = 0; i < XI; ++i) *(u32x4*)(lds + (tid + NT * i) * 16) = xr[i];
+        for (int i = 0; i < XI; ++i) *(u32x4*)(l0 + (tid + NT * i) * 16) = xr[i];
 #pragma unroll
         for (int i = 0; i < WI; ++i)
-            if (brings_w(i)) *(u32x4*)(lds + XB + (tid + NT * i) * 16) = wr[i];
+            if (brings_w(i)) *(u32x4*)(l0 + XB + (tid + NT * i) * 16) = wr[i];
         __syncthreads();
-        multiply(0, some, from, to);
+        multiply(l0, some, from, to);
         __syncthreads();
     };
 
@@ -329,8 +326,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         }
         const char* xb = (const char*)x;
         const char* wb = (const char*)(KN ? w + n0 : w + (int64_t)n0 * ldw);
-        auto bring = [&](int buf) {
-            char* xs = lds + buf * (XB + WB);
+        auto bring = [&](char* xs) {
 #pragma unroll
             for (int i = 0; i < XI; ++i) bring_piece(xb, xo[i], xs + (wave * 64 + NT * i) * 16);
 #pragma unroll
@@ -339,13 +335,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             xb += KB * SZ;
             wb += KN ? KB * ldw * SZ : KB * SZ;
         };
-        bring(0);
-        __syncthreads();
-        for (int i = 0; i < full; ++i) {
-            if (i + 1 < full) bring((i + 1) & 1);
-            multiply(i & 1, std::false_type{}, 0, 0);
-            __syncthreads();
+        bring(l0);
+        if (full > 1) bring(l1);
+        // At the barrier this step has arrived for every wave, and every wave is done with the step before, whose buffer takes the
+        // step after next; the next one's requests (a wave's XI of x, and its WI of w) may still be out.
+        auto turn = [&](int i, const char* now, char* free) {
+            if (i + 1 >= full) __builtin_amdgcn_s_waitcnt(0x0070);                    // vmcnt(0) lgkmcnt(0)
+            else if (brings_w(WI - 1)) __builtin_amdgcn_s_waitcnt(0x0070 | (XI + WI));
+            else __builtin_amdgcn_s_waitcnt(0x0070 | (XI + WI - 1));
+            __builtin_amdgcn_s_barrier();
+            if (i + 2 < full) bring(free);
+            multiply(now, std::false_type{}, 0, 0);
+        };
+        static_assert(XI + WI < 16, "a wait's low counter");
+        for (int i = 0; i < full; i += 3) {
+            turn(i, l0, l2);
+            if (i + 1 < full) turn(i + 1, l1, l0);
+            if (i + 2 < full) turn(i + 2, l2, l1);
         }
+        __syncthreads();
     }
     for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, std::false_type{}, 0, 0);
 
@@ -365,7 +373,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
     put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
-                        lds + wave * put_scratch<T, NR>());
+                        (wave < PUTS ? l0 : wave < 2 * PUTS ? l1 : l2) + wave % PUTS * put_scratch<T, NR>());
 }
 
 // ------------------------------------------------------------------------------------------
@@ -426,7 +434,7 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
 #pragma unroll
         for (int m = 0; m < MR; ++m)
 #pragma unroll
-            for (int n = 0; n < NR; ++n) acc[n][m] = M::mma(f.w[n], f.x[m], acc[n][m]);
+            for (int n = 0; n < NR; ++n) acc[n][m] = mma<T>(f.w[n], f.x[m], acc[n][m]);
     };
     // rows from .. to - 1 of the wave's only
     auto multiply_some = [&](const Frags& f, int from, int to) {
@@ -438,13 +446,13 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
                 const bool in = 16 * m + l15 >= from && 16 * m + l15 < to;
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    const Acc d = M::mma(f.w[n], f.x[m], acc[n][m]);
+                    const Acc d = mma<T>(f.w[n], f.x[m], acc[n][m]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
                 }
             } else {
 #pragma unroll
-                for (int n = 0; n < NR; ++n) acc[n][m] = M::mma(f.w[n], f.x[m], acc[n][m]);
+                for (int n = 0; n < NR; ++n) acc[n][m] = mma<T>(f.w[n], f.x[m], acc[n][m]);
             }
         }
     };
@@ -638,20 +646,13 @@ static int launch_few(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     return 0;
 }
 
-template <typename T, int TN, bool KN, int LOW>
-static int rows_thin(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
-    // (128 rows a tile; 64 where that leaves the CUs short of blocks)
-    if (a.sg.rows / 128 + a.sg.S >= 4 * ctx->prop.multiProcessorCount) return launch_tile<T, 128, TN, 4, 1, KN, LOW>(ctx, a, name);
-    return launch_tile<T, 64, TN, 4, 1, KN, LOW>(ctx, a, name);
-}
-
 template <typename T, bool KN, int LOW>
 static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t cus = ctx->prop.multiProcessorCount, rows = a.sg.rows;
     if constexpr (LOW != 2) {
-        if (a.N <= 16) return rows_thin<T, 16, KN, LOW>(ctx, a, name);
-        if (a.N <= 32) return rows_thin<T, 32, KN, LOW>(ctx, a, name);
-        if (a.N <= 48) return rows_thin<T, 48, KN, LOW>(ctx, a, name);
+        if (a.N <= 16) return launch_tile<T, 64, 16, 4, 1, KN, LOW>(ctx, a, name);
+        if (a.N <= 32) return launch_tile<T, 64, 32, 4, 1, KN, LOW>(ctx, a, name);
+        if (a.N <= 48) return launch_tile<T, 64, 48, 4, 1, KN, LOW>(ctx, a, name);
         // 16 bits: the larger the tile the less it asks of the memory for its products (us, 64 x 64 / 128 x 128 / 256 x 256: 65,536 x
         // 2048 x 2048 1185 / 800 / 599; 16,384 x 1024 x 1024 65 / 57 / 46), as long as there is one for every CU.  32 and 64 bits
         // have time for that: 64 x 64 leaves the least over at the ends (f32 120,011 x 351 x 128 105 against 142 us, f64 16,384 x
@@ -672,9 +673,14 @@ static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         if (mean <= 32) return launch_few<T, KN, 2, 0>(ctx, a, name);
         return rows_t<T, KN, 0>(ctx, a, name);
     }
-    if (rows <= 16) return launch_few<T, KN, 1, 2>(ctx, a, name);
-    if (rows <= 32) return launch_few<T, KN, 2, 2>(ctx, a, name);
-    if (rows * a.N <= 64 * 16 * 2 * cus) return launch_few<T, KN, 4, 2>(ctx, a, name);
+    // up to two blocks of 64 x 16 for every CU; lower ones where that leaves CUs without (64 rows x 2048: 23.1 us with 64 rows a block,
+    // 15.4 with 32, 15.6 with 16)
+    if (rows * a.N <= 64 * 16 * 2 * cus) {
+        const int64_t wide = (a.N + 15) / 16;
+        if (rows <= 16 || (rows + 31) / 32 * wide < cus / 2) return launch_few<T, KN, 1, 2>(ctx, a, name);
+        if (rows <= 32 || (rows + 63) / 64 * wide < cus) return launch_few<T, KN, 2, 2>(ctx, a, name);
+        return launch_few<T, KN, 4, 2>(ctx, a, name);
+    }
     if (mean >= 64) return rows_t<T, KN, 1>(ctx, a, name);
     return rows_t<T, KN, 2>(ctx, a, name);
 }
