@@ -206,10 +206,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     constexpr int XB = TM * 128, WB = TN * 128, XI = TM * 8 / NT, WI = (TN * 8 + NT - 1) / NT;
     constexpr int LINE = TN * SZ / 16;                                                // pieces of a line of w [k, n]
     static_assert(TM * 8 % NT == 0 && TN * 8 % 64 == 0, "whole waves of pieces");
-    // (three variables, not one array: the compiler then knows that reading one does not wait for what is brought into another)
-    __shared__ __attribute__((aligned(1024))) char l0[XB + WB], l1[XB + WB], l2[XB + WB];
+    // Three buffers for 16 bits, whose products are over before a step's bytes come; two for the others, which gain more from the
+    // blocks that then fit beside each other (f32 120,011 x 351 x 128 with adapters: 137 against 128 us).
+    // (variables of their own, not one array: the compiler then knows that reading one does not wait for what is brought into another)
+    constexpr bool THREE = SZ == 2;
+    __shared__ __attribute__((aligned(1024))) char l0[XB + WB], l1[XB + WB], l2[THREE ? XB + WB : 16];
     constexpr int PUTS = (XB + WB) / put_scratch<T, NR>();                            // put_tile's rows: waves a buffer has room for
-    static_assert(3 * PUTS >= WM * WN && PUTS > 0, "put_tile's rows");
+    static_assert((THREE ? 3 : 2) * PUTS >= WM * WN && PUTS > 0, "put_tile's rows");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
     const unsigned id = die_order(blockIdx.x, gridDim.x);
@@ -275,13 +278,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         }
     };
 
-    // one step through registers: what lies past klen (or, in a line of w, past N) is 0
-    auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen, auto some, int from, int to) {
-        u32x4 xr[XI], wr[WI];
+    // a step through registers: what lies past klen (or, in a line of w, past N) is 0
+    struct Pieces {
+        u32x4 x[XI], w[WI];
+    };
+    auto fetch = [&](Pieces& p, const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen) {
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             const int q = tid + NT * i, row = q >> 3;
-            xr[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ row) & 7) * E, klen);
+            p.x[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ row) & 7) * E, klen);
         }
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
@@ -289,17 +294,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             const int q = tid + NT * i;
             if (KN) {
                 const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
-                wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
+                p.w[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
             } else {
                 const int row = q >> 3;
-                wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
+                p.w[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
             }
         }
+    };
+    auto apply = [&](const Pieces& p, auto some, int from, int to) {
 #pragma unroll
-        for (int i = 0; i < XI; ++i) *(u32x4*)(l0 + (tid + NT * i) * 16) = xr[i];
+        for (int i = 0; i < XI; ++i) *(u32x4*)(l0 + (tid + NT * i) * 16) = p.x[i];
 #pragma unroll
         for (int i = 0; i < WI; ++i)
-            if (brings_w(i)) *(u32x4*)(l0 + XB + (tid + NT * i) * 16) = wr[i];
+            if (brings_w(i)) *(u32x4*)(l0 + XB + (tid + NT * i) * 16) = p.w[i];
         __syncthreads();
         multiply(l0, some, from, to);
         __syncthreads();
@@ -308,6 +315,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     const T* x = (const T*)a.x + r0 * a.ldx;
     const T* w = (const T*)a.w + (LOW ? 0 : slot * a.w_stride);
     const int64_t ldw = KN ? a.N : a.K;
+    // what comes behind the steps of the LDS-DMA, asked for before them: the last, uneven step, and the first adapter's first
+    Pieces rest, first;
+    if (full * KB < a.K) fetch(rest, x, a.ldx, w, ldw, full * KB, a.K);
+    // the first segment of the tile from s on that has rows in it and an adapter; a.sg.S: none
+    auto next_adapter = [&](int s, int64_t* lo, int64_t* hi, int* k) {
+        for (; s < a.sg.S; ++s) {
+            *lo = seg_off(a.sg, s);
+            *hi = seg_off(a.sg, s + 1);
+            if (*lo >= r1) break;
+            *k = seg_slot(a.sg, s);
+            if (*hi > r0 && *lo < *hi && *k >= 0) return s;
+        }
+        return a.sg.S;
+    };
+    const T* p = (const T*)a.p + r0 * a.ldp;
+    int64_t lo = 0, hi = 0;
+    int s = 0, k = 0;
+    if (LOW == 1) {
+        s = next_adapter(max(0, wave_search(a.sg.S, r0, [&](int i) { return seg_off(a.sg, i); })), &lo, &hi, &k);
+        if (s < a.sg.S) fetch(first, p, a.ldp, (const T*)a.low + k * a.low_stride, KN ? a.N : a.R, 0, a.R);
+    }
     if (full > 0) {
         // offsets of this lane's pieces from the step's first; out of range (nothing is read, LDS gets zeros) past the last column
         unsigned xo[XI], wo[WI];
@@ -336,37 +364,44 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             wb += KN ? KB * ldw * SZ : KB * SZ;
         };
         bring(l0);
-        if (full > 1) bring(l1);
+        if (THREE && full > 1) bring(l1);
         // At the barrier this step has arrived for every wave, and every wave is done with the step before, whose buffer takes the
-        // step after next; the next one's requests (a wave's XI of x, and its WI of w) may still be out.
+        // step after next; the next one's requests (a wave's XI of x, and its WI of w) may still be out.  (Two buffers: the next
+        // step is asked for only here, and waited for whole.)
         auto turn = [&](int i, const char* now, char* free) {
-            if (i + 1 >= full) __builtin_amdgcn_s_waitcnt(0x0070);                    // vmcnt(0) lgkmcnt(0)
+            if (!THREE || i + 1 >= full) __builtin_amdgcn_s_waitcnt(0x0070);          // vmcnt(0) lgkmcnt(0)
             else if (brings_w(WI - 1)) __builtin_amdgcn_s_waitcnt(0x0070 | (XI + WI));
             else __builtin_amdgcn_s_waitcnt(0x0070 | (XI + WI - 1));
             __builtin_amdgcn_s_barrier();
-            if (i + 2 < full) bring(free);
+            if (i + (THREE ? 2 : 1) < full) bring(free);
             multiply(now, std::false_type{}, 0, 0);
         };
         static_assert(XI + WI < 16, "a wait's low counter");
-        for (int i = 0; i < full; i += 3) {
-            turn(i, l0, l2);
-            if (i + 1 < full) turn(i + 1, l1, l0);
-            if (i + 2 < full) turn(i + 2, l2, l1);
+        if constexpr (THREE) {
+            for (int i = 0; i < full; i += 3) {
+                turn(i, l0, l2);
+                if (i + 1 < full) turn(i + 1, l1, l0);
+                if (i + 2 < full) turn(i + 2, l2, l1);
+            }
+        } else {
+            for (int i = 0; i < full; i += 2) {
+                turn(i, l0, l1);
+                if (i + 1 < full) turn(i + 1, l1, l0);
+            }
         }
         __syncthreads();
     }
-    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, std::false_type{}, 0, 0);
-
+    for (int k0 = full * KB; k0 < a.K; k0 += KB) {
+        if (k0 > full * KB) fetch(rest, x, a.ldx, w, ldw, k0, a.K);
+        apply(rest, std::false_type{}, 0, 0);
+    }
     if (LOW == 1) {
-        const T* p = (const T*)a.p + r0 * a.ldp;
-        for (int s = max(0, wave_search(a.sg.S, r0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; ++s) {
-            const int64_t lo = seg_off(a.sg, s), hi = seg_off(a.sg, s + 1);
-            if (lo >= r1) break;
-            const int k = seg_slot(a.sg, s);
-            if (hi <= r0 || lo >= hi || k < 0) continue;
-            const T* low = (const T*)a.low + k * a.low_stride;
+        for (bool waits = true; s < a.sg.S; waits = false, s = next_adapter(s + 1, &lo, &hi, &k)) {
             const int from = lo > r0 ? (int)(lo - r0) - wm : 0, to = hi < r1 ? (int)(hi - r0) - wm : TM;
-            for (int k0 = 0; k0 < a.R; k0 += KB) step(p, a.ldp, low, KN ? a.N : a.R, k0, a.R, std::true_type{}, from, to);
+            for (int k0 = 0; k0 < a.R; k0 += KB) {
+                if (!waits || k0 > 0) fetch(first, p, a.ldp, (const T*)a.low + k * a.low_stride, KN ? a.N : a.R, k0, a.R);
+                apply(first, std::true_type{}, from, to);
+            }
         }
     }
     if (LOW == 2) add_adapters<T, KN, MR, NR>(a, r0 + wm, r1, n0 + wn, 0, 1, acc);

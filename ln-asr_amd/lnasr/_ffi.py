@@ -276,8 +276,9 @@ def _in(x, dtype):
     return np.ascontiguousarray(x, dtype=dtype)
 
 
-# dtype codes of the feature transforms
+# dtype codes of the feature transforms, and the names of other libraries' dtypes as they are met
 _CODES = {"float64": F64, "float32": F32, "float16": F16, "bfloat16": BF16}
+_KINDS = {}
 
 
 class _Arg:
@@ -295,8 +296,11 @@ class _Arg:
         elif getattr(x, "is_cuda", False):
             if x.get_device() != ctx.device:
                 raise LnasrError("%s lies on device %d, the context on device %d" % (name, x.get_device(), ctx.device))
-            self.obj, self.ptr, self.shape, self.kind = x, x.data_ptr(), tuple(x.shape), str(x.dtype).replace("torch.", "")
-            self.ld = 1
+            dtype = x.dtype
+            kind = _KINDS.get(dtype)
+            if kind is None:
+                kind = _KINDS[dtype] = str(dtype).replace("torch.", "")
+            self.obj, self.ptr, self.shape, self.kind, self.ld = x, x.data_ptr(), tuple(x.shape), kind, 1
             if not ctx._tensors_checked:
                 # pointers of another copy of the HIP runtime mean nothing to this one
                 if self.ptr and lib().lnasr_debug_require_device_ptr(self.ptr) != 0:
