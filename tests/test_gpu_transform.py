@@ -76,6 +76,27 @@ def test_projection_grad(ctx, kind, size):
             ref.check(got[k], want[k], err[k], k)
 
 
+@pytest.mark.parametrize("size", [(9001, 840, 2056, 5, 4, 24), (17000, 72, 1032, 3, 2, 40), (16500, 1030, 270, 9, 3, 9),
+                                  (24000, 512, 520, 40, 32, 16)], ids=str)
+def test_wide_tiles(ctx, size):
+    """16-bit products wide and long enough for the largest tiles: k of several turns of the buffers, of one step and of less,
+    uneven edges, segments that end inside a tile."""
+    d = typed(ref.make(12, size, empties=False, negative=True), "float16")
+    y = ctx.projection(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["bias"], d["scale"], d["slots"])
+    ref.check(y, *ref.projection("float16", d["x"], d["offsets"], d["w"], d["a"], d["b"], d["bias"], d["scale"], d["slots"], d["y0"]), "projection")
+    got = ctx.projection_grad(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"])
+    want, err = ref.projection_grad("float16", d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"], d["dx0"])
+    for k in want:
+        ref.check(got[k], want[k], err[k], "projection_grad " + k)
+    d["slots"] = np.maximum(d["slots"], 0)
+    y = ctx.affine(d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"])
+    ref.check(y, *ref.affine("float16", d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], d["y0"]), "affine")
+    got = ctx.affine_grad(d["x"], d["offsets"], d["w3"], d["dy"], d["slots"])
+    want, err = ref.affine_grad("float16", d["x"], d["offsets"], d["w3"], d["dy"], d["slots"], d["dx0"])
+    for k in want:
+        ref.check(got[k], want[k], err[k], "affine_grad " + k)
+
+
 def test_gradients_against_differences(ctx):
     """The loss sum(y * c) is linear in each argument by itself: the central difference along a direction is the gradient's
     product with it but for rounding -- 64-bit sums of a few thousand terms of size one, divided by a step of 1/2."""
