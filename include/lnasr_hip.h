@@ -54,8 +54,6 @@ extern "C" {
 
 #define LNASR_F64 0
 #define LNASR_F32 1
-#define LNASR_F16 2    /* feature transforms only */
-#define LNASR_BF16 3   /* feature transforms only */
 
 #define LNASR_OK 0
 #define LNASR_E_INVALID (-1)   /* bad argument / shape */
@@ -74,12 +72,6 @@ int lnasr_device_count(int* out);
 int lnasr_ctx_create(int device_id, lnasr_ctx** out);
 void lnasr_ctx_destroy(lnasr_ctx* ctx);
 int lnasr_sync(lnasr_ctx* ctx);
-/* Sends the context's further calls to another stream of its device (a hipStream_t; NULL is the default stream), behind what
- * was enqueued so far; own != 0: back to the context's own stream.  For callers whose device arrays are produced on a stream
- * of theirs.  The stream has to live until the context is sent elsewhere or destroyed; refused while either stream is being
- * captured.  A call of the feature transforms on device memory may be captured into a graph once it has run (its workspaces
- * then exist and stay); graphs of one context share its workspaces and are replayed one after the other. */
-int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own);
 /* every stream of the context's device has drained (hipDeviceSynchronize): the bracket of a timed region */
 int lnasr_device_sync(lnasr_ctx* ctx);
 /* LNASR_* test / ablation switches are read once per process; this re-reads them from the environment.  Test-only:
@@ -292,40 +284,6 @@ int lnasr_mfcc(lnasr_ctx* ctx, const void* signal, int sample_kind, const int64_
  * (variable-length utterances batched by an offsets array).  row_offsets is a host array. */
 int lnasr_pad_rows(lnasr_ctx* ctx, const double* packed, const int64_t* row_offsets, int U, int W, int64_t pad_rows,
                    double* padded);
-
-/* ---- feature transforms --------------------------------------------------------------------
- * Between the features (lnasr_mfcc) and the bank (lnasr_decode ...): an affine transform per speaker or class, and a projection
- * that all rows share with a low-rank adapter per speaker beside it; with gradients.  The reference has none of these.
- *   Rows are packed; segment s (an utterance, a request) holds rows offsets[s] .. offsets[s + 1] - 1 of `rows` (offsets [S + 1]
- * int64, not falling; segments may be empty).  slots [S] int32 names the group (speaker) of each segment, several may name the
- * same one; NULL: segment s is group s, S == G.  Rows that belong to no segment are left as they were in y and dx.
- *   dtype: LNASR_F64, F32, F16 or BF16, the type of every matrix; sums are held in 64 bits for F64, in 32 for the others, and
- * rounded once.  ld*: elements from one row to the next.  No alignment is asked for beyond that of the type.
- *   Arrays may be host or device memory as everywhere; host offsets and slots are checked, device ones are brought into range
- * (values out of order then give numbers without meaning, no access out of bounds).  An output may not overlap an input or
- * another output.  With device arrays the call only enqueues. */
-
-/* y[r] = W[k] x[r] + bias[k], k the group of row r: x [rows, din], w [G, dout, din], bias [G, dout] or NULL, y [rows, dout].
- * A host slot outside [0, G) is refused, rows of such a device slot are left as they were. */
-int lnasr_affine(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
-                 const int32_t* slots_or_null, int S, const void* w, const void* bias_or_null, int G, int dout, void* y, int64_t ldy);
-/* From dy = dL/dy: dx[r] = W[k]^T dy[r], dw[k] = sum over the rows of group k of dy x^T, dbias[k] = sum of dy (a group without
- * rows: zeros).  Each may be NULL (dbias only with dw); x is read for dw only, w for dx only.  The sums run in the order of the
- * batch: the same bits every time. */
-int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
-                      const int32_t* slots_or_null, int S, const void* w, int G, int dout, const void* dy, int64_t lddy,
-                      void* dx_or_null, int64_t lddx, void* dw_or_null, void* dbias_or_null);
-/* y[r] = W x[r] + bias + scale[k] B[k] (A[k] x[r]): w [dout, din], bias [dout] or NULL, a [G, rank, din], b [G, dout, rank],
- * scale [G] fp64 or NULL (1).  Slot -1: the projection alone.  The middle (scale A x) is held in `dtype`. */
-int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
-                     const int32_t* slots_or_null, int S, const void* w, const void* bias_or_null, int dout, const void* a,
-                     const void* b, const double* scale_or_null, int G, int rank, void* y, int64_t ldy);
-/* dx = W^T dy + scale A^T B^T dy, da[k] = sum scale (B^T dy) x^T, db[k] = sum dy (scale A x)^T, dw = sum dy x^T over the rows of
- * all segments, dbias = sum dy.  Each may be NULL (dbias only with dw); an input that no wanted gradient needs is not read. */
-int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
-                          const int32_t* slots_or_null, int S, const void* w, int dout, const void* a, const void* b,
-                          const double* scale_or_null, int G, int rank, const void* dy, int64_t lddy, void* dx_or_null,
-                          int64_t lddx, void* da_or_null, void* db_or_null, void* dw_or_null, void* dbias_or_null);
 
 /* ---- multi-GPU (one process per GPU, RCCL over xGMI) --------------------------------- */
 #define LNASR_UNIQUE_ID_BYTES 128

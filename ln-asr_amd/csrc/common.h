@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/lnasr_hip.h"
+#include "../../include/lnasr_transform.h"
 
 namespace lnasr {
 

@@ -5,4 +5,4 @@ Same module / class / function surface as the reference package (`lnasr.hmm.HMM`
 `lnasr.recognizer.*`); the arithmetic runs in hand-written HIP kernels reached through a
 ctypes C-ABI (`include/lnasr_hip.h`).  No PyTorch, no CPU fallback.
 """
-__all__ = ["utils", "gmm", "hmm", "gmmhmm", "mfcc", "recognizer"]
+__all__ = ["utils", "gmm", "hmm", "gmmhmm", "mfcc", "transform", "recognizer"]

@@ -36,7 +36,6 @@ SIGNATURES = {
     "lnasr_ctx_create": [_i, _P(_vp)],
     "lnasr_ctx_destroy": [_vp],
     "lnasr_sync": [_vp],
-    "lnasr_ctx_use_stream": [_vp, _vp, _i],
     "lnasr_device_sync": [_vp],
     "lnasr_reload_switches": [],
     "lnasr_host_alloc": [_vp, _sz, _P(_vp)],
@@ -87,11 +86,6 @@ SIGNATURES = {
     "lnasr_split_frames": [_vp, _vp, _i64, _i, _i, _vp],
     "lnasr_mfcc": [_vp, _vp, _i, _vp, _i, _P(MfccCfgStruct), _vp, _vp, _vp, _vp, _vp],
     "lnasr_pad_rows": [_vp, _vp, _vp, _i, _i, _i64, _vp],
-    "lnasr_affine": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i64],
-    "lnasr_affine_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _vp],
-    "lnasr_projection": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64],
-    "lnasr_projection_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64,
-                              _vp, _vp, _vp, _vp],
     "lnasr_comm_unique_id": [_vp],
     "lnasr_comm_init": [_vp, _vp, _i, _i],
     "lnasr_comm_destroy": [_vp],
@@ -99,6 +93,15 @@ SIGNATURES = {
     "lnasr_allgather_u32": [_vp, _vp, _sz, _vp],
     "lnasr_allgather_paths": [_vp, _vp, _sz, _i, _vp],
     "lnasr_allreduce_f64": [_vp, _vp, _sz],
+}
+# the entry points of include/lnasr_transform.h
+TRANSFORM_SIGNATURES = {
+    "lnasr_ctx_use_stream": [_vp, _vp, _i],
+    "lnasr_affine": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i64],
+    "lnasr_affine_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _vp],
+    "lnasr_projection": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64],
+    "lnasr_projection_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64,
+                              _vp, _vp, _vp, _vp],
 }
 _RESTYPES = {"lnasr_last_error": C.c_char_p, "lnasr_ctx_destroy": None}
 
@@ -117,7 +120,7 @@ def lib():
                 raise LnasrError("%s not found: build it with `python ln-asr_amd/build.py` "
                                  "(there is no CPU fallback)" % _LIB_PATH)
             l = C.CDLL(_LIB_PATH)
-            for name, args in SIGNATURES.items():
+            for name, args in list(SIGNATURES.items()) + list(TRANSFORM_SIGNATURES.items()):
                 fn = getattr(l, name)
                 fn.argtypes = args
                 fn.restype = _RESTYPES.get(name, C.c_int)

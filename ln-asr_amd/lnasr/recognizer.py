@@ -11,6 +11,7 @@ import numpy as np
 
 from .mfcc import MFCC
 from .gmmhmm import GMMHMM
+from .transform import SpeakerTransforms
 
 
 class AcousticModel:
@@ -32,10 +33,15 @@ class Recognizer:
     def __init__(self, model: dict):
         self.am = AcousticModel(model["am"])
         self.lm = LanguageModel(model["lm"]) if model.get("lm") is not None else None
+        # "transform" (an extension): a file of SpeakerTransforms, applied between MFCC and decoding
+        self.transforms = None
+        if model.get("transform") is not None:
+            self.transforms = SpeakerTransforms()
+            self.transforms.load(model["transform"])
 
-    def recognize(self, data: np.ndarray):
+    def recognize(self, data: np.ndarray, speaker=0):
         """PCM samples (int16 as read_pcm returns them, utils.py:100-104, or float64) -> most likely HMM state sequence
-        (uint32 [Nf])."""
+        (uint32 [Nf]).  speaker: whose transform the features take, where the model has transforms."""
         data = np.ascontiguousarray(data)
         if data.dtype != np.int16:
             data = np.ascontiguousarray(data, dtype=np.float64)
@@ -44,4 +50,27 @@ class Recognizer:
         cfg, win, bank = mf._cfg()
         d_pcm = ctx.to_device(data)
         _, _, feat, _ = ctx.mfcc(d_pcm, np.array([0, len(data)], dtype=np.int64), cfg, win, bank, False, False)
+        if self.transforms is not None:
+            feat = self.transforms.apply(feat, np.array([0, feat.shape[0]], dtype=np.int64), np.array([speaker], dtype=np.int32))
         return gh.decode(feat)
+
+    def recognize_batch(self, utterances, speakers=None):
+        """Many utterances at once (all int16, or float64) -> a list of state sequences.  speakers: the speaker of each, where the
+        model has transforms (default: speaker 0).  Features, transforms, emissions and trellises stay in HBM."""
+        utterances = [np.asarray(u) for u in utterances]
+        if not utterances:
+            return []
+        dt = np.int16 if all(u.dtype == np.int16 for u in utterances) else np.float64
+        mf, gh = self.am.mfcc, self.am.gmmhmm
+        ctx = gh.ctx
+        cfg, win, bank = mf._cfg()
+        offsets = np.concatenate([[0], np.cumsum([len(u) for u in utterances])]).astype(np.int64)
+        d_pcm = ctx.to_device(np.concatenate(utterances).astype(dt))
+        _, _, feat, rows = ctx.mfcc(d_pcm, offsets, cfg, win, bank, False, False)
+        if self.transforms is not None:
+            speakers = np.zeros(len(utterances), dtype=np.int32) if speakers is None else np.asarray(speakers, dtype=np.int32)
+            feat = self.transforms.apply(feat, rows, speakers)
+        obs, lens = ctx.pad_rows(feat, rows)
+        gh.upload()
+        path = gh.decode_batch(obs, lens=lens).to_host()
+        return [path[u, :n] for u, n in enumerate(lens)]

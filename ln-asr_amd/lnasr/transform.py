@@ -15,6 +15,7 @@ With GPU tensors, choose their stream first (`ctx.use_stream`).
 import numpy as np
 
 from ._ffi import default_ctx
+from .hmm import _load, _save
 
 
 def affine(x, offsets, w, bias=None, slots=None, out=None, *, ctx=None):
@@ -39,3 +40,47 @@ def projection_grad(x, offsets, w, a, b, dy, scale=None, slots=None, want=("x", 
     """The gradients of `projection` by "x", "a", "b", "w" and "bias", as `affine_grad` returns them; leave "w" and "bias" out to
     train adapters beside a frozen projection."""
     return (ctx or default_ctx()).projection_grad(x, offsets, w, a, b, dy, scale, slots, want, out)
+
+
+class SpeakerTransforms:
+    """A bank of affine feature transforms, one per speaker: `w` [G, dout, din] and `bias` [G, dout] in float64, kept on the device.
+    `Recognizer` applies one between MFCC and decoding."""
+
+    def __init__(self, w=None, bias=None, *, ctx=None):
+        self._ctx = ctx
+        self._set(w, bias)
+
+    def _set(self, w, bias):
+        self._held = None
+        if w is None:
+            self.w = self.bias = None
+            return
+        self.w = np.ascontiguousarray(w, dtype=np.float64)
+        if self.w.ndim != 3:
+            raise ValueError("w must have shape (speakers, dout, din), got %s" % (self.w.shape,))
+        self.bias = np.zeros(self.w.shape[:2]) if bias is None else np.ascontiguousarray(bias, dtype=np.float64)
+        if self.bias.shape != self.w.shape[:2]:
+            raise ValueError("bias must have shape %s, got %s" % (self.w.shape[:2], self.bias.shape))
+
+    @property
+    def ctx(self):
+        if self._ctx is None:
+            self._ctx = default_ctx()
+        return self._ctx
+
+    def apply(self, features, offsets, speakers=None, out=None):
+        """Features [F, din] of utterances (rows offsets[u] .. offsets[u+1]-1, float64: a numpy array or a DeviceArray) -> [F, dout].
+        speakers [U]: the speaker of each; without it utterance u is speaker u's.  To change w or bias, make a new bank or `load`."""
+        if self.w is None:
+            raise ValueError("no transforms: give w, or load them")
+        if self._held is None:
+            self._held = (self.ctx.to_device(self.w), self.ctx.to_device(self.bias))
+        return self.ctx.affine(features, offsets, *self._held, slots=speakers, out=out)
+
+    def save(self, filename):
+        """Datasets 'w' and 'bias', in the files the models use."""
+        _save(filename, {"w": self.w, "bias": self.bias})
+
+    def load(self, filename):
+        d = _load(filename, ("w", "bias"))
+        self._set(d["w"], d["bias"])

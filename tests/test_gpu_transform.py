@@ -284,6 +284,61 @@ def test_long_group_is_joined(ctx):
         assert np.array_equal(g["w"][0], dy.T @ x) and np.array_equal(g["bias"][0], dy.sum(0))
 
 
+def test_recognizer_with_speaker_transforms(tmp_path, synth, oracle):
+    """MFCC -> speaker's transform -> decode, one utterance and a ragged batch, against the oracle's MFCC and decoding with the
+    transform written out between them."""
+    from lnasr.gmmhmm import GMMHMM
+    from lnasr.recognizer import Recognizer
+    from lnasr.transform import SpeakerTransforms
+    rng = np.random.default_rng(13)
+    pcm = [np.clip(synth.synth_signal(n, seed=30 + i) * 5, -32768, 32767).astype(np.int16) for i, n in enumerate((9000, 16000, 4400, 12345))]
+    with np.errstate(divide="ignore"):
+        feats = [oracle.mfcc(p.astype(np.float64))[2] for p in pcm]
+    w = np.eye(39) + 0.1 * rng.standard_normal((3, 39, 39))
+    bias = rng.standard_normal((3, 39))
+    speakers = [2, 0, 1, 2]
+    moved = [f @ w[k].T + bias[k] for f, k in zip(feats, speakers)]
+    every = np.concatenate(moved)
+    N, M, D = 8, 3, 39
+    m = synth.synth_model(N, M, D, seed=5)
+    pick = rng.choice(len(every), N * M, replace=False)
+    mu, var = every[pick].reshape(N, M, D), np.broadcast_to(every.var(0) * 0.5 + 1.0, (N, M, D))
+    si = np.zeros((N, M, D, D))
+    si[:, :, np.arange(D), np.arange(D)] = var
+    want = [oracle.decode_diag(f, m["A"], m["pi"], m["w"], mu, var) for f in moved]
+    assert min(len(set(p.tolist())) for p in want) >= 3                    # the paths move between states
+    GMMHMM(N, M, D, m["A"], m["pi"], m["w"], mu, si).save(str(tmp_path / "am.npz"))
+    SpeakerTransforms(w, bias).save(str(tmp_path / "speakers.npz"))
+    rec = Recognizer({"am": str(tmp_path / "am.npz"), "lm": None, "transform": str(tmp_path / "speakers.npz")})
+    for p, k, path in zip(pcm, speakers, want):
+        assert np.array_equal(rec.recognize(p, speaker=k), path)
+    got = rec.recognize_batch(pcm, speakers)
+    assert len(got) == 4 and all(np.array_equal(a, b) for a, b in zip(got, want))
+    plain = Recognizer({"am": str(tmp_path / "am.npz")})
+    assert plain.transforms is None
+    assert all(np.array_equal(a, plain.recognize(p)) for a, p in zip(plain.recognize_batch(pcm), pcm))
+    with pytest.raises(Exception, match="slots"):
+        rec.recognize(pcm[0], speaker=3)
+
+
+def test_calls_of_a_training_loop(ctx):
+    """Forward, gradients and a step on the speakers' transforms under a quadratic loss, in fp64: along the gradient the loss differs
+    by the gradient's square times the step, less the quadratic term, at every one of three steps."""
+    d = ref.make(14, (400, 39, 39, 8, 3, 4))
+    target = d["y0"]
+    loss = lambda w, c: 0.5 * float(((ctx.affine(d["x"], d["offsets"], w, c, d["slots"]) - target) ** 2).sum())
+    w, c = d["w3"].copy(), d["bias2"].copy()
+    for _ in range(3):
+        r = ctx.affine(d["x"], d["offsets"], w, c, d["slots"]) - target
+        g = ctx.affine_grad(d["x"], d["offsets"], w, r, d["slots"], want=("w", "bias"))
+        n = float((g["w"] ** 2).sum() + (g["bias"] ** 2).sum())
+        curve = float((ctx.affine(d["x"], d["offsets"], g["w"], g["bias"], d["slots"]) ** 2).sum())
+        h, before = 1e-4, loss(w, c)
+        after = loss(w - h * g["w"], c - h * g["bias"])
+        assert abs(before - after - (h * n - 0.5 * h * h * curve)) <= 1e-10 * before
+        w, c = w - n / curve * g["w"], c - n / curve * g["bias"]
+
+
 def test_refusals(ctx):
     from lnasr import _ffi
     x, w, off = np.zeros((6, 4)), np.zeros((2, 3, 4)), np.array([0, 2, 6])

@@ -1,9 +1,13 @@
 """CPU: the feature transforms' entry points refuse before they touch a device; the plain forms of the GPU tests agree with
 central differences and notice a planted mistake."""
+import os
+import re
+
 import numpy as np
 import pytest
 
 import _transform_ref as ref
+from conftest import REPO
 
 
 def test_entry_points_refuse_a_null_context():
@@ -17,6 +21,17 @@ def test_entry_points_refuse_a_null_context():
                                    None, None, None) == -1
     assert b"null ctx" in l.lnasr_last_error()
     assert l.lnasr_ctx_use_stream(None, None, 1) == -1
+
+
+def test_table_matches_the_header():
+    from lnasr import _ffi
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(REPO, "include", "lnasr_transform.h")).read(), flags=re.S)
+    assert sorted(_ffi.TRANSFORM_SIGNATURES) == sorted(set(re.findall(r"\b(lnasr_[a-z0-9_]+)\s*\(", text)))
+    assert not set(_ffi.TRANSFORM_SIGNATURES) & set(_ffi.SIGNATURES)
+    for name, args in _ffi.TRANSFORM_SIGNATURES.items():                            # one type for each declared argument
+        declared = re.search(r"\b%s\s*\(([^)]*)\)" % name, text).group(1)
+        assert len(args) == declared.count(",") + 1, name
+        assert hasattr(_ffi.lib(), name)
 
 
 class _Ctx:
