@@ -206,10 +206,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     constexpr int XB = TM * 128, WB = TN * 128, XI = TM * 8 / NT, WI = (TN * 8 + NT - 1) / NT;
     constexpr int LINE = TN * SZ / 16;                                                // pieces of a line of w [k, n]
     static_assert(TM * 8 % NT == 0 && TN * 8 % 64 == 0, "whole waves of pieces");
-    // Three buffers for 16 bits, whose products are over before a step's bytes come; two for the others, which gain more from the
-    // blocks that then fit beside each other (f32 120,011 x 351 x 128 with adapters: 137 against 128 us).
+    // Three buffers for 16 bits, whose products are over before a step's bytes come; two for the others and for the large tile, which
+    // gain more from the blocks that then fit beside each other (f32 120,011 x 351 x 128 with adapters: 137 against 128 us).
     // (variables of their own, not one array: the compiler then knows that reading one does not wait for what is brought into another)
-    constexpr bool THREE = SZ == 2;
+    constexpr bool THREE = SZ == 2 && 3 * (XB + WB) <= (160 << 10) / 3;
     __shared__ __attribute__((aligned(1024))) char l0[XB + WB], l1[XB + WB], l2[THREE ? XB + WB : 16];
     constexpr int PUTS = (XB + WB) / put_scratch<T, NR>();                            // put_tile's rows: waves a buffer has room for
     static_assert((THREE ? 3 : 2) * PUTS >= WM * WN && PUTS > 0, "put_tile's rows");
