@@ -20,7 +20,8 @@ extern "C" {
  * was enqueued so far; own != 0: back to the context's own stream.  For callers whose device arrays are produced on a stream
  * of theirs.  The stream has to live until the context is sent elsewhere or destroyed; refused while either stream is being
  * captured.  A call of the feature transforms on device memory may be captured into a graph once it has run (its workspaces
- * then exist and stay); graphs of one context share its workspaces and are replayed one after the other. */
+ * then exist and stay, after the context is destroyed too); it is left out of the profile.  Graphs of one context share its
+ * workspaces: a replay, other replays and the context's own calls run one after the other, as on one stream. */
 int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own);
 
 /*
@@ -33,7 +34,8 @@ int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own);
  * rounded once.  ld*: elements from one row to the next.  No alignment is asked for beyond that of the type.
  *   Arrays may be host or device memory as everywhere; host offsets and slots are checked, device ones are brought into range
  * (values out of order then give numbers without meaning, no access out of bounds).  An output may not overlap an input or
- * another output.  With device arrays the call only enqueues. */
+ * another output, from its first element to its last (columns of one buffer beside each other do).  With device arrays the call
+ * only enqueues.  Threads may share a context: their calls run one after the other. */
 
 /* y[r] = W[k] x[r] + bias[k], k the group of row r: x [rows, din], w [G, dout, din], bias [G, dout] or NULL, y [rows, dout].
  * A host slot outside [0, G) is refused, rows of such a device slot are left as they were. */

@@ -9,6 +9,7 @@
 #include <cstring>
 #include <map>
 #include <string>
+#include <mutex>
 #include <vector>
 
 #include "../../include/lnasr_hip.h"
@@ -200,10 +201,11 @@ struct lnasr_ctx {
     size_t mfcc_meta_cap = 0;                              // ... in elements
     hipEvent_t mfcc_meta_ev = nullptr;                     // the upload that last read mfcc_meta
     // feature transforms (transform.hip): workspaces, grow-only.  Once a stream of this context has been captured into a graph,
-    // a buffer that has to grow is kept in `tr_retired` instead of being freed: a replay may still use it
+    // none is freed any more, not with the context either: a replay may still use it.  One call at a time (tr_mutex): its
+    // launches share the workspaces and must follow one another on the stream
     lnasr::DevBuf tr_ws[18];
-    std::vector<void*> tr_retired;
     bool tr_captured = false;
+    std::mutex tr_mutex;
     // profiling
     bool prof_on = false;
     std::vector<std::string> prof_names;
@@ -218,6 +220,16 @@ struct lnasr_ctx {
 
 namespace lnasr {
 
+// Leaves the thread's device as it was: the caller may use others beside the context's
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(lnasr_ctx* ctx) {
+        if (ctx && hipGetDevice(&before) != hipSuccess) before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
 // LN_LAUNCH (and its profiling events) follow ctx->stream: device helpers are sent to another stream of the context
 // by this guard, which puts the stream back on EVERY way out of the scope (an early return through LN_TRY included)
 struct StreamScope {

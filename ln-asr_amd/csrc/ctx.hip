@@ -309,8 +309,9 @@ void lnasr_ctx_destroy(lnasr_ctx* ctx) {
                      &ctx->ws_out3, &ctx->ws_b, &ctx->ws_bm, &ctx->ws_v, &ctx->ws_alpha, &ctx->ws_beta,
                      &ctx->ws_misc, &ctx->ws_misc2, &ctx->ws_lens, &ctx->ws_stats, &ctx->ws_p, &ctx->ws_q, &ctx->ws_raw, &ctx->ws_w1, &ctx->ws_w2, &ctx->ws_w3, &ctx->ws_pad, &ctx->ws_bp, &ctx->ws_btb, &ctx->ws_clock, &ctx->ws_fs, &ctx->ws_lvl, &ctx->ws_lvl2, &ctx->mfcc_const, &ctx->nan_flag, &ctx->nan_slots};
     for (DevBuf* b : all) b->release();
-    for (DevBuf& b : ctx->tr_ws) b.release();
-    for (void* p : ctx->tr_retired) (void)hipFree(p);
+    // (what a graph may replay is left to the process: a replay on freed memory would be a fault of the GPU)
+    if (!ctx->tr_captured)
+        for (DevBuf& b : ctx->tr_ws) b.release();
     for (auto& r : ctx->prof_recs) {
         (void)hipEventDestroy(r.e0);
         (void)hipEventDestroy(r.e1);
@@ -338,8 +339,10 @@ int lnasr_sync(lnasr_ctx* ctx) {
 }
 
 int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own) {
-    LN_ENTER(ctx);
     LN_REQUIRE(ctx, "null ctx");
+    DeviceScope scope(ctx);
+    LN_ENTER(ctx);
+    const std::lock_guard<std::mutex> lock(ctx->tr_mutex);
     const hipStream_t to = own ? ctx->own_stream : (hipStream_t)stream;
     if (to == ctx->stream) return 0;
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -349,6 +352,9 @@ int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own) {
             return fail(LNASR_E_INVALID, "a stream is being captured: choose the context's stream before the capture begins");
         }
     }
+    hipDevice_t of = ctx->device;
+    if (to) LN_HIP(hipStreamGetDevice(to, &of));
+    LN_REQUIRE(of == ctx->device, "a stream of device %d, the context is on device %d", (int)of, ctx->device);
     // what was enqueued so far comes first: the context's workspaces are shared by both streams
     LN_HIP(hipEventRecord(ctx->ev_fork, ctx->stream));
     LN_HIP(hipStreamWaitEvent(to, ctx->ev_fork, 0));

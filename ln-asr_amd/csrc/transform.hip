@@ -1,6 +1,7 @@
 // Feature transforms: entry points.  Checks, staging of host arrays and the sequence of products; the kernels are in
 // transform_rows.hip and transform_grad.hip.
 #include <algorithm>
+#include <exception>
 
 #include "transform.h"
 
@@ -14,10 +15,9 @@ int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out) {
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         LN_HIP(hipStreamIsCapturing(ctx->stream, &st));
         LN_REQUIRE(st == hipStreamCaptureStatusNone, "a workspace of %zu bytes cannot be allocated while the stream is captured: run the call once before", bytes);
-        if (ctx->tr_captured && b.p) {
-            ctx->tr_retired.push_back(b.p);
-            b.p = nullptr;
-            b.cap = 0;
+        if (ctx->tr_captured) {                           // (left to the graphs; twice as large, so that few are)
+            bytes = std::max(bytes, 2 * b.cap);
+            b = DevBuf();
         }
         LN_TRY(b.reserve(bytes));
     }
@@ -27,19 +27,8 @@ int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out) {
 
 namespace {
 
-// Leaves the thread's device as it was: the caller may use others beside the context's
-struct DeviceScope {
-    int before = -1;
-    explicit DeviceScope(lnasr_ctx* ctx) {
-        if (ctx && hipGetDevice(&before) != hipSuccess) before = -1;
-    }
-    ~DeviceScope() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
 struct Call {
-    lnasr_ctx* ctx;
+    lnasr_ctx* const ctx;
     bool capturing = false;
     struct Range { const char *lo, *hi; bool out; const char* what; };
     Range ranges[16];
@@ -47,13 +36,26 @@ struct Call {
     struct Back { void* host; void* dev; size_t bytes; };
     Back back[5];
     int nback = 0;
+    bool pinned = false;                                  // a copy from pinned host memory is on its way
+    std::unique_lock<std::mutex> lock;
+    const bool prof;
 
-    int begin(lnasr_ctx* c) {
-        ctx = c;
+    explicit Call(lnasr_ctx* c) : ctx(c), lock(c->tr_mutex), prof(c->prof_on) {}
+    ~Call() {
+        if (capturing) ctx->prof_on = prof;
+    }
+
+    int begin() {
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-        LN_HIP(hipStreamIsCapturing(ctx->stream, &st));
+        if (hipStreamIsCapturing(ctx->stream, &st) != hipSuccess) {
+            (void)hipGetLastError();
+            return fail(LNASR_E_INVALID, "the default stream takes no calls while another stream is captured");
+        }
         capturing = st != hipStreamCaptureStatusNone;
-        if (capturing) ctx->tr_captured = true;
+        if (capturing) {
+            ctx->tr_captured = true;
+            ctx->prof_on = false;                         // (its events would belong to the graph)
+        }
         return 0;
     }
     // 1: memory of the context's device, 0: host memory, negative: error
@@ -63,6 +65,7 @@ struct Call {
             (void)hipGetLastError();
             return 0;
         }
+        if (at.type == hipMemoryTypeHost) pinned = true;
         if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged) return 0;
         if (at.device != ctx->device)
             return fail(LNASR_E_INVALID, "%s lies on device %d, the context on device %d", what, at.device, ctx->device);
@@ -114,7 +117,8 @@ struct Call {
     }
     int finish() {
         for (int i = 0; i < nback; ++i) LN_HIP(hipMemcpyAsync(back[i].host, back[i].dev, back[i].bytes, hipMemcpyDeviceToHost, ctx->stream));
-        if (nback) LN_HIP(hipStreamSynchronize(ctx->stream));
+        // copies from pinned memory run later: the caller may change it once the call has returned
+        if (nback || pinned) LN_HIP(hipStreamSynchronize(ctx->stream));
         return 0;
     }
 };
@@ -178,7 +182,7 @@ using namespace lnasr;
 extern "C" {
 
 int lnasr_affine(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets, const int32_t* slots,
-                 int S, const void* w, const void* bias, int G, int dout, void* y, int64_t ldy) {
+                 int S, const void* w, const void* bias, int G, int dout, void* y, int64_t ldy) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
     LN_ENTER(ctx);
@@ -187,8 +191,8 @@ int lnasr_affine(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din
     LN_TRY(check_matrix("x", rows, din, ldx));
     LN_TRY(check_matrix("y", rows, dout, ldy));
     const size_t e = transform_size(dtype);
-    Call c;
-    LN_TRY(c.begin(ctx));
+    Call c(ctx);
+    LN_TRY(c.begin());
     Segments sg;
     bool covered;
     LN_TRY(segments(c, offsets, slots, S, G, rows, true, &sg, &covered));
@@ -209,11 +213,13 @@ int lnasr_affine(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din
     a.N = dout;
     LN_TRY(transform_rows(ctx, dtype, a, "affine"));
     return c.finish();
+} catch (const std::exception& e) {
+    return fail(LNASR_E_INVALID, "%s", e.what());
 }
 
 int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
                       const int32_t* slots, int S, const void* w, int G, int dout, const void* dy, int64_t lddy, void* dx, int64_t lddx,
-                      void* dw, void* dbias) {
+                      void* dw, void* dbias) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
     LN_ENTER(ctx);
@@ -224,8 +230,8 @@ int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, in
     LN_TRY(check_matrix("dx", rows, din, dx ? lddx : din));
     LN_REQUIRE(!dbias || dw, "the gradient of bias comes with that of w");
     const size_t e = transform_size(dtype);
-    Call c;
-    LN_TRY(c.begin(ctx));
+    Call c(ctx);
+    LN_TRY(c.begin());
     Segments sg;
     bool covered;
     LN_TRY(segments(c, offsets, slots, S, G, rows, true, &sg, &covered));
@@ -270,11 +276,13 @@ int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, in
         LN_TRY(transform_sum(ctx, dtype, a, "affine_dw"));
     }
     return c.finish();
+} catch (const std::exception& e) {
+    return fail(LNASR_E_INVALID, "%s", e.what());
 }
 
 int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
                      const int32_t* slots, int S, const void* w, const void* bias, int dout, const void* a, const void* b,
-                     const double* scale, int G, int rank, void* y, int64_t ldy) {
+                     const double* scale, int G, int rank, void* y, int64_t ldy) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
     LN_ENTER(ctx);
@@ -284,8 +292,8 @@ int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int
     LN_TRY(check_matrix("x", rows, din, ldx));
     LN_TRY(check_matrix("y", rows, dout, ldy));
     const size_t e = transform_size(dtype);
-    Call c;
-    LN_TRY(c.begin(ctx));
+    Call c(ctx);
+    LN_TRY(c.begin());
     Segments sg;
     bool covered;
     LN_TRY(segments(c, offsets, slots, S, G, rows, false, &sg, &covered));
@@ -325,11 +333,13 @@ int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int
     }
     LN_TRY(transform_rows(ctx, dtype, m, "projection"));
     return c.finish();
+} catch (const std::exception& e) {
+    return fail(LNASR_E_INVALID, "%s", e.what());
 }
 
 int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
                           const int32_t* slots, int S, const void* w, int dout, const void* a, const void* b, const double* scale, int G,
-                          int rank, const void* dy, int64_t lddy, void* dx, int64_t lddx, void* da, void* db, void* dw, void* dbias) {
+                          int rank, const void* dy, int64_t lddy, void* dx, int64_t lddx, void* da, void* db, void* dw, void* dbias) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
     LN_ENTER(ctx);
@@ -342,8 +352,8 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
     LN_TRY(check_matrix("dx", rows, din, dx ? lddx : din));
     LN_REQUIRE(!dbias || dw, "the gradient of bias comes with that of w");
     const size_t e = transform_size(dtype);
-    Call c;
-    LN_TRY(c.begin(ctx));
+    Call c(ctx);
+    LN_TRY(c.begin());
     Segments sg;
     bool covered;
     LN_TRY(segments(c, offsets, slots, S, G, rows, false, &sg, &covered));
@@ -454,6 +464,8 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
         LN_TRY(transform_sum(ctx, dtype, s, "projection_dw"));
     }
     return c.finish();
+} catch (const std::exception& e) {
+    return fail(LNASR_E_INVALID, "%s", e.what());
 }
 
 }  // extern "C"

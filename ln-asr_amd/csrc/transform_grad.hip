@@ -100,10 +100,10 @@ __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes
             for (int g = before + 1; g <= k; ++g) group_off[g] = at;
         }
         __syncthreads();
-        if (tid == kSortNT - 1) carry += sum;
+        if (tid == kSortNT - 1) carry = min(carry + sum, sg.rows);
         __syncthreads();
     }
-    const int64_t total = min(carry, sg.rows);
+    const int64_t total = carry;
     if (tid == 0) place[sg.S] = total;
     const int last = key(in[sg.S - 1]);
     for (int g = last + 1 + tid; g <= sg.G; g += kSortNT) group_off[g] = total;
@@ -140,7 +140,7 @@ int transform_sort(lnasr_ctx* ctx, int dtype, SumArgs* a) {
     int64_t* goff = place + sg.S + 1;
     int* ord0 = (int*)(goff + sg.G + 1);
     a->group_off = goff;
-    const bool mapped = !rows_together(sg, dtype);
+    const bool mapped = sg.rows > 0 && !rows_together(sg, dtype);
     if (mapped) a->rowmap = map;
     a->place = place;
     a->ord = ord0;

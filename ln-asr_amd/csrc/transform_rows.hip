@@ -666,7 +666,8 @@ static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 template <typename T, bool KN, int LOW>
 static int launch_deep(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t tiles_n = (a.N + 255) / 256, tiles_m = LOW == 0 ? a.sg.rows / 256 + a.sg.S : (a.sg.rows + 255) / 256;
-    LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
+    LN_REQUIRE(tiles_n * tiles_m < (1ll << 31) && tiles_m < (1ll << 28), "%lld rows x %d results are too many for one call",
+               (long long)a.sg.rows, a.N);
     int full = KN && a.N % 8 ? (a.K - 1) / 64 : a.K / 64;                             // as in launch_tile
     if (a.ldx * 512 >= (1ll << 31) || (KN ? a.N : a.K) * 512ll >= (1ll << 31)) full = 0;
     LN_LAUNCH(ctx, name, (rows_deep<T, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_m, (unsigned)tiles_n, full);

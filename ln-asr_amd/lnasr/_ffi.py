@@ -287,11 +287,13 @@ _KINDS = {}
 class _Arg:
     """An array handed to a feature transform: a numpy array (or what becomes one), a DeviceArray, or a tensor of another library
     on the GPU (an object with data_ptr(), shape, dtype, stride() and is_cuda, as torch's).  `obj` keeps it alive."""
-    __slots__ = ("ptr", "shape", "ld", "kind", "obj")
+    __slots__ = ("ptr", "shape", "ld", "kind", "obj", "loose")
 
     def __init__(self, ctx, x, name, ndim, like=None, out=False):
         """like: the _Arg whose type this one must have (None: any of the four; a kind: exactly that)."""
+        self.loose = False            # its memory is used in the order of another stream than the context's
         if isinstance(x, DeviceArray):
+            self.loose = x.ctx is not ctx
             if not x.ptr or x.ctx.device != ctx.device:
                 raise LnasrError("%s: a DeviceArray that was freed, or of another device" % name)
             self.obj, self.ptr, self.shape, self.kind = x, x.ptr, x.shape, x.dtype.name
@@ -304,6 +306,7 @@ class _Arg:
             if kind is None:
                 kind = _KINDS[dtype] = str(dtype).replace("torch.", "")
             self.obj, self.ptr, self.shape, self.kind, self.ld = x, x.data_ptr(), tuple(x.shape), kind, 1
+            self.loose = getattr(ctx, "_stream", None) is None
             if not ctx._tensors_checked:
                 # pointers of another copy of the HIP runtime mean nothing to this one
                 if self.ptr and lib().lnasr_debug_require_device_ptr(self.ptr) != 0:
@@ -324,8 +327,12 @@ class _Arg:
                     raise LnasrError("%s must be a writable C-contiguous numpy array, a DeviceArray or a tensor" % name)
             else:
                 x = np.asarray(x)
+                if x.dtype.kind not in "biuf":
+                    raise LnasrError("%s is an array of %s" % (name, x.dtype.name))
                 if isinstance(like, str):
-                    x = np.ascontiguousarray(x, dtype=like)
+                    given, x = x, np.ascontiguousarray(x, dtype=like)
+                    if given.dtype != x.dtype and x.dtype.kind == "i" and not np.array_equal(given, x):
+                        raise LnasrError("%s holds values that are not %s" % (name, like))
                 else:
                     kind = like.kind if like is not None and like.kind != "bfloat16" else x.dtype.name
                     x = np.ascontiguousarray(x, dtype=kind if kind in _CODES else np.float64)
@@ -920,6 +927,14 @@ class Context:
 
     # -- feature transforms ------------------------------------------------------------------------
     # (lnasr/transform.py has what the arguments mean)
+    def _call(self, fn, arrays, *args):
+        loose = any(a.loose for a in arrays if a)
+        if loose:                     # (a caller that wants no waits chooses the stream: use_stream)
+            self.device_sync()
+        check(fn(self.handle, *args))
+        if loose:
+            self.sync()
+
     def _rows(self, x, offsets, slots, groups):
         """(_Args of x, offsets, slots, number of segments, whether every row is known to belong to a segment)."""
         x = _Arg(self, x, "x", 2)
@@ -931,13 +946,15 @@ class Context:
         if slots is not None:
             sl = _Arg(self, slots, "slots", 1, like="int32")
             _need(sl, "slots", (S,))
-        elif S != groups:
-            raise ValueError("%d segments of %d groups: without slots there is one segment for each group" % (S, groups))
+        else:
+            G = groups.shape[0] if hasattr(groups, "shape") else len(groups)
+            if S != G:
+                raise ValueError("%d segments of %d groups: without slots there is one segment for each group" % (S, G))
         known = isinstance(off.obj, np.ndarray) and (sl is None or isinstance(sl.obj, np.ndarray))
         return x, off, sl, S, known and off.obj[0] == 0 and off.obj[-1] == x.shape[0]
 
     def affine(self, x, offsets, w, bias=None, slots=None, out=None):
-        x, off, sl, S, covered = self._rows(x, offsets, slots, w.shape[0])
+        x, off, sl, S, covered = self._rows(x, offsets, slots, w)
         w = _Arg(self, w, "w", 3, like=x)
         G, O, I = w.shape
         _need(x, "x", (x.shape[0], I))
@@ -949,12 +966,13 @@ class Context:
         y = out if out is not None else x.empty(self, (x.shape[0], O), not covered)
         ya = _Arg(self, y, "out", 2, like=x, out=True)
         _need(ya, "out", (x.shape[0], O))
-        check(lib().lnasr_affine(self.handle, _CODES[x.kind], x.ptr, x.shape[0], I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr,
-                                 bias and bias.ptr, G, O, ya.ptr, ya.ld))
+        self._call(lib().lnasr_affine, (x, off, sl, w, bias, ya), _CODES[x.kind], x.ptr, x.shape[0], I, x.ld, off.ptr, sl and sl.ptr, S,
+                   w.ptr, bias and bias.ptr, G, O, ya.ptr, ya.ld)
         return y
 
     def _grads(self, x, shapes, want, out, covered):
-        """The arrays that gradients go to: `out` (a dict: exactly those), or new ones for the names in `want`."""
+        """The arrays that gradients go to: `out` (a dict: exactly those), or new ones for the names in `want`; their _Args by name,
+        the pointer of a name (None: not wanted), and the row stride of "x"."""
         given = out is not None
         names = tuple(out) if given else tuple(want)
         for k in names:
@@ -966,19 +984,19 @@ class Context:
             _need(a, "out[%r]" % k, shapes[k])
             if k != "x" and len(a.shape) == 2 and a.ld != a.shape[1]:
                 raise LnasrError("out[%r] must be contiguous" % k)
-        return res, (lambda k: args[k].ptr if k in args else None), (args["x"].ld if "x" in args else 0)
+        return res, args, (lambda k: args[k].ptr if k in args else None), (args["x"].ld if "x" in args else 0)
 
     def affine_grad(self, x, offsets, w, dy, slots=None, want=("x", "w", "bias"), out=None):
-        x, off, sl, S, covered = self._rows(x, offsets, slots, w.shape[0])
+        x, off, sl, S, covered = self._rows(x, offsets, slots, w)
         w = _Arg(self, w, "w", 3, like=x)
         G, O, I = w.shape
         F = x.shape[0]
         _need(x, "x", (F, I))
         dy = _Arg(self, dy, "dy", 2, like=x)
         _need(dy, "dy", (F, O))
-        res, ptr, lddx = self._grads(x, {"x": (F, I), "w": (G, O, I), "bias": (G, O)}, want, out, covered)
-        check(lib().lnasr_affine_grad(self.handle, _CODES[x.kind], x.ptr, F, I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr, G, O,
-                                      dy.ptr, dy.ld, ptr("x"), lddx, ptr("w"), ptr("bias")))
+        res, args, ptr, lddx = self._grads(x, {"x": (F, I), "w": (G, O, I), "bias": (G, O)}, want, out, covered)
+        self._call(lib().lnasr_affine_grad, (x, off, sl, w, dy, *args.values()), _CODES[x.kind], x.ptr, F, I, x.ld, off.ptr,
+                   sl and sl.ptr, S, w.ptr, G, O, dy.ptr, dy.ld, ptr("x"), lddx, ptr("w"), ptr("bias"))
         return res
 
     def _adapters(self, x, w, a, b, scale):
@@ -997,7 +1015,7 @@ class Context:
         return w, a, b, scale, I, O, G, R
 
     def projection(self, x, offsets, w, a, b, bias=None, scale=None, slots=None, out=None):
-        x, off, sl, S, covered = self._rows(x, offsets, slots, a.shape[0])
+        x, off, sl, S, covered = self._rows(x, offsets, slots, a)
         w, a, b, scale, I, O, G, R = self._adapters(x, w, a, b, scale)
         if bias is not None:
             bias = _Arg(self, bias, "bias", 1, like=x)
@@ -1005,20 +1023,20 @@ class Context:
         y = out if out is not None else x.empty(self, (x.shape[0], O), not covered)
         ya = _Arg(self, y, "out", 2, like=x, out=True)
         _need(ya, "out", (x.shape[0], O))
-        check(lib().lnasr_projection(self.handle, _CODES[x.kind], x.ptr, x.shape[0], I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr,
-                                     bias and bias.ptr, O, a.ptr, b.ptr, scale and scale.ptr, G, R, ya.ptr, ya.ld))
+        self._call(lib().lnasr_projection, (x, off, sl, w, bias, a, b, scale, ya), _CODES[x.kind], x.ptr, x.shape[0], I, x.ld, off.ptr,
+                   sl and sl.ptr, S, w.ptr, bias and bias.ptr, O, a.ptr, b.ptr, scale and scale.ptr, G, R, ya.ptr, ya.ld)
         return y
 
     def projection_grad(self, x, offsets, w, a, b, dy, scale=None, slots=None, want=("x", "a", "b", "w", "bias"), out=None):
-        x, off, sl, S, covered = self._rows(x, offsets, slots, a.shape[0])
+        x, off, sl, S, covered = self._rows(x, offsets, slots, a)
         w, a, b, scale, I, O, G, R = self._adapters(x, w, a, b, scale)
         F = x.shape[0]
         dy = _Arg(self, dy, "dy", 2, like=x)
         _need(dy, "dy", (F, O))
-        res, ptr, lddx = self._grads(x, {"x": (F, I), "a": (G, R, I), "b": (G, O, R), "w": (O, I), "bias": (O,)}, want, out, covered)
-        check(lib().lnasr_projection_grad(self.handle, _CODES[x.kind], x.ptr, F, I, x.ld, off.ptr, sl and sl.ptr, S, w.ptr, O, a.ptr,
-                                          b.ptr, scale and scale.ptr, G, R, dy.ptr, dy.ld, ptr("x"), lddx, ptr("a"), ptr("b"),
-                                          ptr("w"), ptr("bias")))
+        res, args, ptr, lddx = self._grads(x, {"x": (F, I), "a": (G, R, I), "b": (G, O, R), "w": (O, I), "bias": (O,)}, want, out, covered)
+        self._call(lib().lnasr_projection_grad, (x, off, sl, w, a, b, scale, dy, *args.values()), _CODES[x.kind], x.ptr, F, I, x.ld,
+                   off.ptr, sl and sl.ptr, S, w.ptr, O, a.ptr, b.ptr, scale and scale.ptr, G, R, dy.ptr, dy.ld, ptr("x"), lddx,
+                   ptr("a"), ptr("b"), ptr("w"), ptr("bias"))
         return res
 
     # -- multi-GPU ---------------------------------------------------------------------------------

@@ -9,8 +9,10 @@ offsets[0] .. offsets[-1] are left as they were in `out`, and are zeros in an ar
 Arrays are numpy arrays, `DeviceArray`s, or GPU tensors of another library (torch's, which is not imported here: a tensor only
 has to have data_ptr(), shape, dtype, stride()); what comes back is of the same kind as x.  x, matrices and results share one
 type: float64, float32, float16 or (tensors) bfloat16.  Sums are held in 64 bits for float64 and in 32 for the others.  Rows may
-be strided (a slice of columns); matrices are contiguous.  Results may be written into `out`, which must not overlap an input.
-With GPU tensors, choose their stream first (`ctx.use_stream`).
+be strided (a slice of columns); matrices are contiguous.  numpy arrays are converted to the type of x.  Results may be written
+into `out`, which must not overlap an input (nor lie beside it in the columns of one buffer).  With GPU tensors, choose their
+stream first (`ctx.use_stream`) and import their library before lnasr; where no stream was chosen, and for `DeviceArray`s of
+another context, a call waits for the device before it begins and until it is done.
 """
 import numpy as np
 

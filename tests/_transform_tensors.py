@@ -269,7 +269,83 @@ def far_rows():
     assert not bool(g["w"][:2].any())
 
 
-CHECKS = {f.__name__: f for f in (bfloat16, bfloat16_wide, strides, streams, graphs, far_rows)}
+def unchosen_streams():
+    """No stream was chosen: a call waits for what its tensors come from, and is done when it returns."""
+    c = _ffi.Context(0)
+    t, h = up(ref.make(30, (4000, 64, 48, 5, 5, 8), slots=False), "float32")
+    want, bound = ref.affine("float32", h["x"], h["offsets"], h["w3"], h["bias2"], None, h["y0"])
+    slow = torch.randn(4096, 4096, device="cuda")
+    for s in (torch.cuda.Stream(), torch.cuda.default_stream()):
+        late = torch.zeros_like(t["x"])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                slow = slow @ slow * 1e-3
+            late.copy_(t["x"])
+        y = transform.affine(late, t["offsets"], t["w3"], t["bias2"], ctx=c)
+        z = y + 0
+        torch.cuda.synchronize()
+        ref.check(host(z), want, bound)
+    c.close()
+
+
+def pinned():
+    """Pinned host arrays may change as soon as the call is back."""
+    s = torch.cuda.Stream()
+    c = _ffi.Context(0)
+    c.use_stream(s)
+    t, h = up(ref.make(31, (300, 512, 512, 40, 40, 8), slots=False), "float32")
+    want, bound = ref.affine("float32", h["x"], h["offsets"], h["w3"], None, None, h["y0"])
+    w = torch.empty(t["w3"].shape, pin_memory=True)
+    w.copy_(t["w3"])
+    off = torch.empty(t["offsets"].shape, dtype=torch.int64, pin_memory=True)
+    off.copy_(t["offsets"])
+    slow = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            slow = slow @ slow * 1e-3
+        y = transform.affine(t["x"], off.numpy(), w.numpy(), ctx=c)
+    w.fill_(float("nan"))
+    off.fill_(0)
+    torch.cuda.synchronize()
+    ref.check(host(y), want, bound)
+    c.use_stream(None)
+    c.close()
+
+
+def graph_outlives_context():
+    """Captured while the context profiles; replayed after it was closed, on workspaces that stay."""
+    s = torch.cuda.Stream()
+    c = _ffi.Context(0)
+    c.use_stream(s)
+    t, h = up(ref.make(32, (500, 72, 80, 4, 3, 16)), "float32")
+    y = torch.zeros_like(t["y0"])
+    run = lambda: transform.projection(t["x"], t["offsets"], t["w"], t["a"], t["b"], t["bias"], t["scale"], t["slots"], out=y, ctx=c)
+    with torch.cuda.stream(s):
+        run()
+        torch.cuda.synchronize()
+        c.prof_enable(True)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            run()
+        run()
+        torch.cuda.synchronize()
+        assert [v[0] for k, v in c.prof_report().items() if k.startswith("projection")] == [1, 1]      # the eager call's
+        c.prof_enable(False)
+        c.use_stream(None)
+        c.close()
+        other = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(4)]
+        want, bound = ref.projection("float32", h["x"], h["offsets"], h["w"], h["a"], h["b"], h["bias"], h["scale"], h["slots"], h["y0"])
+        for _ in range(3):
+            y.fill_(5.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            ref.check(host(y), want, bound)
+        del other
+
+
+CHECKS = {f.__name__: f for f in (bfloat16, bfloat16_wide, strides, streams, graphs, far_rows, unchosen_streams, pinned, graph_outlives_context)}
 
 if __name__ == "__main__":
     for name in sys.argv[1:]:

@@ -380,3 +380,90 @@ def test_refusals(ctx):
         ctx.affine(ctx.to_device(np.zeros((6, 4), np.int32)), off, w)
     # the context works after all of that
     assert not ctx.affine(x, off, w).any()
+
+
+def test_rows_of_empty_segments_with_slots(ctx):
+    """No rows at all, but segments with groups: nothing to look up, every sum is zero."""
+    w, a, b = np.ones((3, 4, 5)), np.ones((3, 2, 5)), np.ones((3, 4, 2))
+    x, dy, off, sl = np.zeros((0, 5)), np.zeros((0, 4)), np.zeros(3, dtype=np.int64), np.array([2, 2], dtype=np.int32)
+    assert ctx.affine(x, off, w, slots=sl).shape == ctx.projection(x, off, w[0], a, b, slots=sl).shape == (0, 4)
+    for g in (ctx.affine_grad(x, off, w, dy, slots=sl), ctx.projection_grad(x, off, w[0], a, b, dy, slots=sl)):
+        assert all(not v.any() for v in g.values())
+
+
+def test_threads_share_a_context(ctx):
+    """Two threads, one context: each call's launches share its workspaces and stay together."""
+    import threading
+    sizes = [(900, 72, 80, 4, 3, 16), (700, 80, 72, 5, 2, 40)]
+    data = [ref.make(60 + i, size) for i, size in enumerate(sizes)]
+
+    def run(d):
+        y = ctx.projection(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["bias"], d["scale"], d["slots"])
+        g = ctx.projection_grad(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"])
+        return [y] + [g[k] for k in sorted(g)]
+
+    alone = [run(d) for d in data]
+    wrong, failed = [], []
+
+    def work(i):
+        try:
+            for _ in range(20):
+                if not all(np.array_equal(u, v) for u, v in zip(run(data[i]), alone[i])):
+                    wrong.append(i)
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and not failed, (wrong, failed)
+
+
+def test_arrays_of_another_context(ctx):
+    """DeviceArrays of another context of the device: its work comes first, and it may read the result at once."""
+    from lnasr import _ffi
+    other = _ffi.Context(0)
+    d = ref.make(62, (20000, 64, 48, 3, 3, 8), slots=False)
+    x, w, y = other.to_device(d["x"]), other.to_device(d["w3"]), other.to_device(d["y0"])
+    assert ctx.affine(x, d["offsets"], w, out=y) is y
+    got = y.to_host()
+    del x, w, y
+    other.close()
+    ref.check(got, *ref.affine("float64", d["x"], d["offsets"], d["w3"], None, None, d["y0"]))
+
+
+def test_values_that_do_not_fit_are_refused(ctx):
+    from lnasr import _ffi
+    x, w, off = np.ones((6, 4)), [[[1.0] * 4] * 3] * 2, [0, 2, 6]
+    assert (ctx.affine(x, off, w) == 4.0).all()                                     # lists become arrays
+    for match, call in (("slots holds values", lambda: ctx.affine(x, off, w, slots=np.array([0, (1 << 32) + 1]))),
+                        ("offsets holds values", lambda: ctx.affine(x, np.array([0, 1.5, 6]), w)),
+                        ("offsets holds values", lambda: ctx.affine(x, np.array([0, 2, 1 << 63], dtype=np.uint64), w)),
+                        ("array of complex", lambda: ctx.affine(x + 1j, off, w)),
+                        ("array of str", lambda: ctx.affine(np.full((6, 4), "a"), off, w))):
+        with pytest.raises(_ffi.LnasrError, match=match):
+            call()
+
+
+@pytest.mark.parametrize("size", [(9001, 840, 520, 6, 3, 24), (2000, 130, 200, 6, 3, 16), (90, 130, 200, 6, 3, 16)], ids=str)
+def test_device_offsets_out_of_order_in_the_wide_forms(ctx, size):
+    """The same at sizes that the tiles through LDS take: every offset is brought into range, whatever their order."""
+    d = ref.make(63, size)
+    F, S = size[0], size[3]
+    bad = np.array([-50, 1 << 40, F // 3, F - 5, -(1 << 60), 1 << 62, F], dtype=np.int64)
+    sl = np.array([0, 99, 1, 1 << 30, 2, 1], dtype=np.int32)
+    up = lambda v, kind: ctx.to_device(np.ascontiguousarray(v, dtype=kind))
+    for kind in ("float16", "float32"):
+        x, dy, w3, w, a, b = (up(d[k], kind) for k in ("x", "dy", "w3", "w", "a", "b"))
+        for off in (bad, bad[::-1].copy(), np.full(S + 1, F), np.array([7] * S + [F])):
+            off, slots = ctx.to_device(off.astype(np.int64)), ctx.to_device(sl)
+            y, p = ctx.affine(x, off, w3, slots=slots), ctx.projection(x, off, w, a, b, slots=slots)
+            g, h = ctx.affine_grad(x, off, w3, dy, slots), ctx.projection_grad(x, off, w, a, b, dy, slots=slots)
+            ctx.sync()
+            assert y.shape == p.shape == (F, size[2]) and len(g) == 3 and len(h) == 5
+    # the last of them, seven rows that belong to nobody, is in order
+    want = d["y0"].astype("float32")
+    got = ctx.affine(x, off, w3, slots=slots, out=up(want, "float32")).to_host()
+    assert np.array_equal(got[:7], want[:7])

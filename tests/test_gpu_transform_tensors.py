@@ -9,7 +9,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-CHECKS = ["bfloat16", "bfloat16_wide", "strides", "streams", "graphs", "far_rows"]
+CHECKS = ["bfloat16", "bfloat16_wide", "strides", "streams", "graphs", "far_rows", "unchosen_streams", "pinned", "graph_outlives_context"]
 
 
 @pytest.fixture(scope="module")
