@@ -242,11 +242,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         for (int m = 0; m < MR; ++m) acc[n][m] = Acc{0, 0, 0, 0};
 
     // acc += X W' over the 128 bytes of k in a buffer; with SOME only for the rows from .. to - 1 of the wave's
-    auto multiply = [&](const char* xs, auto some, int from, int to) {
+    auto multiply = [&](const char* xs, auto some, int from, int to, int left = 1 << 20) {
         constexpr bool SOME = decltype(some)::value;
         const char* ws = xs + XB;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            if (SOME && h && left <= KB / 2) break;                                   // (an adapter of a low rank)
             u32x4 xf[MR], wf[NR];
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
@@ -301,14 +302,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             }
         }
     };
-    auto apply = [&](const Pieces& p, auto some, int from, int to) {
+    auto apply = [&](const Pieces& p, auto some, int from, int to, int left = 1 << 20) {
 #pragma unroll
         for (int i = 0; i < XI; ++i) *(u32x4*)(l0 + (tid + NT * i) * 16) = p.x[i];
 #pragma unroll
         for (int i = 0; i < WI; ++i)
             if (brings_w(i)) *(u32x4*)(l0 + XB + (tid + NT * i) * 16) = p.w[i];
         __syncthreads();
-        multiply(l0, some, from, to);
+        multiply(l0, some, from, to, left);
         __syncthreads();
     };
 
@@ -400,7 +401,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             const int from = lo > r0 ? (int)(lo - r0) - wm : 0, to = hi < r1 ? (int)(hi - r0) - wm : TM;
             for (int k0 = 0; k0 < a.R; k0 += KB) {
                 if (!waits || k0 > 0) fetch(first, p, a.ldp, (const T*)a.low + k * a.low_stride, KN ? a.N : a.R, k0, a.R);
-                apply(first, std::true_type{}, from, to);
+                apply(first, std::true_type{}, from, to, a.R - k0);
             }
         }
     }
@@ -418,6 +419,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 // cores, the LDS and the memory each work ahead of one another, with one barrier a step and a wait that counts (the newest four
 // requests, x of the step after next, may be out).
 // ------------------------------------------------------------------------------------------
+// Up to 64 segments, a lane each: the tiles of 256 rows numbered without gaps (find_span leaves some), so that the dies get equally
+// many: 16,384 x 1024 x 1024 of one group 55 -> 36 us.  (All whole tiles before the segments' last ones, for a shorter last turn of
+// the CUs, gained nothing: those then fetch their matrices again.)  False: no tile for this block.
+__device__ __forceinline__ bool exact_tile(const Segments& sg, unsigned id, unsigned tiles_n, unsigned* tn, int* slot, int64_t* r0, int64_t* r1) {
+    const int lane = threadIdx.x & 63, s = min(lane, sg.S - 1);
+    const int64_t lo = seg_off(sg, s), n = max((int64_t)0, seg_off(sg, s + 1) - lo);
+    const int k = lane < sg.S ? seg_slot(sg, s) : -1, mine = k < 0 ? 0 : (int)((n + 255) >> 8);
+    int sum = mine;                                                                   // running sum over the segments
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(sum, d);
+        sum += lane >= d ? v : 0;
+    }
+    const unsigned tiles = (unsigned)__builtin_amdgcn_readlane(sum, 63);
+    if (id >= tiles * tiles_n) return false;
+    unsigned tm;
+    tile_order(die_order(id, tiles * tiles_n), tiles, tiles_n, &tm, tn);
+    const int from = __builtin_ctzll(__ballot(sum > (int)tm));
+    *slot = __builtin_amdgcn_readlane(k, from);
+    *r0 = seg_off(sg, from) + (int64_t)(tm - (unsigned)__builtin_amdgcn_readlane(sum - mine, from)) * 256;
+    *r1 = min(*r0 + 256, max(*r0, seg_off(sg, from + 1)));
+    return true;
+}
+
 template <typename T, bool KN, int LOW>
 __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m, unsigned tiles_n, int full) {
     using M = Mat<T>;
@@ -429,16 +454,20 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / 4 * 128, wn = wave % 4 * 64;
     unsigned tm, tn;
-    tile_order(die_order(blockIdx.x, gridDim.x), tiles_m, tiles_n, &tm, &tn);
-    const int n0 = (int)tn * TN;
     int64_t r0, r1;
     int slot = 0;
-    if (LOW == 0) {
+    if (LOW == 0 && a.sg.S <= 64) {
+        if (!exact_tile(a.sg, blockIdx.x, tiles_n, &tn, &slot, &r0, &r1)) return;
+    } else {
+        tile_order(die_order(blockIdx.x, gridDim.x), tiles_m, tiles_n, &tm, &tn);
+    }
+    const int n0 = (int)tn * TN;
+    if (LOW == 0 && a.sg.S > 64) {
         const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, tm, 8, &r0, &r1);
         if (s < 0) return;
         slot = seg_slot(a.sg, s);
         if (slot < 0) return;
-    } else {
+    } else if (LOW) {
         r0 = seg_off(a.sg, 0) + (int64_t)tm * TM;
         r1 = seg_off(a.sg, a.sg.S);
         if (r1 > r0 + TM) r1 = r0 + TM;
@@ -666,7 +695,7 @@ static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 template <typename T, bool KN, int LOW>
 static int launch_deep(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t tiles_n = (a.N + 255) / 256, tiles_m = LOW == 0 ? a.sg.rows / 256 + a.sg.S : (a.sg.rows + 255) / 256;
-    LN_REQUIRE(tiles_n * tiles_m < (1ll << 31) && tiles_m < (1ll << 28), "%lld rows x %d results are too many for one call",
+    LN_REQUIRE(tiles_n * tiles_m < (1ll << 31) && tiles_m < (1ll << 24), "%lld rows x %d results are too many for one call",
                (long long)a.sg.rows, a.N);
     int full = KN && a.N % 8 ? (a.K - 1) / 64 : a.K / 64;                             // as in launch_tile
     if (a.ldx * 512 >= (1ll << 31) || (KN ? a.N : a.K) * 512ll >= (1ll << 31)) full = 0;
@@ -690,7 +719,7 @@ static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         if (a.N <= 32) return launch_tile<T, 64, 32, 4, 1, KN, LOW>(ctx, a, name);
         if (a.N <= 48) return launch_tile<T, 64, 48, 4, 1, KN, LOW>(ctx, a, name);
         // 16 bits: the larger the tile the less it asks of the memory for its products (us, 64 x 64 / 128 x 128 / 256 x 256: 65,536 x
-        // 2048 x 2048 1185 / 800 / 599; 16,384 x 1024 x 1024 65 / 57 / 46), as long as there is one for every CU.  32 and 64 bits
+        // 2048 x 2048 1185 / 634 / 496; 16,384 x 1024 x 1024 65 / 47 / 36), as long as there is one for every CU.  32 and 64 bits
         // have time for that: 64 x 64 leaves the least over at the ends (f32 120,011 x 351 x 128 105 against 142 us, f64 16,384 x
         // 1024 x 1024 609 against 640; f32 65,536 x 1024 x 1024 1169 against 1165).
         if constexpr (sizeof(T) == 2) {
