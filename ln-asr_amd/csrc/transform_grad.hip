@@ -552,17 +552,21 @@ __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typen
     const int64_t go = clamped(g), ge = clamped(g + 1), n = (ge - go + (1ll << ts) - 1) >> ts;
     if (n <= 1) return;
     const int64_t t = (go >> ts) + g, size = (int64_t)a.I * a.J;
-    for (int64_t e = (int64_t)(blockIdx.x % per) * 256 + threadIdx.x; e < size + a.I; e += (int64_t)per * 256) {
-        if (e < size) {
-            Sum v = 0;
-#pragma unroll 8
-            for (int64_t k = 0; k < n; ++k) v += parts[(t + k) * size + e];
-            ((T*)a.out)[g * size + e] = (T)v;
-        } else if (a.cols) {
-            Sum v = 0;
-            for (int64_t k = 0; k < n; ++k) v += col_parts[(t + k) * a.I + e - size];
-            ((T*)a.cols)[g * a.I + e - size] = (T)v;
+    // n values `step` apart, in their order, eight on their way at a time
+    auto total = [&](const Sum* from, int64_t step) {
+        Sum v = 0;
+        for (int64_t k = 0; k < n; k += 8) {
+            Sum u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = from[min(k + i, n - 1) * step];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += k + i < n ? u[i] : (Sum)0;
         }
+        return (T)v;
+    };
+    for (int64_t e = (int64_t)(blockIdx.x % per) * 256 + threadIdx.x; e < size + a.I; e += (int64_t)per * 256) {
+        if (e < size) ((T*)a.out)[g * size + e] = total(parts + t * size + e, size);
+        else if (a.cols) ((T*)a.cols)[g * a.I + e - size] = total(col_parts + t * a.I + e - size, a.I);
     }
 }
 

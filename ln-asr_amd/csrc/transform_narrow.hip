@@ -19,6 +19,21 @@ struct Chunk {
 #pragma unroll
         for (int i = 0; i < HF; ++i) v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, at + 1024 * i, 0, 0));
     }
+    // the same for values first, first + 1, .. of src up to value c of the chunk, second + c, .. up to value `live`, then zeros
+    __device__ __forceinline__ void load_two(const T* src, int64_t first, int64_t second, int c, int live) {
+        constexpr int E = Mat<T>::E;
+#pragma unroll
+        for (int i = 0; i < HF; ++i) {
+            T e[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const int at = ((threadIdx.x & 63) + 64 * i) * E + j;
+                e[j] = src[at < c ? first + at : at < live ? second + at : first];
+                if (at >= live) e[j] = (T)0;
+            }
+            __builtin_memcpy(&v[i], e, 16);
+        }
+    }
     // the same where the array ends after `room` bytes
     __device__ __forceinline__ void load_end(const char* src, int64_t room) {
 #pragma unroll
@@ -251,26 +266,41 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
         while (i + 1 < a.sg.S && a.place[i + 1] <= q) ++i;
         return seg_off(a.sg, a.ord[i]) + min(q, a.place[i + 1]) - a.place[i];
     };
-    // first of the R rows from place k of the span on, -1 if they do not lie together (the same for every lane)
-    auto run_at = [&](int k) -> int64_t {
-        if (k + R > n) return -1;
-        if (!a.place) return q0 + k;
-        while (seg + 1 < a.sg.S && a.place[seg + 1] <= q0 + k) ++seg;
-        return q0 + k + R <= a.place[seg + 1] ? seg_off(a.sg, a.ord[seg]) + q0 + k - a.place[seg] : (int64_t)-1;
-    };
-    auto fetch = [&](int64_t row) {                        // (R rows of the array: nothing past its end)
-        an.load((const char*)a.a + row * I * SZ, a_bytes);
-        bn.load((const char*)a.b + row * J * SZ, b_bytes);
+    // The R rows from place k of the span on, as many as there are (the same for every lane): true if they come from one or two
+    // segments, and then asks for them
+    auto fetch = [&](int k) {
+        const int live = min(R, n - k);
+        int64_t first = q0 + k, second = 0;
+        int c = live;                                      // rows of the first segment
+        if (a.place) {
+            while (seg + 1 < a.sg.S && a.place[seg + 1] <= q0 + k) ++seg;
+            first += seg_off(a.sg, a.ord[seg]) - a.place[seg];
+            const int64_t left = a.place[seg + 1] - (q0 + k);
+            if (left < live) {
+                c = (int)left;
+                int i = seg + 1;
+                while (i + 1 < a.sg.S && a.place[i + 1] <= q0 + k + c) ++i;
+                if (i >= a.sg.S || a.place[i + 1] < q0 + k + live) return false;
+                second = seg_off(a.sg, a.ord[i]) - c;
+            }
+        }
+        if (c == R) {                                      // (R rows of the array: nothing past its end)
+            an.load((const char*)a.a + first * I * SZ, a_bytes);
+            bn.load((const char*)a.b + first * J * SZ, b_bytes);
+        } else {
+            an.load_two((const T*)a.a, first * I, second * I, c * I, live * I);
+            bn.load_two((const T*)a.b, first * J, second * J, c * J, live * J);
+        }
+        return true;
     };
     int k0 = wave * R;
-    int64_t row = k0 < n ? run_at(k0) : -1;
+    bool came = k0 < n && fetch(k0);
     int here = seg;
-    if (row >= 0) fetch(row);
     for (; k0 < n; k0 += 4 * R) {
-        if (row >= 0) {
+        if (came) {
             an.store(as, a_bytes);
             bn.store(bs, b_bytes);
-        } else {                                           // the span's last rows, or rows that lie apart: one value at a time
+        } else {                                           // rows of three segments and more: one value at a time
             for (int e = lane; e < R * I; e += 64) {
                 const int k = e / I;
                 const int64_t at = k0 + k < n ? row_at(q0 + k0 + k, here) : -1;
@@ -285,9 +315,8 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
         wave_lds_order();
         const int k1 = k0 + 4 * R;
         if (k1 < n) {
-            row = run_at(k1);
+            came = fetch(k1);
             here = seg;
-            if (row >= 0) fetch(row);
         }
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -354,7 +383,7 @@ static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name)
     constexpr int HA = R * 16 * IF * SZ / 1024, HB = R * 16 * JF * SZ / 1024;
     const int64_t size = (int64_t)a.I * a.J + a.I;
     int ts = 8;
-    while (ts < 40 && ((a.sg.rows >> ts) > 4 * ctx->prop.multiProcessorCount || (a.sg.rows >> ts) * size * (int64_t)sizeof(Sum) > (256ll << 20))) ++ts;
+    while (ts < 40 && ((a.sg.rows >> ts) > 2 * ctx->prop.multiProcessorCount || (a.sg.rows >> ts) * size * (int64_t)sizeof(Sum) > (256ll << 20))) ++ts;
     const int64_t spans = (a.sg.rows >> ts) + a.groups;
     LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d groups are too many for one call", (long long)a.sg.rows, a.groups);
     void* parts = nullptr;
