@@ -146,6 +146,7 @@ __device__ __forceinline__ u32x4 load_piece(const T* line, long c, long end) {
         __builtin_memcpy(&v, line + c, 16);
         return v;
     }
+    if (sizeof(T) == 2 && c >= end) return u32x4{0, 0, 0, 0};                     // (adapters of rank 32: 80 -> 75 us; 4 elements are as soon looked at)
     T e[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) e[j] = c + j < end ? line[c + j] : (T)0;
