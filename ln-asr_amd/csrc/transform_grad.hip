@@ -8,7 +8,8 @@ namespace lnasr {
 // ------------------------------------------------------------------------------------------
 // Segments sorted by group, one block: a stable radix sort (eight bits of the group a pass; equal digits of a wave are found
 // by ballots), then the running sum of their lengths.  Segments without a group go last and are left out.  Order matters: the
-// rows of a group are summed in the order of the batch, so a gradient is the same bits every time.
+// rows of a group are summed in the order of the batch, so a gradient is the same bits every time.  8 us for 300 segments, an empty
+// launch timed the same way 6; with everything in LDS it was no faster.
 // ------------------------------------------------------------------------------------------
 constexpr int kSortNT = 1024;
 __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes, int* ord0, int* ord1, int64_t* place,
@@ -177,6 +178,8 @@ __device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int
 // LDS-DMA step by step, the last and uneven one through registers; otherwise -- segments of a few rows -- all of them through
 // registers, row by row as rowmap says, loaded a step ahead.  A group with one span is written at once, the others leave sums of 32
 // bits or more per span, which join_parts adds in the order of the spans.
+// f32 20,011 rows x 512 x 429: 98 us, 90 TFLOP/s of the 153 of a large library product (CUs busy 72 % of the time: 1120 blocks on
+// 1280 places).  bf16 16,384 rows x 16 x 1024: 14 us (an empty launch 6), 34 MB.
 // ------------------------------------------------------------------------------------------
 template <typename T, int TI, int TJ, int WI, int WJ, bool TOGETHER>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned tiles_i, unsigned tiles_j, int ts, typename Mat<T>::Sum* parts,
@@ -348,6 +351,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
 // 4 kk .. 4 kk + 3 and 16 more.  Lines of 512 bytes, two to a kilobyte that a wave brings, each kilobyte 64 bytes further on and the
 // odd line's runs of 16 columns swapped in pairs: the eight lines that one read touches lie in other banks, and the reads need two
 // addresses instead of eight (registers).
+// bf16 32,768 rows x 2048 x 1024 in 16 ragged groups: 173 us, 790 TFLOP/s; most of the rest is the longest groups' blocks, one to two
+// turns of the CUs (cutting them finer costs as much in sums written and read).
 // ------------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, unsigned tiles_j, int ts, float* parts) {
@@ -505,7 +510,8 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
 }
 
 // Column sums of a beside sum_deep: cols[k, i] = sum of a[r, i], a span and 512 columns a block, eight of them a thread; the rows of the
-// span go to the four waves in turn, which meet in LDS.
+// span go to the four waves in turn, which meet in LDS.  bf16 32,768 x 2048: 28 us, 4.8 TB/s.  (Summed beside the products instead, by
+// matrix instructions or from LDS, it has no registers left.)
 template <typename T>
 __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int ts, float* col_parts) {
     __shared__ float part[3][64][8];
@@ -540,6 +546,7 @@ __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int t
     }
 }
 
+// out and cols of the groups that have more than one span.  fp64 64 groups of 39 x 39 in 350 spans: 7 us, an empty launch 6.
 template <typename T>
 __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typename Mat<T>::Sum* parts, const typename Mat<T>::Sum* col_parts,
                                                   unsigned per) {
