@@ -467,3 +467,47 @@ def test_device_offsets_out_of_order_in_the_wide_forms(ctx, size):
     want = d["y0"].astype("float32")
     got = ctx.affine(x, off, w3, slots=slots, out=up(want, "float32")).to_host()
     assert np.array_equal(got[:7], want[:7])
+
+
+def everything(ctx, kind, d):
+    y = ctx.projection(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["bias"], d["scale"], d["slots"])
+    ref.check(y, *ref.projection(kind, d["x"], d["offsets"], d["w"], d["a"], d["b"], d["bias"], d["scale"], d["slots"], d["y0"]), "projection")
+    got = ctx.projection_grad(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"])
+    want, err = ref.projection_grad(kind, d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"], d["dx0"])
+    for k in want:
+        ref.check(got[k], want[k], err[k], "projection_grad " + k)
+    if d["slots"] is not None:
+        d["slots"] = np.maximum(d["slots"], 0)
+    y = ctx.affine(d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"])
+    ref.check(y, *ref.affine(kind, d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], d["y0"]), "affine")
+    got = ctx.affine_grad(d["x"], d["offsets"], d["w3"], d["dy"], d["slots"])
+    want, err = ref.affine_grad(kind, d["x"], d["offsets"], d["w3"], d["dy"], d["slots"], d["dx0"])
+    for k in want:
+        ref.check(got[k], want[k], err[k], "affine_grad " + k)
+
+
+@pytest.mark.parametrize("size,slots", [((20000, 1024, 1030, 90, 4, 9), True), ((20000, 1032, 1024, 70, 70, 8), False),
+                                        ((16384, 72, 1030, 1, 1, 3), False), ((16640, 1024, 1024, 2, 1, 16), True)], ids=str)
+def test_wide_tiles_of_many_segments_and_of_one(ctx, size, slots):
+    """The largest tiles where the segments are more than a wave's lanes, and where there are one or two."""
+    everything(ctx, "float16", typed(ref.make(70, size, slots=slots), "float16"))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [(3, 1, 70001, 2, 2, 3), (3, 70001, 1, 2, 2, 3), (40, 24, 40, 5, 3, 300), (200, 351, 128, 6, 4, 12),
+                                  (3000, 3, 700, 4, 3, 2), (3000, 700, 3, 4, 3, 2), (2500, 30, 30, 160, 9, 2), (2500, 30, 30, 900, 40, 2)], ids=str)
+def test_extreme_widths_ranks_and_segments(ctx, kind, size):
+    """One value in or out, ranks past both widths, narrow rows whose segments are as short as the pieces they are summed in."""
+    everything(ctx, kind, typed(ref.make(71, size, negative=True), kind))
+
+
+def test_inputs_and_outputs_of_different_places(ctx):
+    """numpy in and DeviceArrays out, and the other way round."""
+    d = ref.make(72, (300, 39, 40, 7, 3, 8))
+    want, bound = ref.affine("float64", d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], d["y0"])
+    out = ctx.to_device(d["y0"])
+    assert ctx.affine(d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], out=out) is out
+    ref.check(out.to_host(), want, bound)
+    out = d["y0"].copy()
+    assert ctx.affine(ctx.to_device(d["x"]), ctx.to_device(d["offsets"]), d["w3"], ctx.to_device(d["bias2"]), d["slots"], out=out) is out
+    ref.check(out, want, bound)
