@@ -511,3 +511,9 @@ def test_inputs_and_outputs_of_different_places(ctx):
     out = d["y0"].copy()
     assert ctx.affine(ctx.to_device(d["x"]), ctx.to_device(d["offsets"]), d["w3"], ctx.to_device(d["bias2"]), d["slots"], out=out) is out
     ref.check(out, want, bound)
+
+
+@pytest.mark.parametrize("size,slots", [((16384, 128, 1024, 1, 1, 3), False), ((30000, 1024, 1030, 12, 5, 8), True)], ids=str)
+def test_wide_tiles_of_few_segments_in_full_turns(ctx, size, slots):
+    """The largest tiles where they fill the chip in whole turns (the sizes above leave a turn half empty)."""
+    everything(ctx, "float16", typed(ref.make(73, size, slots=slots), "float16"))
