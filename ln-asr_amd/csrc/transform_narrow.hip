@@ -75,7 +75,8 @@ __device__ __forceinline__ void put_chunk(char* to, const char* lds, int bytes) 
 // y[r] = scale (W x[r]) + bias: the four waves of a block share a span of rows, each takes 16 at a time.  The next 16 rows are on
 // their way while the current ones multiply, and the stores of the last ones are not waited for.  N <= 16 NF, K sizeof(T) <= 64
 // HF; with a bias K + 1 values fit: the bias is a column of W that meets a one behind each row (and takes no scale: no call has both).
-// fp64 1,024,000 x 39 x 39: 145-155 us, 4.2-4.4 TB/s of the 5.2 of a large copy; 64 single rows: 8 us, an empty launch 6.
+// fp64 1,024,000 x 39 x 39: 145-155 us, 4.2-4.4 TB/s of the 5.2 of a large copy; 64 single rows: 6.4 us, three
+// latencies of memory.
 // ------------------------------------------------------------------------------------------
 template <typename T, int NF, int HF>
 __global__ __launch_bounds__(256, NF * HF <= 15 ? 3 : 1) void rows_narrow(RowsArgs a, int ts, int wave_lds) {

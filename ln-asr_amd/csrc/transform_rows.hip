@@ -120,8 +120,8 @@ __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_
 // ------------------------------------------------------------------------------------------
 // A few rows: 16 MR rows x 16 results a block, its eight waves divide k between them.  Bound by the latency of memory and, with many
 // groups, by the matrices read once: fragments go from memory to registers, many at a time, and meet in LDS at the end.
-// bf16 64 single rows x 2048 -> 2048, 48 adapters of rank 16: 8 us for the middle and 15 for the rest (an empty launch timed the same
-// way: 6), 15 MB; through the tiles below 120.
+// bf16 64 single rows x 2048 -> 2048, 48 adapters of rank 16: 5.5 us for the middle and 12 for the rest, 15 MB; through the
+// tiles below 120.
 // ------------------------------------------------------------------------------------------
 template <typename T, bool KN, int MR, int LOW>
 __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, int ts) {
