@@ -146,7 +146,8 @@ __device__ __forceinline__ u32x4 load_piece(const T* line, long c, long end) {
         __builtin_memcpy(&v, line + c, 16);
         return v;
     }
-    if (sizeof(T) == 2 && c >= end) return u32x4{0, 0, 0, 0};                     // (adapters of rank 32: 80 -> 75 us; 4 elements are as soon looked at)
+    // (16 bits: adapters of rank 32 beside 16,384 x 1024 x 2048 80 -> 75 us; two or four elements are looked at as soon)
+    if (sizeof(T) == 2 && c >= end) return u32x4{0, 0, 0, 0};
     T e[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) e[j] = c + j < end ? line[c + j] : (T)0;
@@ -204,7 +205,8 @@ __device__ __forceinline__ u32x4 strided_fragment(const char* tile, int h, int c
         const int k = 32 * h + 8 * kk + (l15 >> 2);
         const int at = k * (C * 2) + (((c / 16) ^ spread<T, C>(k)) << 5) + (l15 & 3) * 8;
         const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(tile + at)));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(tile + (at + 4 * (C * 2)))));    // spread(k + 4) == spread(k)
+        // (spread(k + 4) == spread(k))
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(tile + (at + 4 * (C * 2)))));
         f = u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
         T e[E];

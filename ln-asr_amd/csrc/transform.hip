@@ -14,7 +14,8 @@ int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out) {
     if (bytes > b.cap || !b.p) {
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         LN_HIP(hipStreamIsCapturing(ctx->stream, &st));
-        LN_REQUIRE(st == hipStreamCaptureStatusNone, "a workspace of %zu bytes cannot be allocated while the stream is captured: run the call once before", bytes);
+        LN_REQUIRE(st == hipStreamCaptureStatusNone,
+                   "a workspace of %zu bytes cannot be allocated while the stream is captured: run the call once before", bytes);
         if (ctx->tr_captured) {                           // (left to the graphs; twice as large, so that few are)
             bytes = std::max(bytes, 2 * b.cap);
             b = DevBuf();
@@ -148,7 +149,8 @@ int segments(Call& c, const int64_t* offsets, const int32_t* slots, int S, int G
         LN_REQUIRE(offsets[0] >= 0 && offsets[S] <= rows, "offsets run from %lld to %lld, there are %lld rows", (long long)offsets[0],
                    (long long)offsets[S], (long long)rows);
         for (int s = 0; s < S; ++s)
-            LN_REQUIRE(offsets[s] <= offsets[s + 1], "offsets fall from %lld to %lld at segment %d", (long long)offsets[s], (long long)offsets[s + 1], s);
+            LN_REQUIRE(offsets[s] <= offsets[s + 1], "offsets fall from %lld to %lld at segment %d", (long long)offsets[s],
+                       (long long)offsets[s + 1], s);
         known = offsets[0] == 0 && offsets[S] == rows;
     }
     const void* d;

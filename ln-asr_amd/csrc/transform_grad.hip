@@ -290,9 +290,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
             };
             if (full > 0) bring(0);
             const int rest = rows - full * KB;
-            auto load_rest = [&]() { load(rest, [&](int k) { return row0 + full * KB + k; }); };
-            constexpr bool EARLY = TI * TJ < 256 * 256;                               // (registers)
-            if (EARLY && rest > 0) load_rest();
+            if (rest > 0) load(rest, [&](int k) { return row0 + full * KB + k; });
             __syncthreads();
             for (int i = 0; i < full; ++i) {
                 if (i + 1 < full) bring((i + 1) & 1);
@@ -300,7 +298,6 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
                 __syncthreads();
             }
             if (rest > 0) {
-                if (!EARLY) load_rest();
                 store(0);
                 __syncthreads();
                 multiply(0);

@@ -240,7 +240,8 @@ int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const ch
 // 60).  187 MB take 36 us at a large copy's rate; the rest is the blocks' start and end, eight to sixteen chunks a wave.
 // ------------------------------------------------------------------------------------------
 template <typename T, int IF, int JF, int HA, int HB>
-__global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts, typename Mat<T>::Sum* col_parts, int wave_lds) {
+__global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts,
+                                                                                    typename Mat<T>::Sum* col_parts, int wave_lds) {
     using M = Mat<T>;
     using Sum = typename M::Sum;
     constexpr int SZ = (int)sizeof(T), E = M::E, R = SZ == 2 ? 32 : 16, H = R / (4 * E);
@@ -387,7 +388,10 @@ static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name)
     constexpr int HA = R * 16 * IF * SZ / 1024, HB = R * 16 * JF * SZ / 1024;
     const int64_t size = (int64_t)a.I * a.J + a.I;
     int ts = 8;
-    while (ts < 40 && ((a.sg.rows >> ts) > 2 * ctx->prop.multiProcessorCount || (a.sg.rows >> ts) * size * (int64_t)sizeof(Sum) > (256ll << 20))) ++ts;
+    // spans: as many as the CUs hold blocks of 64-bit sums (fp64 300,007 x 39 x 39 with the join: 68 us; twice as many 71, four times 73),
+    // and no more than 256 MB of sums
+    const int64_t most = 2 * ctx->prop.multiProcessorCount;
+    while (ts < 40 && ((a.sg.rows >> ts) > most || (a.sg.rows >> ts) * size * (int64_t)sizeof(Sum) > (256ll << 20))) ++ts;
     const int64_t spans = (a.sg.rows >> ts) + a.groups;
     LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d groups are too many for one call", (long long)a.sg.rows, a.groups);
     void* parts = nullptr;
@@ -397,17 +401,20 @@ static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name)
     const int wave_lds = (R * a.I * SZ + 15) / 16 * 16 + (R * a.J * SZ + 15) / 16 * 16;
     const int lds = std::max(4 * wave_lds, 16 * IF * 16 * JF * (int)sizeof(Sum));
     LN_LAUNCH(ctx, name, (sum_narrow<T, IF, JF, HA, HB>), dim3((unsigned)spans), dim3(256), lds, a, ts, (Sum*)parts, cp, wave_lds);
-    return split ? transform_join(ctx, a, sizeof(T) == 8 ? LNASR_F64 : sizeof(T) == 4 ? LNASR_F32 : std::is_same<T, _Float16>::value ? LNASR_F16 : LNASR_BF16,
-                                  ts, parts, cp)
-                 : 0;
+    constexpr int dtype = SZ == 8 ? LNASR_F64 : SZ == 4 ? LNASR_F32 : std::is_same<T, _Float16>::value ? LNASR_F16 : LNASR_BF16;
+    return split ? transform_join(ctx, a, dtype, ts, parts, cp) : 0;
 }
 
 template <typename T>
 static int sum_narrow_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
-    const int j = a.J + (a.cols ? 1 : 0);
+    const int j = a.J + (a.cols ? 1 : 0);              // columns of b, and the ones
     if (a.I <= 16) return j <= 48 ? launch_sum_narrow<T, 1, 3>(ctx, a, name) : launch_sum_narrow<T, 1, 4>(ctx, a, name);
-    if (a.I <= 48) return j <= 16 ? launch_sum_narrow<T, 3, 1>(ctx, a, name) : j <= 48 ? launch_sum_narrow<T, 3, 3>(ctx, a, name) : launch_sum_narrow<T, 3, 4>(ctx, a, name);
-    return j <= 16 ? launch_sum_narrow<T, 4, 1>(ctx, a, name) : j <= 48 ? launch_sum_narrow<T, 4, 3>(ctx, a, name) : launch_sum_narrow<T, 4, 4>(ctx, a, name);
+    if (a.I <= 48) {
+        if (j <= 16) return launch_sum_narrow<T, 3, 1>(ctx, a, name);
+        return j <= 48 ? launch_sum_narrow<T, 3, 3>(ctx, a, name) : launch_sum_narrow<T, 3, 4>(ctx, a, name);
+    }
+    if (j <= 16) return launch_sum_narrow<T, 4, 1>(ctx, a, name);
+    return j <= 48 ? launch_sum_narrow<T, 4, 3>(ctx, a, name) : launch_sum_narrow<T, 4, 4>(ctx, a, name);
 }
 
 bool sum_narrow_ok(const SumArgs& a) {
