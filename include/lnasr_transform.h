@@ -48,7 +48,8 @@ int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, in
                       const int32_t* slots_or_null, int S, const void* w, int G, int dout, const void* dy, int64_t lddy,
                       void* dx_or_null, int64_t lddx, void* dw_or_null, void* dbias_or_null);
 /* y[r] = W x[r] + bias + scale[k] B[k] (A[k] x[r]): w [dout, din], bias [dout] or NULL, a [G, rank, din], b [G, dout, rank],
- * scale [G] fp64 or NULL (1).  Slot -1: the projection alone.  The middle (scale A x) is held in `dtype`. */
+ * scale [G] fp64 or NULL (1).  Slot -1: the projection alone.  The middle (scale A x; in the gradients scale B^T dy, too) is held in
+ * 64 bits for F64, in 32 for the others. */
 int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din, int64_t ldx, const int64_t* offsets,
                      const int32_t* slots_or_null, int S, const void* w, const void* bias_or_null, int dout, const void* a,
                      const void* b, const double* scale_or_null, int G, int rank, void* y, int64_t ldy);

@@ -2,6 +2,8 @@
 // points and dispatch; transform_rows.hip: products with one result row per feature row; transform_grad.hip: products that
 // sum over rows).  Internal.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace lnasr {
@@ -66,6 +68,11 @@ struct Mat<__bf16> {
     }
     static __device__ __forceinline__ int row(int r, int kk) { return 4 * kk + r; }
 };
+
+// The type a projection's narrow middle is held in: never under 32 bits.  (Rounded to 16 bits it took a whole rounding more than the
+// results' own, and in f16 a middle past 65504 was lost.)
+template <typename T>
+using Mid = std::conditional_t<sizeof(T) == 2, float, T>;
 
 template <typename T>
 __device__ __forceinline__ typename Mat<T>::Acc mma(u32x4 a, u32x4 b, typename Mat<T>::Acc c) {
@@ -155,6 +162,29 @@ __device__ __forceinline__ u32x4 load_piece(const T* line, long c, long end) {
     return v;
 }
 
+// the same as values of type U, which may be wider than those of the line
+template <typename U, typename T>
+__device__ __forceinline__ u32x4 load_as(const T* line, long c, long end) {
+    if constexpr (std::is_same<U, T>::value) {
+        return load_piece(line, c, end);
+    } else {
+        constexpr int E = Mat<U>::E;
+        T t[E];
+        if (c + E <= end) {
+            __builtin_memcpy(t, line + c, sizeof(t));
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) t[j] = c + j < end ? line[c + j] : (T)0;
+        }
+        U e[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) e[j] = (U)t[j];
+        u32x4 v;
+        __builtin_memcpy(&v, e, 16);
+        return v;
+    }
+}
+
 // LDS of one wave is its own: order its writes and reads for the compiler (the hardware keeps the order of a wave's LDS accesses)
 __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -183,22 +213,23 @@ __device__ __forceinline__ void bring_piece(const char* base, unsigned offset, c
 
 // A tile of C columns whose k is strided, in LDS as lines of k: the run of 16 columns (sizeof(T) pieces) at place p of line k
 // is run p ^ spread(k), so that the lines one fragment read touches (they differ in (lane & 15) >> 2 and lane >> 4 for 16 bit,
-// in lane >> 4 alone for the others) lie in other banks.
-template <typename T, int C>
+// in lane >> 4 alone for the others) lie in other banks.  U: the type the values are multiplied in, T or a wider one.
+template <typename T, int C, typename U = T>
 __device__ __forceinline__ int spread(int k) {
     constexpr int RUNS = C / 16;
     if ((RUNS & (RUNS - 1)) != 0) return 0;
+    if (sizeof(U) != sizeof(T)) return k >> 2 & (RUNS < 4 ? RUNS - 1 : 3);
     if (sizeof(T) == 2) return ((k & 3) | (k >> 1 & 4)) & (RUNS < 8 ? RUNS - 1 : 7);
     if (sizeof(T) == 4) return k >> 2 & (RUNS < 4 ? RUNS - 1 : 3);
     return k >> 1 & (RUNS < 2 ? RUNS - 1 : 1);
 }
-// the wave's fragment of columns c .. c + 15 (c a multiple of 16), half h of the 128 bytes of k
-template <typename T, int C>
+// the wave's fragment of columns c .. c + 15 (c a multiple of 16) as values of type U, half h of their 128 bytes of k
+template <typename T, int C, typename U = T>
 __device__ __forceinline__ u32x4 strided_fragment(const char* tile, int h, int c) {
-    constexpr int SZ = (int)sizeof(T), E = Mat<T>::E;
+    constexpr int SZ = (int)sizeof(T), E = Mat<U>::E;
     const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
     u32x4 f;
-    if constexpr (SZ == 2) {
+    if constexpr (SZ == 2 && sizeof(U) == 2) {
         // each 16 lanes read 4 lines of 16 columns, 8 bytes a lane; the lane gets the 4 k of its column
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4 lds16x4;
@@ -209,11 +240,11 @@ __device__ __forceinline__ u32x4 strided_fragment(const char* tile, int h, int c
         const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(tile + (at + 4 * (C * 2)))));
         f = u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
-        T e[E];
+        U e[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             const int k = (4 * h + kk) * E + j;
-            e[j] = *(const T*)(tile + k * (C * SZ) + (((c / 16) ^ spread<T, C>(k)) * 16 + l15) * SZ);
+            e[j] = (U) * (const T*)(tile + k * (C * SZ) + (((c / 16) ^ spread<T, C, U>(k)) * 16 + l15) * SZ);
         }
         __builtin_memcpy(&f, e, 16);
     }
@@ -222,7 +253,7 @@ __device__ __forceinline__ u32x4 strided_fragment(const char* tile, int h, int c
 
 // y[r, :] = scale_k * (x[r, :] W_k') + bias_k  for the rows of the segments; W_k' = W_k^T (kn false, W_k [n, k]) or W_k (kn
 // true, W_k [k, n]).  w_stride 0: one W for all rows, tiles of rows then run across segments; with `low` each row also gets
-// p[r, :] L_k' of its segment's group (none where the group is negative).
+// p[r, :] L_k' of its segment's group (none where the group is negative).  p, and y where `mid` says so, are of type Mid.
 struct RowsArgs {
     Segments sg;
     const void *x, *w, *bias, *p, *low;
@@ -231,12 +262,12 @@ struct RowsArgs {
     int64_t ldx, ldy, ldp;
     int64_t w_stride, bias_stride, low_stride;
     int K, N, R;
-    bool kn;
+    bool kn, mid;
 };
 int transform_rows(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name);
 
 // out[k, i, j] = sum over the rows r of group k of a[r, i] b[r, j];  cols[k, i] = sum of a[r, i] (or null).  Every group is
-// written, zeros where it has no rows.
+// written, zeros where it has no rows.  a is of type Mid with mid_a, b with mid_b (one of them at most, and then no cols).
 struct SumArgs {
     Segments sg;
     const int64_t* group_off;   // group g: places group_off[g * group_step] .. group_off[(g + 1) * group_step] of the sorted rows
@@ -248,6 +279,7 @@ struct SumArgs {
     void *out, *cols;
     int64_t lda, ldb;
     int groups, I, J;
+    bool mid_a, mid_b;
 };
 // Span t of 2^ts places of the sorted rows: its group, first place and rows; false: nothing to do.  (A group without rows has one
 // span without rows, to be written as zeros.)
@@ -300,5 +332,6 @@ enum { kTrX, kTrOff, kTrSlots, kTrW, kTrBias, kTrA, kTrB, kTrScale, kTrDy, kTrOu
        kTrSort, kTrPart, kTrCount };
 
 inline size_t transform_size(int dtype) { return dtype == LNASR_F64 ? 8 : dtype == LNASR_F32 ? 4 : 2; }
+inline size_t transform_mid_size(int dtype) { return dtype == LNASR_F64 ? 8 : 4; }
 
 }  // namespace lnasr

@@ -315,11 +315,12 @@ int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int
     m.K = low.K = din;
     m.N = dout;
     if (G > 0) {
-        // the narrow middle, held in the type of the features (one rounding more than the formula: at most half a step of each
-        // of its values), rows padded to whole 16-byte pieces
-        const int64_t ldp = (rank * e + 15) / 16 * 16 / e;
+        // the narrow middle, held in 32 bits or more, rows padded to whole 16-byte pieces
+        const size_t me = transform_mid_size(dtype);
+        const int64_t ldp = (rank * me + 15) / 16 * 16 / me;
         void* p;
-        LN_TRY(transform_ws(ctx, kTrLow, (size_t)rows * ldp * e, &p));
+        LN_TRY(transform_ws(ctx, kTrLow, (size_t)rows * ldp * me, &p));
+        low.mid = true;
         low.x = m.x;
         low.w_stride = (int64_t)rank * din;
         low.y = p;
@@ -373,15 +374,17 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
     LN_TRY(c.out(db, (size_t)G * dout * rank * e, kTrOut2, false, "db", &d_db));
     LN_TRY(c.out(dw, (size_t)dout * din * e, kTrOut3, false, "dw", &d_dw));
     LN_TRY(c.out(dbias, (size_t)dout * e, kTrOut4, false, "dbias", &d_dbias));
-    const int64_t ldp = (rank * e + 15) / 16 * 16 / e;
+    const size_t me = transform_mid_size(dtype);
+    const int64_t ldp = (rank * me + 15) / 16 * 16 / me;
     RowsArgs r{};
     r.sg = sg;
+    r.mid = true;
     r.scale = d_scale;
     r.ldy = ldp;
     r.N = rank;
     r.w_stride = (int64_t)rank * din;
     if (G > 0 && (d_dx || d_da)) {                       // scale_k B_k^T dy
-        LN_TRY(transform_ws(ctx, kTrDlow, (size_t)rows * ldp * e, &dp));
+        LN_TRY(transform_ws(ctx, kTrDlow, (size_t)rows * ldp * me, &dp));
         r.x = d_dy;
         r.ldx = lddy;
         r.K = dout;
@@ -392,7 +395,7 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
         LN_TRY(transform_rows(ctx, dtype, r, "projection_dlow"));
     }
     if (d_db) {                                          // scale_k A_k x
-        LN_TRY(transform_ws(ctx, kTrLow, (size_t)rows * ldp * e, &p));
+        LN_TRY(transform_ws(ctx, kTrLow, (size_t)rows * ldp * me, &p));
         r.x = d_x;
         r.ldx = ldx;
         r.K = din;
@@ -436,6 +439,7 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
         t.b = d_x;
         t.ldb = ldx;
         t.J = din;
+        t.mid_a = true;
         t.out = d_da;
         LN_TRY(transform_sum(ctx, dtype, t, "projection_da"));
     }
@@ -446,6 +450,8 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
         t.b = p;
         t.ldb = ldp;
         t.J = rank;
+        t.mid_a = false;
+        t.mid_b = true;
         t.out = d_db;
         LN_TRY(transform_sum(ctx, dtype, t, "projection_db"));
     }

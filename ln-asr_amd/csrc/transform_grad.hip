@@ -178,26 +178,36 @@ __device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int
 // LDS-DMA step by step, the last and uneven one through registers; otherwise -- segments of a few rows -- all of them through
 // registers, row by row as rowmap says, loaded a step ahead.  A group with one span is written at once, the others leave sums of 32
 // bits or more per span, which join_parts adds in the order of the spans.
+// A: the type of a, B: of b; where they differ (the gradients of adapters) both are multiplied in the wider one, C.
 // f32 20,011 rows x 512 x 429: 98 us, 90 TFLOP/s of the 153 of a large library product (CUs busy 72 % of the time: 1120 blocks on
 // 1280 places).  bf16 16,384 rows x 16 x 1024: 11.6 us, 34 MB.
 // ------------------------------------------------------------------------------------------
-template <typename T, int TI, int TJ, int WI, int WJ, bool TOGETHER>
+template <typename A, typename B>
+using Wider = std::conditional_t<(sizeof(A) >= sizeof(B)), A, B>;
+// bytes of a step of a and b in LDS
+template <typename A, typename B, int TI, int TJ>
+constexpr int sum_step() {
+    return 128 / (int)sizeof(Wider<A, B>) * (TI * (int)sizeof(A) + TJ * (int)sizeof(B));
+}
+template <typename T, typename A, typename B, int TI, int TJ, int WI, int WJ, bool TOGETHER>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned tiles_i, unsigned tiles_j, int ts, typename Mat<T>::Sum* parts,
                                                             typename Mat<T>::Sum* col_parts) {
-    using M = Mat<T>;
+    using C = Wider<A, B>;
+    using M = Mat<C>;
     using Acc = typename M::Acc;
-    constexpr int SZ = (int)sizeof(T), E = M::E, KB = 128 / SZ, NT = 64 * WI * WJ, IR = TI / WI / 16, JR = TJ / WJ / 16;
-    constexpr int AL = TI * SZ / 16, BL = TJ * SZ / 16;                               // pieces of a line
-    constexpr int AP = (TI * 8 + NT - 1) / NT, BP = (TJ * 8 + NT - 1) / NT;
-    static_assert(TI * 8 % 64 == 0 && TJ * 8 % 64 == 0, "whole waves of pieces");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (TI + TJ) * 128];
+    constexpr int SA = (int)sizeof(A), SB = (int)sizeof(B), EA = 16 / SA, EB = 16 / SB, KB = 128 / (int)sizeof(C), NT = 64 * WI * WJ;
+    constexpr int IR = TI / WI / 16, JR = TJ / WJ / 16, STEP = sum_step<A, B, TI, TJ>(), BAT = TI * SA * KB;
+    constexpr int AL = TI * SA / 16, BL = TJ * SB / 16;                               // pieces of a line
+    constexpr int AN = KB * AL, BN = KB * BL, AP = (AN + NT - 1) / NT, BP = (BN + NT - 1) / NT;
+    static_assert(AN % 64 == 0 && BN % 64 == 0, "whole waves of pieces");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STEP];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wi = wave / WJ * (TI / WI), wj = wave % WJ * (TJ / WJ);
     const unsigned tiles = tiles_i * tiles_j, id = die_order(blockIdx.x, gridDim.x);
     const int i0 = (int)(id % tiles / tiles_j) * TI, j0 = (int)(id % tiles_j) * TJ;
     const int64_t t = id / tiles;
-    auto brings_a = [&](int i) { return TI * 8 % NT == 0 || wave * 64 + NT * i < TI * 8; };
-    auto brings_b = [&](int i) { return TJ * 8 % NT == 0 || wave * 64 + NT * i < TJ * 8; };
+    auto brings_a = [&](int i) { return AN % NT == 0 || wave * 64 + NT * i < AN; };
+    auto brings_b = [&](int i) { return BN % NT == 0 || wave * 64 + NT * i < BN; };
     int g, n;
     int64_t q0;
     bool whole;
@@ -213,25 +223,25 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
     const bool want_col = a.cols && j0 == 0 && wj == 0;
     u32x4 ones;
     {
-        T e[E];
+        C e[M::E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) e[j] = (T)1;
+        for (int j = 0; j < M::E; ++j) e[j] = (C)1;
         __builtin_memcpy(&ones, e, 16);
     }
     auto multiply = [&](int buf) {
-        const char* as = lds + buf * (TI + TJ) * 128;
-        const char* bs = as + TI * 128;
+        const char* as = lds + buf * STEP;
+        const char* bs = as + BAT;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             u32x4 af[IR], bf[JR];
 #pragma unroll
-            for (int i = 0; i < IR; ++i) af[i] = strided_fragment<T, TI>(as, h, wi + 16 * i);
+            for (int i = 0; i < IR; ++i) af[i] = strided_fragment<A, TI, C>(as, h, wi + 16 * i);
 #pragma unroll
-            for (int j = 0; j < JR; ++j) bf[j] = strided_fragment<T, TJ>(bs, h, wj + 16 * j);
-            mma_all<T>(af, bf, acc);
+            for (int j = 0; j < JR; ++j) bf[j] = strided_fragment<B, TJ, C>(bs, h, wj + 16 * j);
+            mma_all<C>(af, bf, acc);
             if (want_col)
 #pragma unroll
-                for (int i = 0; i < IR; ++i) col[i] = mma<T>(af[i], ones, col[i]);
+                for (int i = 0; i < IR; ++i) col[i] = mma<C>(af[i], ones, col[i]);
         }
     };
     // a step through registers: row(k) of its k-th place, for k < left; zeros for the others and past the last column
@@ -239,23 +249,23 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
     auto load = [&](int left, auto row) {
 #pragma unroll
         for (int i = 0; i < AP; ++i) {
-            const int q = tid + NT * i, k = q / AL, c = i0 + (q % AL ^ spread<T, TI>(k) * SZ) * E;
-            if (brings_a(i)) ar[i] = k < left ? load_piece((const T*)a.a + row(k) * a.lda, c, a.I) : u32x4{0, 0, 0, 0};
+            const int q = tid + NT * i, k = q / AL, c = i0 + (q % AL ^ spread<A, TI, C>(k) * SA) * EA;
+            if (brings_a(i)) ar[i] = k < left ? load_piece((const A*)a.a + row(k) * a.lda, c, a.I) : u32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int i = 0; i < BP; ++i) {
-            const int q = tid + NT * i, k = q / BL, c = j0 + (q % BL ^ spread<T, TJ>(k) * SZ) * E;
-            if (brings_b(i)) br[i] = k < left ? load_piece((const T*)a.b + row(k) * a.ldb, c, a.J) : u32x4{0, 0, 0, 0};
+            const int q = tid + NT * i, k = q / BL, c = j0 + (q % BL ^ spread<B, TJ, C>(k) * SB) * EB;
+            if (brings_b(i)) br[i] = k < left ? load_piece((const B*)a.b + row(k) * a.ldb, c, a.J) : u32x4{0, 0, 0, 0};
         }
     };
     auto store = [&](int buf) {
-        char* as = lds + buf * (TI + TJ) * 128;
+        char* as = lds + buf * STEP;
 #pragma unroll
         for (int i = 0; i < AP; ++i)
             if (brings_a(i)) *(u32x4*)(as + (tid + NT * i) * 16) = ar[i];
 #pragma unroll
         for (int i = 0; i < BP; ++i)
-            if (brings_b(i)) *(u32x4*)(as + TI * 128 + (tid + NT * i) * 16) = br[i];
+            if (brings_b(i)) *(u32x4*)(as + BAT + (tid + NT * i) * 16) = br[i];
     };
     if constexpr (TOGETHER) {
         // offsets of this lane's pieces from the step's first; out of range (nothing is read, LDS gets zeros) past the last column.
@@ -264,29 +274,29 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
         unsigned ao[AP], bo[BP];
 #pragma unroll
         for (int i = 0; i < AP; ++i) {
-            const int q = tid + NT * i, k = q / AL, c = (q % AL ^ spread<T, TI>(k) * SZ) * E;
-            ao[i] = i0 + c < a.I ? (unsigned)k * (unsigned)(a.lda * SZ) + c * SZ : 0xffffffffu;
+            const int q = tid + NT * i, k = q / AL, c = (q % AL ^ spread<A, TI, C>(k) * SA) * EA;
+            ao[i] = i0 + c < a.I ? (unsigned)k * (unsigned)(a.lda * SA) + c * SA : 0xffffffffu;
         }
 #pragma unroll
         for (int i = 0; i < BP; ++i) {
-            const int q = tid + NT * i, k = q / BL, c = (q % BL ^ spread<T, TJ>(k) * SZ) * E;
-            bo[i] = j0 + c < a.J ? (unsigned)k * (unsigned)(a.ldb * SZ) + c * SZ : 0xffffffffu;
+            const int q = tid + NT * i, k = q / BL, c = (q % BL ^ spread<B, TJ, C>(k) * SB) * EB;
+            bo[i] = j0 + c < a.J ? (unsigned)k * (unsigned)(a.ldb * SB) + c * SB : 0xffffffffu;
         }
-        const int uneven = a.I % E || a.J % E ? 1 : 0;
+        const int uneven = a.I % EA || a.J % EB ? 1 : 0;
         each_run(a, q0, q0 + n, [&](int64_t row0, int rows) {
             const int full = (rows - uneven) / KB;
-            const char* ab = (const char*)((const T*)a.a + row0 * a.lda + i0);
-            const char* bb = (const char*)((const T*)a.b + row0 * a.ldb + j0);
+            const char* ab = (const char*)((const A*)a.a + row0 * a.lda + i0);
+            const char* bb = (const char*)((const B*)a.b + row0 * a.ldb + j0);
             auto bring = [&](int buf) {
-                char* as = lds + buf * (TI + TJ) * 128;
+                char* as = lds + buf * STEP;
 #pragma unroll
                 for (int i = 0; i < AP; ++i)
                     if (brings_a(i)) bring_piece(ab, ao[i], as + (wave * 64 + NT * i) * 16);
 #pragma unroll
                 for (int i = 0; i < BP; ++i)
-                    if (brings_b(i)) bring_piece(bb, bo[i], as + TI * 128 + (wave * 64 + NT * i) * 16);
-                ab += KB * a.lda * SZ;
-                bb += KB * a.ldb * SZ;
+                    if (brings_b(i)) bring_piece(bb, bo[i], as + BAT + (wave * 64 + NT * i) * 16);
+                ab += KB * a.lda * SA;
+                bb += KB * a.ldb * SB;
             };
             if (full > 0) bring(0);
             const int rest = rows - full * KB;
@@ -604,10 +614,10 @@ static int span_length(const SumArgs& a, int64_t tiles, int64_t want, size_t sum
     return ts;
 }
 
-template <typename T, int TI, int TJ, int WI, int WJ>
+template <typename T, int TI, int TJ, int WI, int WJ, typename A = T, typename B = T>
 static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     using Sum = typename Mat<T>::Sum;
-    constexpr int KB = 128 / (int)sizeof(T), HOLDS = std::min(8, (160 << 10) / (2 * (TI + TJ) * 128));
+    constexpr int KB = 128 / (int)sizeof(Wider<A, B>), HOLDS = std::min(8, (160 << 10) / (2 * sum_step<A, B, TI, TJ>()));
     const int64_t ti = (a.I + TI - 1) / TI, tj = (a.J + TJ - 1) / TJ, size = (int64_t)a.I * a.J + a.I;
     const int ts = span_length(a, ti * tj, (int64_t)HOLDS * ctx->prop.multiProcessorCount, sizeof(Sum));
     const int64_t spans = (a.sg.rows >> ts) + a.groups;
@@ -619,9 +629,9 @@ static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     Sum* cp = (Sum*)parts + spans * a.I * a.J;
     const dim3 grid((unsigned)(spans * ti * tj)), block(64 * WI * WJ);
     // (with rowmap the segments are short: rows_together)
-    const bool together = !a.rowmap && std::max(a.lda, a.ldb) * KB * (int64_t)sizeof(T) < (1ll << 31);
-    if (together) LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, true>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
-    else LN_LAUNCH(ctx, name, (sum_tile<T, TI, TJ, WI, WJ, false>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
+    const bool together = !a.rowmap && std::max(a.lda * (int64_t)sizeof(A), a.ldb * (int64_t)sizeof(B)) * KB < (1ll << 31);
+    if (together) LN_LAUNCH(ctx, name, (sum_tile<T, A, B, TI, TJ, WI, WJ, true>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
+    else LN_LAUNCH(ctx, name, (sum_tile<T, A, B, TI, TJ, WI, WJ, false>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
     return split ? join_t<T>(ctx, a, ts, parts, cp) : 0;
 }
 
@@ -651,6 +661,18 @@ static int launch_sum_deep(lnasr_ctx* ctx, SumArgs a, const char* name) {
 
 template <typename T>
 static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
+    if constexpr (!std::is_same<T, Mid<T>>::value) {
+        if (a.mid_a) {
+            if (a.I <= 16) return launch_sum<T, 16, 128, 1, 4, Mid<T>, T>(ctx, a, name);
+            if (a.I <= 32) return launch_sum<T, 32, 128, 1, 4, Mid<T>, T>(ctx, a, name);
+            return launch_sum<T, 64, 64, 2, 2, Mid<T>, T>(ctx, a, name);
+        }
+        if (a.mid_b) {
+            if (a.J <= 16) return launch_sum<T, 128, 16, 4, 1, T, Mid<T>>(ctx, a, name);
+            if (a.J <= 32) return launch_sum<T, 128, 32, 4, 1, T, Mid<T>>(ctx, a, name);
+            return launch_sum<T, 64, 64, 2, 2, T, Mid<T>>(ctx, a, name);
+        }
+    }
     if (a.I <= 16) return launch_sum<T, 16, 128, 1, 4>(ctx, a, name);
     if (a.J <= 16) return launch_sum<T, 128, 16, 4, 1>(ctx, a, name);
     if (a.I <= 32) return launch_sum<T, 32, 128, 1, 4>(ctx, a, name);
@@ -666,7 +688,7 @@ static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
 
 int transform_sum(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name) {
     if (a.groups == 0) return 0;
-    if (sum_narrow_ok(a)) return transform_sum_narrow(ctx, dtype, a, name);
+    if (sum_narrow_ok(a) && !((a.mid_a || a.mid_b) && transform_size(dtype) == 2)) return transform_sum_narrow(ctx, dtype, a, name);
     switch (dtype) {
         case LNASR_F64: return sum_t<double>(ctx, a, name);
         case LNASR_F32: return sum_t<float>(ctx, a, name);

@@ -11,12 +11,12 @@ namespace lnasr {
 template <typename T, bool KN, int MR, int NR>
 __device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, int64_t row1, int c0, int turn, int turns,
                                              typename Mat<T>::Acc (&acc)[NR][MR]) {
-    using M = Mat<T>;
-    constexpr int E = M::E;
+    using U = Mid<T>;                                     // (the adapters' matrices, too, are multiplied as values of this type)
+    constexpr int E = Mat<U>::E;
     const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
     if (row0 >= row1) return;
     const int last = (int)(row1 - 1 - row0);
-    const T* p = (const T*)a.p + row0 * a.ldp;
+    const U* p = (const U*)a.p + row0 * a.ldp;
     int count = 0;
     for (int s = max(0, wave_search(a.sg.S, row0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; s += 64) {
         const int mine = min(s + lane, a.sg.S - 1);
@@ -34,12 +34,12 @@ __device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, in
                 for (int n = 0; n < NR; ++n) {
                     const int c = min(c0 + 16 * n + l15, a.N - 1);
                     if (KN) {
-                        T e[E];
+                        U e[E];
 #pragma unroll
-                        for (int j = 0; j < E; ++j) e[j] = k + j < a.R ? low[(int64_t)(k + j) * a.N + c] : (T)0;
+                        for (int j = 0; j < E; ++j) e[j] = k + j < a.R ? (U)low[(int64_t)(k + j) * a.N + c] : (U)0;
                         __builtin_memcpy(&wf[n], e, 16);
                     } else {
-                        wf[n] = load_piece(low + (int64_t)c * a.R, k, a.R);
+                        wf[n] = load_as<U>(low + (int64_t)c * a.R, k, a.R);
                     }
                 }
 #pragma unroll
@@ -51,7 +51,7 @@ __device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, in
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
                         // chosen, not masked by a product with zero: another row's adapter may hold a NaN
-                        const typename M::Acc d = mma<T>(wf[n], pf, acc[n][m]);
+                        const typename Mat<U>::Acc d = mma<U>(wf[n], pf, acc[n][m]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
                     }
@@ -65,16 +65,17 @@ __device__ __forceinline__ void add_adapters(const RowsArgs& a, int64_t row0, in
 // Writes acc (times scale, plus bias) to the rows row0 + 16 m + (lane & 15) < row1, columns c0 + 16 n ..  Sixteen rows at a time pass
 // through `scratch` (the wave's own put_scratch bytes of LDS), so that a row's results leave as whole runs of 16-byte pieces: as the
 // matrix instruction leaves them, 32 bytes of a row at a time, twice the bytes went out to memory.
-template <typename T, int NR>
+// Y: the type of the results.
+template <typename Y, int NR>
 constexpr int put_scratch() {
-    return 16 * (NR * 16 * (int)sizeof(T) + 16);
+    return 16 * (NR * 16 * (int)sizeof(Y) + 16);
 }
-template <typename T, int MR, int NR>
+template <typename T, typename Y, int MR, int NR>
 __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_t row1, int c0, typename Mat<T>::Sum scale, const T* bias,
                                          const typename Mat<T>::Acc (&acc)[NR][MR], char* scratch) {
     using M = Mat<T>;
     using Sum = typename M::Sum;
-    constexpr int SZ = (int)sizeof(T), E = M::E, PITCH = NR * 16 * SZ + 16, PER = NR * SZ;       // bytes, pieces of a row
+    constexpr int SZ = (int)sizeof(Y), E = 16 / SZ, PITCH = NR * 16 * SZ + 16, PER = NR * SZ;    // bytes, pieces of a row
     const int lane = threadIdx.x & 63, l15 = lane & 15, kk = lane >> 4;
     Sum bv[NR][4];
 #pragma unroll
@@ -89,14 +90,14 @@ __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_
         if (row0 + 16 * m >= row1) break;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            T v[4];
+            Y v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(acc[n][m][r] * scale + bv[n][r]);             // the one rounding of the result
+            for (int r = 0; r < 4; ++r) v[r] = (Y)(acc[n][m][r] * scale + bv[n][r]);             // the one rounding of the result
             if constexpr (SZ != 8) {
                 __builtin_memcpy(scratch + l15 * PITCH + (16 * n + 4 * kk) * SZ, v, 4 * SZ);
             } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) *(T*)(scratch + l15 * PITCH + (16 * n + M::row(r, kk)) * SZ) = v[r];
+                for (int r = 0; r < 4; ++r) *(Y*)(scratch + l15 * PITCH + (16 * n + M::row(r, kk)) * SZ) = v[r];
             }
         }
         wave_lds_order();
@@ -105,12 +106,12 @@ __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_
             const int q = lane + 64 * i, row = q / PER, c = c0 + q % PER * E;
             if (q >= 16 * PER || row0 + 16 * m + row >= row1 || c >= a.N) continue;
             const char* from = scratch + row * PITCH + q % PER * 16;
-            T* y = (T*)a.y + (row0 + 16 * m + row) * a.ldy + c;
+            Y* y = (Y*)a.y + (row0 + 16 * m + row) * a.ldy + c;
             if (c + E <= a.N) {
                 const u32x4 v = *(const u32x4*)from;
                 __builtin_memcpy(y, &v, 16);
             } else {
-                for (int j = 0; j < a.N - c; ++j) y[j] = *(const T*)(from + j * SZ);
+                for (int j = 0; j < a.N - c; ++j) y[j] = *(const Y*)(from + j * SZ);
             }
         }
         wave_lds_order();
@@ -123,13 +124,13 @@ __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_
 // bf16 64 single rows x 2048 -> 2048, 48 adapters of rank 16: 5.5 us for the middle and 12 for the rest, 15 MB; through the
 // tiles below 120.
 // ------------------------------------------------------------------------------------------
-template <typename T, bool KN, int MR, int LOW>
+template <typename T, typename Y, bool KN, int MR, int LOW>
 __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, int ts) {
     using M = Mat<T>;
     using Acc = typename M::Acc;
     constexpr int E = M::E, WAVES = 8, DEEP = MR == 1 ? 8 : MR == 2 ? 4 : 2;
     __shared__ Acc part[WAVES - 1][MR][64];
-    __shared__ __attribute__((aligned(16))) char scratch[put_scratch<T, 1>()];
+    __shared__ __attribute__((aligned(16))) char scratch[put_scratch<Y, 1>()];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
     const int c0 = (int)(blockIdx.x % tiles_n) * 16;
     int64_t r0, r1;
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 #pragma unroll
         for (int m = 0; m < MR; ++m) acc[0][m] += part[i][m][lane];
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
-    put_tile<T, MR, 1>(a, r0, r1, c0, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc, scratch);
+    put_tile<T, Y, MR, 1>(a, r0, r1, c0, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc, scratch);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 // 122 us, 88 TFLOP/s of the 153 of a large library product; 20,011 x 512 x 429 100 us, cores busy 59 % of the time.  With few results
 // they wait for memory: f32 200,003 x 351 x 40 95 us, 3.3 TB/s (rows of 351 values begin off any alignment: 352 take a fifth less).
 // ------------------------------------------------------------------------------------------
-template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW>
+template <typename T, typename Y, int TM, int TN, int WM, int WN, bool KN, int LOW>
 __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigned tiles_n, int ts, int full) {
     using M = Mat<T>;
     using Acc = typename M::Acc;
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     // (variables of their own, not one array: the compiler then knows that reading one does not wait for what is brought into another)
     constexpr bool THREE = SZ == 2 && 3 * (XB + WB) <= (160 << 10) / 3;
     __shared__ __attribute__((aligned(1024))) char l0[XB + WB], l1[XB + WB], l2[THREE ? XB + WB : 16];
-    constexpr int PUTS = (XB + WB) / put_scratch<T, NR>();                            // put_tile's rows: waves a buffer has room for
+    constexpr int PUTS = (XB + WB) / put_scratch<Y, NR>();                            // put_tile's rows: waves a buffer has room for
     static_assert((THREE ? 3 : 2) * PUTS >= WM * WN && PUTS > 0, "put_tile's rows");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
@@ -246,23 +247,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 #pragma unroll
         for (int m = 0; m < MR; ++m) acc[n][m] = Acc{0, 0, 0, 0};
 
-    // acc += X W' over the 128 bytes of k in a buffer; with SOME only for the rows from .. to - 1 of the wave's
-    auto multiply = [&](const char* xs, auto some, int from, int to, int left = 1 << 20) {
+    // acc += X W' over the 128 bytes of k, values of type U, in a buffer; with SOME only for the rows from .. to - 1 of the wave's
+    auto multiply = [&](auto type, const char* xs, auto some, int from, int to, int left = 1 << 20) {
+        using U = decltype(type);
         constexpr bool SOME = decltype(some)::value;
         const char* ws = xs + XB;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (SOME && h && left <= KB / 2) break;                                   // (an adapter of a low rank)
+            if (SOME && h && left <= 64 / (int)sizeof(U)) break;                      // (an adapter of a low rank)
             u32x4 xf[MR], wf[NR];
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 const int c = wn + 16 * n;
-                if constexpr (KN) wf[n] = strided_fragment<T, TN>(ws, h, c);
+                if constexpr (KN) wf[n] = strided_fragment<U, TN>(ws, h, c);
                 else wf[n] = *(const u32x4*)(ws + (c + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
             }
 #pragma unroll
             for (int m = 0; m < MR; ++m) xf[m] = *(const u32x4*)(xs + (wm + 16 * m + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
-            if constexpr (!SOME) mma_all<T>(wf, xf, acc);
+            if constexpr (!SOME) mma_all<U>(wf, xf, acc);
             else
 #pragma unroll
             for (int m = 0; m < MR; ++m) {
@@ -272,23 +274,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
                     const bool in = 16 * m + l15 >= from && 16 * m + l15 < to;
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
-                        const Acc d = mma<T>(wf[n], xf[m], acc[n][m]);
+                        const Acc d = mma<U>(wf[n], xf[m], acc[n][m]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
                     }
                 } else {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) acc[n][m] = mma<T>(wf[n], xf[m], acc[n][m]);
+                    for (int n = 0; n < NR; ++n) acc[n][m] = mma<U>(wf[n], xf[m], acc[n][m]);
                 }
             }
         }
     };
 
-    // a step through registers: what lies past klen (or, in a line of w, past N) is 0
+    // a step through registers, w as values of x's type: what lies past klen (or, in a line of w, past N) is 0
     struct Pieces {
         u32x4 x[XI], w[WI];
     };
-    auto fetch = [&](Pieces& p, const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen) {
+    auto fetch = [&](Pieces& p, auto x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen) {
+        using U = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+        constexpr int E = Mat<U>::E, LINE = TN * (int)sizeof(U) / 16;
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             const int q = tid + NT * i, row = q >> 3;
@@ -299,22 +303,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             if (!brings_w(i)) break;
             const int q = tid + NT * i;
             if (KN) {
-                const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
-                p.w[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
+                const int k = q / LINE, c = (q % LINE ^ spread<U, TN>(k) * (int)sizeof(U)) * E;
+                p.w[i] = k0 + k < klen ? load_as<U>(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
             } else {
                 const int row = q >> 3;
-                p.w[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
+                p.w[i] = load_as<U>(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
             }
         }
     };
-    auto apply = [&](const Pieces& p, auto some, int from, int to, int left = 1 << 20) {
+    auto apply = [&](auto type, const Pieces& p, auto some, int from, int to, int left = 1 << 20) {
 #pragma unroll
         for (int i = 0; i < XI; ++i) *(u32x4*)(l0 + (tid + NT * i) * 16) = p.x[i];
 #pragma unroll
         for (int i = 0; i < WI; ++i)
             if (brings_w(i)) *(u32x4*)(l0 + XB + (tid + NT * i) * 16) = p.w[i];
         __syncthreads();
-        multiply(l0, some, from, to, left);
+        multiply(type, l0, some, from, to, left);
         __syncthreads();
     };
 
@@ -335,7 +339,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
         }
         return a.sg.S;
     };
-    const T* p = (const T*)a.p + r0 * a.ldp;
+    using U = Mid<T>;                                                                 // (the adapters' products are of this type)
+    constexpr int KU = 128 / (int)sizeof(U);
+    const U* p = (const U*)a.p + r0 * a.ldp;
     int64_t lo = 0, hi = 0;
     int s = 0, k = 0;
     if (LOW == 1) {
@@ -380,7 +386,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
             else __builtin_amdgcn_s_waitcnt(0x0070 | (XI + WI - 1));
             __builtin_amdgcn_s_barrier();
             if (i + (THREE ? 2 : 1) < full) bring(free);
-            multiply(now, std::false_type{}, 0, 0);
+            multiply(T{}, now, std::false_type{}, 0, 0);
         };
         static_assert(XI + WI < 16, "a wait's low counter");
         if constexpr (THREE) {
@@ -399,22 +405,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     }
     for (int k0 = full * KB; k0 < a.K; k0 += KB) {
         if (k0 > full * KB) fetch(rest, x, a.ldx, w, ldw, k0, a.K);
-        apply(rest, std::false_type{}, 0, 0);
+        apply(T{}, rest, std::false_type{}, 0, 0);
     }
     if (LOW == 1) {
         for (bool waits = true; s < a.sg.S; waits = false, s = next_adapter(s + 1, &lo, &hi, &k)) {
             const int from = lo > r0 ? (int)(lo - r0) - wm : 0, to = hi < r1 ? (int)(hi - r0) - wm : TM;
-            for (int k0 = 0; k0 < a.R; k0 += KB) {
+            for (int k0 = 0; k0 < a.R; k0 += KU) {
                 if (!waits || k0 > 0) fetch(first, p, a.ldp, (const T*)a.low + k * a.low_stride, KN ? a.N : a.R, k0, a.R);
-                apply(first, std::true_type{}, from, to, a.R - k0);
+                apply(U{}, first, std::true_type{}, from, to, a.R - k0);
             }
         }
     }
     if (LOW == 2) add_adapters<T, KN, MR, NR>(a, r0 + wm, r1, n0 + wn, 0, 1, acc);
 
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
-    put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
-                        (wave < PUTS ? l0 : wave < 2 * PUTS ? l1 : l2) + wave % PUTS * put_scratch<T, NR>());
+    put_tile<T, Y, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
+                           (wave < PUTS ? l0 : wave < 2 * PUTS ? l1 : l2) + wave % PUTS * put_scratch<Y, NR>());
 }
 
 // ------------------------------------------------------------------------------------------
@@ -490,16 +496,17 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
     struct Frags {
         u32x4 x[MR], w[NR];
     };
-    auto read = [&](const char* xs, const char* ws, int h, Frags& f) {
+    auto read_as = [&](auto type, const char* xs, const char* ws, int h, Frags& f) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const int c = wn + 16 * n;
-            if constexpr (KN) f.w[n] = strided_fragment<T, TN>(ws, h, c);
+            if constexpr (KN) f.w[n] = strided_fragment<decltype(type), TN>(ws, h, c);
             else f.w[n] = *(const u32x4*)(ws + (c + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
         }
 #pragma unroll
         for (int m = 0; m < MR; ++m) f.x[m] = *(const u32x4*)(xs + (wm + 16 * m + l15) * 128 + (((4 * h + kk) ^ (l15 & 7)) << 4));
     };
+    auto read = [&](const char* xs, const char* ws, int h, Frags& f) { read_as(T{}, xs, ws, h, f); };
     // (a fragment of x meets its four of w and is done with: the next one can take its registers)
     auto multiply = [&](const Frags& f) {
 #pragma unroll
@@ -507,7 +514,9 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
 #pragma unroll
             for (int n = 0; n < NR; ++n) acc[n][m] = mma<T>(f.w[n], f.x[m], acc[n][m]);
     };
-    // rows from .. to - 1 of the wave's only
+    // an adapter's: rows from .. to - 1 of the wave's only
+    using U = Mid<T>;
+    constexpr int KU = 128 / (int)sizeof(U);
     auto multiply_some = [&](const Frags& f, int from, int to) {
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
@@ -517,13 +526,13 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
                 const bool in = 16 * m + l15 >= from && 16 * m + l15 < to;
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    const Acc d = mma<T>(f.w[n], f.x[m], acc[n][m]);
+                    const Acc d = mma<U>(f.w[n], f.x[m], acc[n][m]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[n][m][r] = in ? d[r] : acc[n][m][r];
                 }
             } else {
 #pragma unroll
-                for (int n = 0; n < NR; ++n) acc[n][m] = mma<T>(f.w[n], f.x[m], acc[n][m]);
+                for (int n = 0; n < NR; ++n) acc[n][m] = mma<U>(f.w[n], f.x[m], acc[n][m]);
             }
         }
     };
@@ -633,18 +642,20 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
         }
         __syncthreads();
     }
-    // one step through registers: what lies past klen (or, in a line of w, past N) is 0
-    auto step = [&](const T* x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen, bool some, int from, int to) {
+    // one step through registers, w as values of x's type: what lies past klen (or, in a line of w, past N) is 0
+    auto step = [&](auto x, int64_t ldx, const T* w, int64_t ldw, int k0, int klen, auto some, int from, int to) {
+        using V = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+        constexpr int E = Mat<V>::E, LINE = TN * (int)sizeof(V) / 16;
         u32x4 xr[4], wr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int q = tid + NT * i, row = q >> 3;
             xr[i] = load_piece(x + (int64_t)min(row, nrow - 1) * ldx, k0 + ((q ^ row) & 7) * E, klen);
             if (KN) {
-                const int k = q / LINE, c = (q % LINE ^ spread<T, TN>(k) * SZ) * E;
-                wr[i] = k0 + k < klen ? load_piece(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
+                const int k = q / LINE, c = (q % LINE ^ spread<V, TN>(k) * (int)sizeof(V)) * E;
+                wr[i] = k0 + k < klen ? load_as<V>(w + (int64_t)(k0 + k) * ldw, n0 + c, a.N) : u32x4{0, 0, 0, 0};
             } else {
-                wr[i] = load_piece(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
+                wr[i] = load_as<V>(w + (int64_t)min(n0 + row, a.N - 1) * ldw, k0 + ((q ^ row) & 7) * E, klen);
             }
         }
 #pragma unroll
@@ -655,17 +666,17 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
         __syncthreads();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (h && klen - k0 <= KB / 2) break;
+            if (h && klen - k0 <= 64 / (int)sizeof(V)) break;
             Frags f;
-            read(u0, u1, h, f);
-            if (some) multiply_some(f, from, to);
+            read_as(V{}, u0, u1, h, f);
+            if constexpr (decltype(some)::value) multiply_some(f, from, to);
             else multiply(f);
         }
         __syncthreads();
     };
-    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, false, 0, 0);
+    for (int k0 = full * KB; k0 < a.K; k0 += KB) step(x, a.ldx, w, ldw, k0, a.K, std::false_type{}, 0, 0);
     if (LOW == 1) {
-        const T* p = (const T*)a.p + r0 * a.ldp;
+        const U* p = (const U*)a.p + r0 * a.ldp;
         for (int s = max(0, wave_search(a.sg.S, r0, [&](int i) { return seg_off(a.sg, i); })); s < a.sg.S; ++s) {
             const int64_t lo = seg_off(a.sg, s), hi = seg_off(a.sg, s + 1);
             if (lo >= r1) break;
@@ -673,17 +684,17 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
             if (hi <= r0 || lo >= hi || k < 0) continue;
             const T* low = (const T*)a.low + k * a.low_stride;
             const int from = lo > r0 ? (int)(lo - r0) - wm : 0, to = hi < r1 ? (int)(hi - r0) - wm : TM;
-            for (int k0 = 0; k0 < a.R; k0 += KB) step(p, a.ldp, low, KN ? a.N : a.R, k0, a.R, true, from, to);
+            for (int k0 = 0; k0 < a.R; k0 += KU) step(p, a.ldp, low, KN ? a.N : a.R, k0, a.R, std::true_type{}, from, to);
         }
     }
     const typename M::Sum scale = LOW == 0 && a.scale ? (typename M::Sum)a.scale[slot] : (typename M::Sum)1;
-    put_tile<T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
-                        (wave < 4 ? u0 : u1) + wave % 4 * put_scratch<T, NR>());
+    put_tile<T, T, MR, NR>(a, r0 + wm, r1, n0 + wn, scale, a.bias ? (const T*)a.bias + (LOW ? 0 : slot * a.bias_stride) : nullptr, acc,
+                           (wave < 4 ? u0 : u1) + wave % 4 * put_scratch<T, NR>());
 }
 
 constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
-template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW>
+template <typename T, int TM, int TN, int WM, int WN, bool KN, int LOW, typename Y = T>
 static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     static_assert(TM == 1 << log2_of(TM), "tile heights");
     constexpr int KB = 128 / (int)sizeof(T), E = Mat<T>::E;
@@ -694,7 +705,7 @@ static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t ldw = KN ? a.N : a.K;
     int full = KN && a.N % E ? (a.K - 1) / KB : a.K / KB;
     if (a.ldx * TM * (int64_t)sizeof(T) >= (1ll << 31) || ldw * std::max(TN, KB) * (int64_t)sizeof(T) >= (1ll << 31)) full = 0;
-    LN_LAUNCH(ctx, name, (rows_tile<T, TM, TN, WM, WN, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(64 * WM * WN), 0, a,
+    LN_LAUNCH(ctx, name, (rows_tile<T, Y, TM, TN, WM, WN, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(64 * WM * WN), 0, a,
               (unsigned)tiles_n, log2_of(TM), full);
     return 0;
 }
@@ -714,13 +725,27 @@ template <typename T, bool KN, int MR, int LOW>
 static int launch_few(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t tiles_n = (a.N + 15) / 16, tiles_m = LOW == 0 ? a.sg.rows / (16 * MR) + a.sg.S : (a.sg.rows + 16 * MR - 1) / (16 * MR);
     LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
-    LN_LAUNCH(ctx, name, (rows_few<T, KN, MR, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_n, log2_of(16 * MR));
+    const dim3 grid((unsigned)(tiles_n * tiles_m));
+    if constexpr (LOW == 0 && !std::is_same<T, Mid<T>>::value)
+        if (a.mid) {
+            LN_LAUNCH(ctx, name, (rows_few<T, Mid<T>, KN, MR, LOW>), grid, dim3(512), 0, a, (unsigned)tiles_n, log2_of(16 * MR));
+            return 0;
+        }
+    LN_LAUNCH(ctx, name, (rows_few<T, T, KN, MR, LOW>), grid, dim3(512), 0, a, (unsigned)tiles_n, log2_of(16 * MR));
     return 0;
 }
 
 template <typename T, bool KN, int LOW>
 static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t cus = ctx->prop.multiProcessorCount, rows = a.sg.rows;
+    if constexpr (LOW == 0 && !std::is_same<T, Mid<T>>::value) {                      // a middle: narrow, in a type of its own
+        if (a.mid) {
+            if (a.N <= 16) return launch_tile<T, 64, 16, 4, 1, KN, LOW, Mid<T>>(ctx, a, name);
+            if (a.N <= 32) return launch_tile<T, 64, 32, 4, 1, KN, LOW, Mid<T>>(ctx, a, name);
+            if (a.N <= 48) return launch_tile<T, 64, 48, 4, 1, KN, LOW, Mid<T>>(ctx, a, name);
+            return launch_tile<T, 64, 64, 2, 2, KN, LOW, Mid<T>>(ctx, a, name);
+        }
+    }
     if constexpr (LOW != 2) {
         if (a.N <= 16) return launch_tile<T, 64, 16, 4, 1, KN, LOW>(ctx, a, name);
         if (a.N <= 32) return launch_tile<T, 64, 32, 4, 1, KN, LOW>(ctx, a, name);
@@ -764,7 +789,7 @@ static int rows_any(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 
 int transform_rows(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name) {
     if (a.sg.rows == 0 || a.sg.S == 0 || a.N == 0) return 0;
-    if (rows_narrow_ok(a)) return transform_rows_narrow(ctx, dtype, a, name);
+    if (rows_narrow_ok(a) && !(a.mid && transform_size(dtype) == 2)) return transform_rows_narrow(ctx, dtype, a, name);
     switch (dtype) {
         case LNASR_F64: return rows_any<double>(ctx, a, name);
         case LNASR_F32: return rows_any<float>(ctx, a, name);

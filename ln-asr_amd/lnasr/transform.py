@@ -34,7 +34,7 @@ def affine_grad(x, offsets, w, dy, slots=None, want=("x", "w", "bias"), out=None
 
 def projection(x, offsets, w, a, b, bias=None, scale=None, slots=None, out=None, *, ctx=None):
     """y[r] = w x[r] + bias + scale[k] b[k] (a[k] x[r]).  w [dout, din], bias [dout], a [G, rank, din], b [G, dout, rank], scale
-    [G] float64 (default 1); slot -1: no adapter.  The middle, scale a x, is held in the type of x."""
+    [G] float64 (default 1); slot -1: no adapter.  The middle, scale a x, is held in 64 bits for float64 and in 32 for the others."""
     return (ctx or default_ctx()).projection(x, offsets, w, a, b, bias, scale, slots, out)
 
 
