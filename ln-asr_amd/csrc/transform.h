@@ -274,7 +274,7 @@ struct SumArgs {
     int64_t group_step;         // 1; S: all segments as one group
     const int* ord;             // [S] the segments in the order of their groups, or null: the rows as they lie
     const int64_t* place;       // [S + 1] (with ord) places of the sorted segments' rows
-    const int64_t* rowmap;      // (with ord, if the segments are short) the row at each place
+    const int64_t* rowmap;      // (with ord, if the segments are short or the rows far apart) the row at each place
     const void *a, *b;
     void *out, *cols;
     int64_t lda, ldb;
@@ -323,8 +323,11 @@ bool sum_narrow_ok(const SumArgs& a);
 int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
 // out and cols from the sums of the spans of 2^ts rows
 int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const void* parts, const void* col_parts);
+// Row strides at which the rows of one step (128 bytes of k) pass the 31 bits of the LDS-DMA's offsets
+inline bool transform_far(int64_t ld) { return ld * 128 >= (1ll << 31); }
 // Sorts the segments by group (stable): group_off, ord, place, rowmap of a.  Without slots the rows are sorted as they lie.
-int transform_sort(lnasr_ctx* ctx, int dtype, SumArgs* a);
+// ld: the largest row stride of what will be summed.
+int transform_sort(lnasr_ctx* ctx, int dtype, int64_t ld, SumArgs* a);
 
 // Workspace `i` of the feature transforms with room for `bytes`
 int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out);

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void map_rows(Segments sg, const int* ord, con
 // Segments long enough for their rows to be taken run by run: four steps of 128 bytes' worth of rows
 static bool rows_together(const Segments& sg, int dtype) { return sg.rows / sg.S >= 4 * 128 / (int64_t)transform_size(dtype); }
 
-int transform_sort(lnasr_ctx* ctx, int dtype, SumArgs* a) {
+int transform_sort(lnasr_ctx* ctx, int dtype, int64_t ld, SumArgs* a) {
     const Segments& sg = a->sg;
     a->rowmap = a->place = nullptr;
     a->ord = nullptr;
@@ -141,7 +141,7 @@ int transform_sort(lnasr_ctx* ctx, int dtype, SumArgs* a) {
     int64_t* goff = place + sg.S + 1;
     int* ord0 = (int*)(goff + sg.G + 1);
     a->group_off = goff;
-    const bool mapped = sg.rows > 0 && !rows_together(sg, dtype);
+    const bool mapped = sg.rows > 0 && (!rows_together(sg, dtype) || transform_far(ld));
     if (mapped) a->rowmap = map;
     a->place = place;
     a->ord = ord0;
@@ -617,7 +617,7 @@ static int span_length(const SumArgs& a, int64_t tiles, int64_t want, size_t sum
 template <typename T, int TI, int TJ, int WI, int WJ, typename A = T, typename B = T>
 static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     using Sum = typename Mat<T>::Sum;
-    constexpr int KB = 128 / (int)sizeof(Wider<A, B>), HOLDS = std::min(8, (160 << 10) / (2 * sum_step<A, B, TI, TJ>()));
+    constexpr int HOLDS = std::min(8, (160 << 10) / (2 * sum_step<A, B, TI, TJ>()));
     const int64_t ti = (a.I + TI - 1) / TI, tj = (a.J + TJ - 1) / TJ, size = (int64_t)a.I * a.J + a.I;
     const int ts = span_length(a, ti * tj, (int64_t)HOLDS * ctx->prop.multiProcessorCount, sizeof(Sum));
     const int64_t spans = (a.sg.rows >> ts) + a.groups;
@@ -628,8 +628,9 @@ static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
     Sum* cp = (Sum*)parts + spans * a.I * a.J;
     const dim3 grid((unsigned)(spans * ti * tj)), block(64 * WI * WJ);
-    // (with rowmap the segments are short: rows_together)
-    const bool together = !a.rowmap && std::max(a.lda * (int64_t)sizeof(A), a.ldb * (int64_t)sizeof(B)) * KB < (1ll << 31);
+    // (through registers the rows are rowmap's, or lie as they are summed: transform_sort knows the strides)
+    const bool together = !a.rowmap && !transform_far(std::max(a.lda, a.ldb));
+    LN_REQUIRE(together || a.rowmap || !a.place, "%s: sorted rows without their map", name);
     if (together) LN_LAUNCH(ctx, name, (sum_tile<T, A, B, TI, TJ, WI, WJ, true>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
     else LN_LAUNCH(ctx, name, (sum_tile<T, A, B, TI, TJ, WI, WJ, false>), grid, block, 0, a, (unsigned)ti, (unsigned)tj, ts, (Sum*)parts, cp);
     return split ? join_t<T>(ctx, a, ts, parts, cp) : 0;
@@ -679,7 +680,7 @@ static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     if (a.J <= 32) return launch_sum<T, 128, 32, 4, 1>(ctx, a, name);
     if constexpr (sizeof(T) == 2) {
         if ((int64_t)(a.I / 256) * (a.J / 256) * std::max<int64_t>(a.groups, a.sg.rows >> 11) >= 128 && (!a.place || a.sg.rows / a.sg.S >= 512) &&
-            std::max(a.lda, a.ldb) * 128 < (1ll << 31))
+            !transform_far(std::max(a.lda, a.ldb)))
             return launch_sum_deep<T>(ctx, a, name);
         if (a.I > 64 && a.J > 64) return launch_sum<T, 128, 128, 2, 2>(ctx, a, name);
     }
