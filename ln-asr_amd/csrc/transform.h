@@ -191,6 +191,15 @@ __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// HIP takes fewer than 2^32 threads along x: beyond 2^31 a launch has rows of blocks, a few of them past the last (their spans are
+// empty).  block_id: a block's number, of block_count().
+inline dim3 transform_grid(int64_t blocks, int threads) {
+    const int64_t most = (1ll << 31) / threads, y = (blocks + most - 1) / most;
+    return dim3((unsigned)(y > 1 ? (blocks + y - 1) / y : blocks), (unsigned)(y > 1 ? y : 1));
+}
+__device__ __forceinline__ unsigned block_count() { return gridDim.x * gridDim.y; }
+__device__ __forceinline__ unsigned block_id() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Consecutive block numbers go to the eight dies (XCDs) in turn, each with an L2 of its own: give every die a run of
 // neighbouring tiles, so that the tiles that share a matrix or a span of rows share an L2.
 __device__ __forceinline__ unsigned die_order(unsigned id, unsigned total) {

@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kSortNT) void sort_segments(Segments sg, int passes
 
 // the row at each place of the sorted order
 __global__ __launch_bounds__(256) void map_rows(Segments sg, const int* ord, const int64_t* place, int64_t* rowmap) {
-    const int64_t q0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64, total = place[sg.S];
+    const int64_t q0 = ((int64_t)block_id() * 4 + (threadIdx.x >> 6)) * 64, total = place[sg.S];
     if (q0 >= total) return;
     int i = wave_search(sg.S, q0, [&](int j) { return place[j]; });
     if (i < 0) return;
@@ -148,7 +148,7 @@ int transform_sort(lnasr_ctx* ctx, int dtype, int64_t ld, SumArgs* a) {
     int passes = 1;
     while (passes < 4 && (sg.G >> (8 * passes)) > 0) ++passes;
     LN_LAUNCH(ctx, "sort_segments", sort_segments, dim3(1), dim3(kSortNT), 0, sg, passes, ord0, ord0 + sg.S, place, goff);
-    if (mapped) LN_LAUNCH(ctx, "map_rows", map_rows, dim3((unsigned)((sg.rows + 255) / 256)), dim3(256), 0, sg, ord0, place, map);
+    if (mapped) LN_LAUNCH(ctx, "map_rows", map_rows, transform_grid((sg.rows + 255) / 256, 256), dim3(256), 0, sg, ord0, place, map);
     return 0;
 }
 
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
     __shared__ __attribute__((aligned(1024))) char lds[2 * STEP];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wi = wave / WJ * (TI / WI), wj = wave % WJ * (TJ / WJ);
-    const unsigned tiles = tiles_i * tiles_j, id = die_order(blockIdx.x, gridDim.x);
+    const unsigned tiles = tiles_i * tiles_j, id = die_order(block_id(), block_count());
     const int i0 = (int)(id % tiles / tiles_j) * TI, j0 = (int)(id % tiles_j) * TJ;
     const int64_t t = id / tiles;
     auto brings_a = [&](int i) { return AN % NT == 0 || wave * 64 + NT * i < AN; };
@@ -372,9 +372,9 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wi = wave / 4 * 128, wj = wave % 4 * 64;
     // (not in die_order: neighbouring blocks are tiles of one span, spread over the dies so that all of them start with the longest)
-    const unsigned tiles = tiles_i * tiles_j, id = blockIdx.x;
+    const unsigned tiles = tiles_i * tiles_j, id = block_id();
     const int i0 = (int)(id % tiles / tiles_j) * TI, j0 = (int)(id % tiles_j) * TJ;
-    const unsigned spans = gridDim.x / tiles;
+    const unsigned spans = block_count() / tiles;
     const int64_t t = spans <= 64 ? longest_span(a, spans, id / tiles, ts) : id / tiles;
     int g, n;
     int64_t q0;
@@ -522,8 +522,8 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
 template <typename T>
 __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int ts, float* col_parts) {
     __shared__ float part[3][64][8];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)(blockIdx.x % tiles) * 512 + lane * 8;
-    const int64_t t = blockIdx.x / tiles;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)(block_id() % tiles) * 512 + lane * 8;
+    const int64_t t = block_id() / tiles;
     int g, n;
     int64_t q0;
     bool whole;
@@ -562,7 +562,8 @@ __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typen
         const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
         return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
     };
-    const int g = (int)(blockIdx.x / per);
+    const int g = (int)(block_id() / per);
+    if (g >= a.groups) return;
     const int64_t go = clamped(g), ge = clamped(g + 1), n = (ge - go + (1ll << ts) - 1) >> ts;
     if (n <= 1) return;
     const int64_t t = (go >> ts) + g, size = (int64_t)a.I * a.J;
@@ -578,7 +579,7 @@ __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typen
         }
         return (T)v;
     };
-    for (int64_t e = (int64_t)(blockIdx.x % per) * 256 + threadIdx.x; e < size + a.I; e += (int64_t)per * 256) {
+    for (int64_t e = (int64_t)(block_id() % per) * 256 + threadIdx.x; e < size + a.I; e += (int64_t)per * 256) {
         if (e < size) ((T*)a.out)[g * size + e] = total(parts + t * size + e, size);
         else if (a.cols) ((T*)a.cols)[g * a.I + e - size] = total(col_parts + t * a.I + e - size, a.I);
     }
@@ -588,7 +589,7 @@ template <typename T>
 static int join_t(lnasr_ctx* ctx, const SumArgs& a, int ts, const void* parts, const void* col_parts) {
     using Sum = typename Mat<T>::Sum;
     const int64_t size = (int64_t)a.I * a.J + a.I, per = std::min<int64_t>((size + 255) / 256, std::max<int64_t>(1, 8192 / a.groups));
-    LN_LAUNCH(ctx, "join_parts", (join_parts<T>), dim3((unsigned)(per * a.groups)), dim3(256), 0, a, ts, (const Sum*)parts,
+    LN_LAUNCH(ctx, "join_parts", (join_parts<T>), transform_grid(per * a.groups, 256), dim3(256), 0, a, ts, (const Sum*)parts,
               (const Sum*)col_parts, (unsigned)per);
     return 0;
 }
@@ -627,7 +628,7 @@ static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     const bool split = a.sg.rows > (1ll << ts);
     if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
     Sum* cp = (Sum*)parts + spans * a.I * a.J;
-    const dim3 grid((unsigned)(spans * ti * tj)), block(64 * WI * WJ);
+    const dim3 grid = transform_grid(spans * ti * tj, 64 * WI * WJ), block(64 * WI * WJ);
     // (through registers the rows are rowmap's, or lie as they are summed: transform_sort knows the strides)
     const bool together = !a.rowmap && !transform_far(std::max(a.lda, a.ldb));
     LN_REQUIRE(together || a.rowmap || !a.place, "%s: sorted rows without their map", name);
@@ -653,8 +654,8 @@ static int launch_sum_deep(lnasr_ctx* ctx, SumArgs a, const char* name) {
         const bool split = a.sg.rows > (1ll << ts);
         if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * 4, &parts));
         float* cp = (float*)parts + spans * a.I * a.J;
-        if (pass) LN_LAUNCH(ctx, "sum_cols", (sum_cols<T>), dim3((unsigned)(spans * tiles)), dim3(256), 0, a, (unsigned)tiles, ts, cp);
-        else LN_LAUNCH(ctx, name, (sum_deep<T>), dim3((unsigned)(spans * tiles)), dim3(512), 0, a, (unsigned)ti, (unsigned)tj, ts, (float*)parts);
+        if (pass) LN_LAUNCH(ctx, "sum_cols", (sum_cols<T>), transform_grid(spans * tiles, 256), dim3(256), 0, a, (unsigned)tiles, ts, cp);
+        else LN_LAUNCH(ctx, name, (sum_deep<T>), transform_grid(spans * tiles, 512), dim3(512), 0, a, (unsigned)ti, (unsigned)tj, ts, (float*)parts);
         if (split) LN_TRY(join_t<T>(ctx, a, ts, parts, cp));
     }
     return 0;

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, NF * HF <= 15 ? 3 : 1) void rows_narrow(RowsAr
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
     char* lds = lds_all + wave * wave_lds;
     int64_t r0, r1;
-    const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, die_order(blockIdx.x, gridDim.x), ts, &r0, &r1);
+    const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, die_order(block_id(), block_count()), ts, &r0, &r1);
     if (s < 0) return;
     const int slot = seg_slot(a.sg, s);
     if (slot < 0) return;
@@ -191,7 +191,7 @@ static int launch_narrow(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d segments are too many for one call", (long long)a.sg.rows, a.sg.S);
     // (a fragment's read may run 64 bytes past the last row, put_chunk's up to the end of its last kilobyte)
     const int wave_lds = std::max(16 * a.K * (int)sizeof(T) + 64, (16 * 16 * NF * (int)sizeof(T) + 1023) / 1024 * 1024);
-    LN_LAUNCH(ctx, name, (rows_narrow<T, NF, HF>), dim3((unsigned)spans), dim3(256), 4 * wave_lds, a, ts, wave_lds);
+    LN_LAUNCH(ctx, name, (rows_narrow<T, NF, HF>), transform_grid(spans, 256), dim3(256), 4 * wave_lds, a, ts, wave_lds);
     return 0;
 }
 
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
     const int I = a.I, J = a.J, a_bytes = R * I * SZ, b_bytes = R * J * SZ;
     char* as = lds_all + wave * wave_lds;
     char* bs = as + (a_bytes + 15) / 16 * 16;
-    const int64_t t = die_order(blockIdx.x, gridDim.x);
+    const int64_t t = die_order(block_id(), block_count());
     int g, n;
     int64_t q0;
     bool whole;
@@ -400,7 +400,7 @@ static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name)
     Sum* cp = (Sum*)parts + spans * a.I * a.J;
     const int wave_lds = (R * a.I * SZ + 15) / 16 * 16 + (R * a.J * SZ + 15) / 16 * 16;
     const int lds = std::max(4 * wave_lds, 16 * IF * 16 * JF * (int)sizeof(Sum));
-    LN_LAUNCH(ctx, name, (sum_narrow<T, IF, JF, HA, HB>), dim3((unsigned)spans), dim3(256), lds, a, ts, (Sum*)parts, cp, wave_lds);
+    LN_LAUNCH(ctx, name, (sum_narrow<T, IF, JF, HA, HB>), transform_grid(spans, 256), dim3(256), lds, a, ts, (Sum*)parts, cp, wave_lds);
     constexpr int dtype = SZ == 8 ? LNASR_F64 : SZ == 4 ? LNASR_F32 : std::is_same<T, _Float16>::value ? LNASR_F16 : LNASR_BF16;
     return split ? transform_join(ctx, a, dtype, ts, parts, cp) : 0;
 }

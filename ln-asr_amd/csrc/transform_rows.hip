@@ -132,16 +132,16 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
     __shared__ Acc part[WAVES - 1][MR][64];
     __shared__ __attribute__((aligned(16))) char scratch[put_scratch<Y, 1>()];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kk = lane >> 4;
-    const int c0 = (int)(blockIdx.x % tiles_n) * 16;
+    const int c0 = (int)(block_id() % tiles_n) * 16;
     int64_t r0, r1;
     int slot = 0;
     if (LOW == 0) {
-        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, blockIdx.x / tiles_n, ts, &r0, &r1);
+        const int s = find_span(a.sg.off, a.sg.S, a.sg.rows, block_id() / tiles_n, ts, &r0, &r1);
         if (s < 0) return;
         slot = seg_slot(a.sg, s);
         if (slot < 0) return;
     } else {
-        r0 = seg_off(a.sg, 0) + (int64_t)(blockIdx.x / tiles_n) * (16 * MR);
+        r0 = seg_off(a.sg, 0) + (int64_t)(block_id() / tiles_n) * (16 * MR);
         r1 = min(seg_off(a.sg, a.sg.S), r0 + 16 * MR);
         if (r0 >= r1) return;
     }
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
     static_assert((THREE ? 3 : 2) * PUTS >= WM * WN && PUTS > 0, "put_tile's rows");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, kk = lane >> 4;
     const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
-    const unsigned id = die_order(blockIdx.x, gridDim.x);
+    const unsigned id = die_order(block_id(), block_count());
     const int n0 = (int)(id % tiles_n) * TN;
     const int64_t t = id / tiles_n;
     auto brings_w = [&](int i) { return TN * 8 % NT == 0 || wave * 64 + NT * i < TN * 8; };
@@ -470,9 +470,10 @@ __global__ __launch_bounds__(512, 2) void rows_deep(RowsArgs a, unsigned tiles_m
     int64_t r0, r1;
     int slot = 0;
     if (LOW == 0 && a.sg.S <= 64) {
-        if (!exact_tile(a.sg, blockIdx.x, tiles_n, &tn, &slot, &r0, &r1)) return;
+        if (!exact_tile(a.sg, block_id(), tiles_n, &tn, &slot, &r0, &r1)) return;
     } else {
-        tile_order(die_order(blockIdx.x, gridDim.x), tiles_m, tiles_n, &tm, &tn);
+        if (block_id() >= tiles_m * tiles_n) return;
+        tile_order(die_order(block_id(), tiles_m * tiles_n), tiles_m, tiles_n, &tm, &tn);
     }
     const int n0 = (int)tn * TN;
     if (LOW == 0 && a.sg.S > 64) {
@@ -705,7 +706,7 @@ static int launch_tile(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t ldw = KN ? a.N : a.K;
     int full = KN && a.N % E ? (a.K - 1) / KB : a.K / KB;
     if (a.ldx * TM * (int64_t)sizeof(T) >= (1ll << 31) || ldw * std::max(TN, KB) * (int64_t)sizeof(T) >= (1ll << 31)) full = 0;
-    LN_LAUNCH(ctx, name, (rows_tile<T, Y, TM, TN, WM, WN, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(64 * WM * WN), 0, a,
+    LN_LAUNCH(ctx, name, (rows_tile<T, Y, TM, TN, WM, WN, KN, LOW>), transform_grid(tiles_n * tiles_m, 64 * WM * WN), dim3(64 * WM * WN), 0, a,
               (unsigned)tiles_n, log2_of(TM), full);
     return 0;
 }
@@ -717,7 +718,7 @@ static int launch_deep(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
                (long long)a.sg.rows, a.N);
     int full = KN && a.N % 8 ? (a.K - 1) / 64 : a.K / 64;                             // as in launch_tile
     if (a.ldx * 512 >= (1ll << 31) || (KN ? a.N : a.K) * 512ll >= (1ll << 31)) full = 0;
-    LN_LAUNCH(ctx, name, (rows_deep<T, KN, LOW>), dim3((unsigned)(tiles_n * tiles_m)), dim3(512), 0, a, (unsigned)tiles_m, (unsigned)tiles_n, full);
+    LN_LAUNCH(ctx, name, (rows_deep<T, KN, LOW>), transform_grid(tiles_n * tiles_m, 512), dim3(512), 0, a, (unsigned)tiles_m, (unsigned)tiles_n, full);
     return 0;
 }
 
@@ -725,7 +726,7 @@ template <typename T, bool KN, int MR, int LOW>
 static int launch_few(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t tiles_n = (a.N + 15) / 16, tiles_m = LOW == 0 ? a.sg.rows / (16 * MR) + a.sg.S : (a.sg.rows + 16 * MR - 1) / (16 * MR);
     LN_REQUIRE(tiles_n * tiles_m < (1ll << 31), "%lld rows x %d results are too many for one call", (long long)a.sg.rows, a.N);
-    const dim3 grid((unsigned)(tiles_n * tiles_m));
+    const dim3 grid = transform_grid(tiles_n * tiles_m, 512);
     if constexpr (LOW == 0 && !std::is_same<T, Mid<T>>::value)
         if (a.mid) {
             LN_LAUNCH(ctx, name, (rows_few<T, Mid<T>, KN, MR, LOW>), grid, dim3(512), 0, a, (unsigned)tiles_n, log2_of(16 * MR));

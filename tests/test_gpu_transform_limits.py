@@ -46,3 +46,40 @@ def test_matrix_gradients_of_rows_far_apart(ctx, kind):
     for k, v in (("a", da), ("b", db), ("w", dws)):
         ref.check(v.to_host(), want[k], err[k], k)
     room.free()
+
+
+def check_columns(kind, x, got, w, slots, what):
+    """got[r] = w[slots[r]] x[r] for one-row segments, as _transform_ref has it, some rows at a time"""
+    for at in range(0, len(x), 8192):
+        r = slice(at, min(at + 8192, len(x)))
+        n = r.stop - at
+        ref.check(got[r], *ref.affine(kind, x[r], np.arange(n + 1), w, None, slots[r], np.zeros((n, w.shape[1]))), what)
+
+
+@pytest.mark.parametrize("kind", ["float32", "float16"])
+def test_more_work_items_than_one_launch_takes(ctx, kind):
+    """66,000 one-row segments of 2048 results: 9 million blocks of 512 threads, past 2^32 items."""
+    rng = np.random.default_rng(2)
+    F, K, N, G = 66000, 12, 2048, 3
+    sl = rng.integers(0, G, F).astype(np.int32)
+    off = np.arange(F + 1, dtype=np.int64)
+    x, w = rng.standard_normal((F, K)).astype(kind), rng.standard_normal((G, N, K)).astype(kind)
+    y = ctx.affine(ctx.to_device(x), off, ctx.to_device(w), slots=sl).to_host()
+    check_columns(kind, x, y, w, sl, "y")
+    wt = np.ascontiguousarray(w.transpose(0, 2, 1))                       # [G, K, N]: dx = wt^T dy has the same values
+    g = ctx.affine_grad(ctx.to_device(np.ones((F, N), kind)), off, ctx.to_device(wt), ctx.to_device(x), sl, want=("x",))["x"].to_host()
+    check_columns(kind, x, g, w, sl, "dx")
+
+
+def test_more_groups_than_one_launch_has_blocks(ctx):
+    """17 million groups of one value: past 2^32 items in the gradients and in the join of their sums."""
+    G = 17_000_000
+    x = (np.arange(G) % 7 - 3).astype(np.float32).reshape(G, 1)
+    dy = (np.arange(G) % 5 - 2).astype(np.float32).reshape(G, 1)
+    off = np.arange(G + 1, dtype=np.int64)
+    off[1:1999] = 1999                                                    # a long group, and some of none
+    want = (x * dy).astype(np.float64).ravel()
+    want[0] = want[:1999].sum()
+    want[1:1999] = 0
+    g = ctx.affine_grad(x, off, np.zeros((G, 1, 1), np.float32), dy, want=("w",))["w"].ravel()
+    assert np.array_equal(g, want)
