@@ -182,6 +182,23 @@ __global__ __launch_bounds__(256, NF * HF <= 15 ? 3 : 1) void rows_narrow(RowsAr
     }
 }
 
+// LDS of a wave: fragments read 64 HF bytes from the start of each of the 16 rows, past the last one's end where K is not as wide;
+// put_chunk reads to the end of its last kilobyte
+constexpr int narrow_lds(int size, int NF, int HF, int K) {
+    const int in = (15 * K * size + 64 * HF + 15) / 16 * 16, out = (16 * 16 * NF * size + 1023) / 1024 * 1024;
+    return in > out ? in : out;
+}
+// every K up to 64 HF bytes: rows and what is read behind the last of them lie in the wave's own LDS
+constexpr bool narrow_lds_holds(int size, int NF, int HF) {
+    for (int K = 1; K * size <= 64 * HF; ++K)
+        for (int h = 0; h < HF; ++h)
+            for (int kk = 0; kk < 4; ++kk) {
+                const int end = (15 * K + (4 * h + kk) * (16 / size)) * size + 16, lds = narrow_lds(size, NF, HF, K);
+                if (end > lds || 16 * K * size > lds || 16 * 16 * NF * size > lds || lds % 16) return false;
+            }
+    return true;
+}
+
 template <typename T, int NF, int HF>
 static int launch_narrow(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     // spans: long ones spread the cost of fetching the matrix, but every CU should have a few blocks
@@ -189,8 +206,8 @@ static int launch_narrow(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     while (ts < 10 && (a.sg.rows >> ts) > 8 * ctx->prop.multiProcessorCount) ++ts;
     const int64_t spans = (a.sg.rows >> ts) + a.sg.S;
     LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d segments are too many for one call", (long long)a.sg.rows, a.sg.S);
-    // (a fragment's read may run 64 bytes past the last row, put_chunk's up to the end of its last kilobyte)
-    const int wave_lds = std::max(16 * a.K * (int)sizeof(T) + 64, (16 * 16 * NF * (int)sizeof(T) + 1023) / 1024 * 1024);
+    static_assert(narrow_lds_holds((int)sizeof(T), NF, HF), "fragments of rows_narrow");
+    const int wave_lds = narrow_lds((int)sizeof(T), NF, HF, a.K);
     LN_LAUNCH(ctx, name, (rows_narrow<T, NF, HF>), transform_grid(spans, 256), dim3(256), 4 * wave_lds, a, ts, wave_lds);
     return 0;
 }

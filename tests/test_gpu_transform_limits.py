@@ -83,3 +83,17 @@ def test_more_groups_than_one_launch_has_blocks(ctx):
     want[1:1999] = 0
     g = ctx.affine_grad(x, off, np.zeros((G, 1, 1), np.float32), dy, want=("w",))["w"].ravel()
     assert np.array_equal(g, want)
+
+
+@pytest.mark.parametrize("kind", ["float64", "float32", "float16"])
+@pytest.mark.parametrize("K", [1, 9, 15, 16, 17, 33, 40, 41, 48, 49, 63, 64])
+def test_narrow_rows_of_every_fragment_width(ctx, kind, K):
+    """Rows whose fragments are read past the row's end, few results and many: all of it in the wave's own LDS (the build checks that
+    for every width), and none of it in a result."""
+    for N in (1, 16, 17, 64):
+        d = ref.make(3, (333, K, N, 5, 3, 2))
+        d = {k: v if k in ("offsets", "slots", "scale") else v.astype(kind) for k, v in d.items()}
+        y = ctx.affine(d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], out=d["y0"].copy())
+        ref.check(y, *ref.affine(kind, d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], d["y0"]), "y")
+        y = ctx.affine(d["x"], d["offsets"], d["w3"], None, d["slots"], out=d["y0"].copy())
+        ref.check(y, *ref.affine(kind, d["x"], d["offsets"], d["w3"], None, d["slots"], d["y0"]), "y without bias")
