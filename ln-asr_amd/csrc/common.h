@@ -43,6 +43,8 @@ int fail(int code, const char* fmt, ...);
 // First statement of every C-ABI entry point that takes a context: the HIP "current device" is per thread, so a
 // call from a thread other than the one that created the context (or after another library moved the thread's device) would
 // otherwise allocate workspaces and launch on device 0.  hipSetDevice is a cheap thread-local store.
+// (The feature transforms' entry points, which threads may share, set the device alone: they change the context only under its lock,
+// and have no use for the count of calls.)
 #define LN_ENTER(ctx)                                          \
     do {                                                       \
         if (ctx) {                                             \

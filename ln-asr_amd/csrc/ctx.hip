@@ -341,7 +341,7 @@ int lnasr_sync(lnasr_ctx* ctx) {
 int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own) {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
-    LN_ENTER(ctx);
+    LN_HIP(hipSetDevice(ctx->device));
     const std::lock_guard<std::mutex> lock(ctx->tr_mutex);
     const hipStream_t to = own ? ctx->own_stream : (hipStream_t)stream;
     if (to == ctx->stream) return 0;

@@ -187,7 +187,7 @@ int lnasr_affine(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int din
                  int S, const void* w, const void* bias, int G, int dout, void* y, int64_t ldy) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
-    LN_ENTER(ctx);
+    LN_HIP(hipSetDevice(ctx->device));
     LN_TRY(check_type(dtype));
     LN_REQUIRE(din > 0 && dout > 0 && din <= kMaxWidth && dout <= kMaxWidth, "widths %d -> %d", din, dout);
     LN_TRY(check_matrix("x", rows, din, ldx));
@@ -224,7 +224,7 @@ int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, in
                       void* dw, void* dbias) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
-    LN_ENTER(ctx);
+    LN_HIP(hipSetDevice(ctx->device));
     LN_TRY(check_type(dtype));
     LN_REQUIRE(din > 0 && dout > 0 && din <= kMaxWidth && dout <= kMaxWidth, "widths %d -> %d", din, dout);
     LN_TRY(check_matrix("x", rows, din, dw ? ldx : din));
@@ -287,7 +287,7 @@ int lnasr_projection(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, int
                      const double* scale, int G, int rank, void* y, int64_t ldy) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
-    LN_ENTER(ctx);
+    LN_HIP(hipSetDevice(ctx->device));
     LN_TRY(check_type(dtype));
     LN_REQUIRE(din > 0 && dout > 0 && din <= kMaxWidth && dout <= kMaxWidth, "widths %d -> %d", din, dout);
     LN_REQUIRE(rank > 0 && rank <= kMaxWidth, "rank %d", rank);
@@ -345,7 +345,7 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
                           int rank, const void* dy, int64_t lddy, void* dx, int64_t lddx, void* da, void* db, void* dw, void* dbias) try {
     LN_REQUIRE(ctx, "null ctx");
     DeviceScope scope(ctx);
-    LN_ENTER(ctx);
+    LN_HIP(hipSetDevice(ctx->device));
     LN_TRY(check_type(dtype));
     LN_REQUIRE(din > 0 && dout > 0 && din <= kMaxWidth && dout <= kMaxWidth, "widths %d -> %d", din, dout);
     LN_REQUIRE(rank > 0 && rank <= kMaxWidth, "rank %d", rank);
