@@ -21,8 +21,12 @@ extern "C" {
  * of theirs.  The stream has to live until the context is sent elsewhere or destroyed; refused while either stream is being
  * captured.  A call of the feature transforms on device memory may be captured into a graph once it has run (its workspaces
  * then exist and stay, after the context is destroyed too); it is left out of the profile.  Graphs of one context share its
- * workspaces: a replay, other replays and the context's own calls run one after the other, as on one stream. */
+ * workspaces: a replay, other replays and the context's own calls run one after the other, as on one stream.
+ * The stream belongs to the context, not to the thread that chose it: threads with streams of their own take a context each, or
+ * choose and call under a lock of theirs (as the Python layer does). */
 int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own);
+/* 1: the context's stream is being captured (or is the default stream while another one is), 0: it is not; negative: an error */
+int lnasr_ctx_capturing(lnasr_ctx* ctx);
 
 /*
  * Between the features (lnasr_mfcc) and the bank (lnasr_decode ...): an affine transform per speaker or class, and a projection
@@ -35,7 +39,8 @@ int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own);
  *   Arrays may be host or device memory as everywhere; host offsets and slots are checked, device ones are brought into range
  * (values out of order then give numbers without meaning, no access out of bounds).  An output may not overlap an input or
  * another output, from its first element to its last (columns of one buffer beside each other do).  With device arrays the call
- * only enqueues.  Threads may share a context: their calls run one after the other. */
+ * only enqueues.  Threads may share a context for the calls below: they run one after the other (the context's other entry points
+ *   belong to one thread at a time). */
 
 /* y[r] = W[k] x[r] + bias[k], k the group of row r: x [rows, din], w [G, dout, din], bias [G, dout] or NULL, y [rows, dout].
  * A host slot outside [0, G) is refused, rows of such a device slot are left as they were. */

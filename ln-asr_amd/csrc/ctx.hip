@@ -362,6 +362,19 @@ int lnasr_ctx_use_stream(lnasr_ctx* ctx, void* stream, int own) {
     return 0;
 }
 
+int lnasr_ctx_capturing(lnasr_ctx* ctx) {
+    LN_REQUIRE(ctx, "null ctx");
+    DeviceScope scope(ctx);
+    LN_HIP(hipSetDevice(ctx->device));
+    const std::lock_guard<std::mutex> lock(ctx->tr_mutex);
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &st) != hipSuccess) {
+        (void)hipGetLastError();                          // (the default stream while another stream is captured)
+        return 1;
+    }
+    return st != hipStreamCaptureStatusNone ? 1 : 0;
+}
+
 int lnasr_device_sync(lnasr_ctx* ctx) {
     LN_ENTER(ctx);
     LN_REQUIRE(ctx, "null ctx");

@@ -97,6 +97,7 @@ SIGNATURES = {
 # the entry points of include/lnasr_transform.h
 TRANSFORM_SIGNATURES = {
     "lnasr_ctx_use_stream": [_vp, _vp, _i],
+    "lnasr_ctx_capturing": [_vp],
     "lnasr_affine": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i64],
     "lnasr_affine_grad": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _vp],
     "lnasr_projection": [_vp, _i, _vp, _i64, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i64],
@@ -287,11 +288,12 @@ _KINDS = {}
 class _Arg:
     """An array handed to a feature transform: a numpy array (or what becomes one), a DeviceArray, or a tensor of another library
     on the GPU (an object with data_ptr(), shape, dtype, stride() and is_cuda, as torch's).  `obj` keeps it alive."""
-    __slots__ = ("ptr", "shape", "ld", "kind", "obj", "loose")
+    __slots__ = ("ptr", "shape", "ld", "kind", "obj", "loose", "tensor")
 
     def __init__(self, ctx, x, name, ndim, like=None, out=False):
         """like: the _Arg whose type this one must have (None: any of the four; a kind: exactly that)."""
-        self.loose = False            # its memory is used in the order of another stream than the context's
+        self.loose = False            # its memory is used in the order of another context's stream
+        self.tensor = False           # ... of a stream of another library
         if isinstance(x, DeviceArray):
             self.loose = x.ctx is not ctx
             if not x.ptr or x.ctx.device != ctx.device:
@@ -306,7 +308,7 @@ class _Arg:
             if kind is None:
                 kind = _KINDS[dtype] = str(dtype).replace("torch.", "")
             self.obj, self.ptr, self.shape, self.kind, self.ld = x, x.data_ptr(), tuple(x.shape), kind, 1
-            self.loose = getattr(ctx, "_stream", None) is None
+            self.tensor = True
             if not ctx._tensors_checked:
                 # pointers of another copy of the HIP runtime mean nothing to this one
                 if self.ptr and lib().lnasr_debug_require_device_ptr(self.ptr) != 0:
@@ -392,6 +394,8 @@ class Context:
         self._model_fp = None         # fingerprint of the parameters the device holds (see upload_*)
         self._tensors_checked = False # a tensor of another library was seen and its memory is known to this HIP runtime
         self._stream = None           # the caller's stream this context works on (None: its own)
+        self._choice = threading.local()   # .stream: the stream the thread chose for its tensors
+        self._order = threading.RLock()    # choosing a stream and the call that goes there are one step
 
     def close(self):
         if self.handle:
@@ -411,9 +415,18 @@ class Context:
     def use_stream(self, stream=None):
         """Send this context's further calls to `stream` (a hipStream_t as an int, or an object with `cuda_stream`, as torch's
         streams have), behind what it was given so far; None: back to its own.  Tensors of another library are produced on a
-        stream of that library: choose that stream here (lnasr_ctx_use_stream)."""
+        stream of that library: choose that stream here (lnasr_ctx_use_stream).
+
+        Each thread chooses for its own tensors: where threads share a context, the feature transforms of a thread go to the
+        stream it chose, whatever another has chosen since.  A thread that has chosen none waits for the device before and after
+        such a call."""
         if stream is not None and not isinstance(stream, int):
             stream = stream.cuda_stream
+        with self._order:
+            self._go(stream)
+            self._choice.stream = stream
+
+    def _go(self, stream):
         if stream != self._stream:
             check(lib().lnasr_ctx_use_stream(self.handle, stream, 1 if stream is None else 0))
             self._stream = stream
@@ -928,12 +941,22 @@ class Context:
     # -- feature transforms ------------------------------------------------------------------------
     # (lnasr/transform.py has what the arguments mean)
     def _call(self, fn, arrays, *args):
-        loose = any(a.loose for a in arrays if a)
-        if loose:                     # (a caller that wants no waits chooses the stream: use_stream)
-            self.device_sync()
-        check(fn(self.handle, *args))
-        if loose:
-            self.sync()
+        with self._order:
+            loose = any(a.loose for a in arrays if a)
+            if any(a.tensor for a in arrays if a):
+                stream = getattr(self._choice, "stream", None)
+                if stream is not None:
+                    self._go(stream)
+                elif not loose:       # (a thread of the library's own may call while another captures: it cannot wait)
+                    rc = lib().lnasr_ctx_capturing(self.handle)
+                    if rc < 0:
+                        check(rc)
+                    loose = rc == 0
+            if loose:                 # (a caller that wants no waits chooses the stream: use_stream)
+                self.device_sync()
+            check(fn(self.handle, *args))
+            if loose:
+                self.sync()
 
     def _rows(self, x, offsets, slots, groups):
         """(_Args of x, offsets, slots, number of segments, whether every row is known to belong to a segment)."""

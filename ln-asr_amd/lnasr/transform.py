@@ -11,8 +11,8 @@ has to have data_ptr(), shape, dtype, stride()); what comes back is of the same 
 type: float64, float32, float16 or (tensors) bfloat16.  Sums are held in 64 bits for float64 and in 32 for the others.  Rows may
 be strided (a slice of columns); matrices are contiguous.  numpy arrays are converted to the type of x.  Results may be written
 into `out`, which must not overlap an input (nor lie beside it in the columns of one buffer).  With GPU tensors, choose their
-stream first (`ctx.use_stream`) and import their library before lnasr; where no stream was chosen, and for `DeviceArray`s of
-another context, a call waits for the device before it begins and until it is done.
+stream first (`ctx.use_stream`, in each thread that calls) and import their library before lnasr; in a thread that chose none, and
+for `DeviceArray`s of another context, a call waits for the device before it begins and until it is done.
 """
 import numpy as np
 
