@@ -5,6 +5,7 @@ every compute entry point raises.  Build the library with `python ln-asr_amd/bui
 """
 import ctypes as C
 import os
+import sys
 import threading
 
 import numpy as np
@@ -285,6 +286,12 @@ _CODES = {"float64": F64, "float32": F32, "float16": F16, "bfloat16": BF16}
 _KINDS = {}
 
 
+def _recording():
+    """Does torch, if somebody imported it, record what happens to tensors?"""
+    torch = sys.modules.get("torch")
+    return torch is None or torch.is_grad_enabled()
+
+
 class _Arg:
     """An array handed to a feature transform: a numpy array (or what becomes one), a DeviceArray, or a tensor of another library
     on the GPU (an object with data_ptr(), shape, dtype, stride() and is_cuda, as torch's).  `obj` keeps it alive."""
@@ -309,6 +316,10 @@ class _Arg:
                 kind = _KINDS[dtype] = str(dtype).replace("torch.", "")
             self.obj, self.ptr, self.shape, self.kind, self.ld = x, x.data_ptr(), tuple(x.shape), kind, 1
             self.tensor = True
+            if getattr(x, "requires_grad", False) and _recording():
+                # (it would come back without a graph, and its gradient would be lost without a word)
+                raise LnasrError("%s requires a gradient, which this call does not record: detach() it, or call under torch.no_grad() "
+                                 "or from the two halves of a torch.autograd.Function" % name)
             if not ctx._tensors_checked:
                 # pointers of another copy of the HIP runtime mean nothing to this one
                 if self.ptr and lib().lnasr_debug_require_device_ptr(self.ptr) != 0:

@@ -12,7 +12,9 @@ type: float64, float32, float16 or (tensors) bfloat16.  Sums are held in 64 bits
 be strided (a slice of columns); matrices are contiguous.  numpy arrays are converted to the type of x.  Results may be written
 into `out`, which must not overlap an input (nor lie beside it in the columns of one buffer).  With GPU tensors, choose their
 stream first (`ctx.use_stream`, in each thread that calls) and import their library before lnasr; in a thread that chose none, and
-for `DeviceArray`s of another context, a call waits for the device before it begins and until it is done.
+for `DeviceArray`s of another context, a call waits for the device before it begins and until it is done.  Calls are not recorded
+by torch's autograd: a tensor that requires a gradient is refused unless recording is off, as under `torch.no_grad()` and in the
+forward and backward of a `torch.autograd.Function`, where these functions and their gradients belong.
 """
 import numpy as np
 

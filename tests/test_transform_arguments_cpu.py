@@ -1,0 +1,33 @@
+"""CPU: arguments of the feature transforms that are refused, or taken for what they are, before the library is called."""
+import sys
+import types
+
+import numpy as np
+import pytest
+
+
+class _Ctx:
+    device = 0
+    _tensors_checked = True
+
+
+class _Tensor:
+    is_cuda, dtype, shape, requires_grad = True, "torch.float32", (4, 3), True
+    data_ptr = lambda self: 4096
+    get_device = lambda self: 0
+    stride = lambda self: (3, 1)
+    is_contiguous = lambda self: True
+
+
+def test_a_tensor_that_requires_a_gradient_is_refused_where_that_is_recorded(monkeypatch):
+    from lnasr import _ffi
+    arg = lambda: _ffi._Arg(_Ctx, _Tensor(), "w", 2)
+    on = types.SimpleNamespace(is_grad_enabled=lambda: True)
+    monkeypatch.setitem(sys.modules, "torch", on)
+    with pytest.raises(_ffi.LnasrError, match="w requires a gradient"):
+        arg()
+    on.is_grad_enabled = lambda: False                             # no_grad(), or inside a Function
+    assert arg().kind == "float32"
+    monkeypatch.setattr(_Tensor, "requires_grad", False)
+    on.is_grad_enabled = lambda: True
+    assert arg().kind == "float32"
