@@ -290,9 +290,18 @@ struct SumArgs {
     int groups, I, J;
     bool mid_a, mid_b;
 };
-// Span t of 2^ts places of the sorted rows: its group, first place and rows; false: nothing to do.  (A group without rows has one
-// span without rows, to be written as zeros.)
-__device__ __forceinline__ bool sum_span(const SumArgs& a, int64_t t, int ts, int* group, int64_t* q0, int* n, bool* whole) {
+// Where the sums of a group of several spans lie: place sum_place of span k = 0, 1, .. of a group that begins at row go, of
+// sum_places.  With few groups the spans' numbers; else 2 floor(go / 2^ts) + k, whatever the number of groups: a group of L > 2^ts
+// rows has ceil(L / 2^ts) <= floor(L / 2^ts) + 1 <= 2 floor(L / 2^ts) spans, and the next one begins floor(L / 2^ts) or more further
+// on.  (Groups of one span write no sums: 128 groups of 4096 x 4096, one of them split, took 8.6 GB.)
+__host__ __device__ inline bool sum_numbered(int64_t rows, int groups, int ts) { return groups <= rows >> ts; }
+inline int64_t sum_places(const SumArgs& a, int ts) { return (a.sg.rows >> ts) + (sum_numbered(a.sg.rows, a.groups, ts) ? a.groups : a.sg.rows >> ts); }
+__device__ __forceinline__ int64_t sum_place(const SumArgs& a, int group, int64_t go, int64_t k, int ts) {
+    return (go >> ts) + k + (sum_numbered(a.sg.rows, a.groups, ts) ? group : go >> ts);
+}
+// Span t of 2^ts places of the sorted rows: its group, first place and rows, and where its sums go; false: nothing to do.  (A group
+// without rows has one span without rows, to be written as zeros.)
+__device__ __forceinline__ bool sum_span(const SumArgs& a, int64_t t, int ts, int* group, int64_t* q0, int* n, bool* whole, int64_t* place) {
     auto clamped = [&](int g) {
         const int64_t o = a.sg.S ? a.group_off[g * a.group_step] : 0;
         return o < 0 ? (int64_t)0 : o > a.sg.rows ? a.sg.rows : o;
@@ -305,6 +314,7 @@ __device__ __forceinline__ bool sum_span(const SumArgs& a, int64_t t, int ts, in
     if (span > 0 && *q0 >= ge) return false;
     *n = (int)min(ge - *q0, (int64_t)1 << ts);
     *whole = go + (1ll << ts) >= ge;
+    *place = sum_place(a, g, go, span, ts);
     return true;
 }
 // The rows that lie together from place q of the sorted rows on, at most up to place end: calls each(first row, rows) run by run

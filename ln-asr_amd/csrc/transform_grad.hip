@@ -209,9 +209,9 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
     auto brings_a = [&](int i) { return AN % NT == 0 || wave * 64 + NT * i < AN; };
     auto brings_b = [&](int i) { return BN % NT == 0 || wave * 64 + NT * i < BN; };
     int g, n;
-    int64_t q0;
+    int64_t q0, at;
     bool whole;
-    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole, &at)) return;
 
     Acc acc[IR][JR], col[IR];
 #pragma unroll
@@ -341,11 +341,11 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void sum_tile(SumArgs a, unsigned 
                 const int jj = j0 + wj + 16 * j + l15;
                 if (jj >= a.J) continue;
                 if (whole) ((T*)a.out)[((int64_t)g * a.I + ii) * a.J + jj] = (T)acc[i][j][r];
-                else parts[(t * a.I + ii) * a.J + jj] = acc[i][j][r];
+                else parts[(at * a.I + ii) * a.J + jj] = acc[i][j][r];
             }
             if (want_col && l15 == 0) {
                 if (whole) ((T*)a.cols)[(int64_t)g * a.I + ii] = (T)col[i][r];
-                else col_parts[t * a.I + ii] = col[i][r];
+                else col_parts[at * a.I + ii] = col[i][r];
             }
         }
 }
@@ -377,9 +377,9 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
     const unsigned spans = block_count() / tiles;
     const int64_t t = spans <= 64 ? longest_span(a, spans, id / tiles, ts) : id / tiles;
     int g, n;
-    int64_t q0;
+    int64_t q0, at;
     bool whole;
-    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole, &at)) return;
 
     Acc acc[IR][JR];
 #pragma unroll
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
                 const int jj = j0 + wj + 16 * j + l15;
                 if (jj >= a.J) continue;
                 if (whole) ((T*)a.out)[((int64_t)g * a.I + ii) * a.J + jj] = (T)acc[i][j][r];
-                else parts[(t * a.I + ii) * a.J + jj] = acc[i][j][r];
+                else parts[(at * a.I + ii) * a.J + jj] = acc[i][j][r];
             }
         }
 }
@@ -525,9 +525,9 @@ __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int t
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)(block_id() % tiles) * 512 + lane * 8;
     const int64_t t = block_id() / tiles;
     int g, n;
-    int64_t q0;
+    int64_t q0, at;
     bool whole;
-    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole, &at)) return;
     float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     each_run(a, q0, q0 + n, [&](int64_t row0, int rows) {
 #pragma unroll 8
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int t
         const float v = sum[j] + part[0][lane][j] + part[1][lane][j] + part[2][lane][j];
         if (c + j >= a.I) continue;
         if (whole) ((T*)a.cols)[(int64_t)g * a.I + c + j] = (T)v;
-        else col_parts[t * a.I + c + j] = v;
+        else col_parts[at * a.I + c + j] = v;
     }
 }
 
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typen
     if (g >= a.groups) return;
     const int64_t go = clamped(g), ge = clamped(g + 1), n = (ge - go + (1ll << ts) - 1) >> ts;
     if (n <= 1) return;
-    const int64_t t = (go >> ts) + g, size = (int64_t)a.I * a.J;
+    const int64_t at = sum_place(a, g, go, 0, ts), size = (int64_t)a.I * a.J;
     // n values `step` apart, in their order, eight on their way at a time
     auto total = [&](const Sum* from, int64_t step) {
         Sum v = 0;
@@ -580,8 +580,8 @@ __global__ __launch_bounds__(256) void join_parts(SumArgs a, int ts, const typen
         return (T)v;
     };
     for (int64_t e = (int64_t)(block_id() % per) * 256 + threadIdx.x; e < size + a.I; e += (int64_t)per * 256) {
-        if (e < size) ((T*)a.out)[g * size + e] = total(parts + t * size + e, size);
-        else if (a.cols) ((T*)a.cols)[g * a.I + e - size] = total(col_parts + t * a.I + e - size, a.I);
+        if (e < size) ((T*)a.out)[g * size + e] = total(parts + at * size + e, size);
+        else if (a.cols) ((T*)a.cols)[g * a.I + e - size] = total(col_parts + at * a.I + e - size, a.I);
     }
 }
 
@@ -605,7 +605,7 @@ int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const vo
 
 // Length of a span, as a power of two: a span's sums are written and read once more (8 or 16 bytes each) beside its 2 x 2^ts products
 // of each, so long ones, but no fewer blocks than the CUs hold at a time (`want`).  Where the groups give that many by themselves,
-// only one far over the mean is cut.  Never more sums than 256 MB beside one for each group.
+// only one far over the mean is cut.  Never more than 512 MB of sums (sum_places).
 static int span_length(const SumArgs& a, int64_t tiles, int64_t want, size_t sum_size) {
     const int64_t size = (int64_t)a.I * a.J + a.I;
     int ts = 8;
@@ -626,8 +626,9 @@ static int launch_sum(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
                a.groups, a.I, a.J);
     void* parts = nullptr;
     const bool split = a.sg.rows > (1ll << ts);
-    if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
-    Sum* cp = (Sum*)parts + spans * a.I * a.J;
+    const int64_t places = sum_places(a, ts);
+    if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)places * size * sizeof(Sum), &parts));
+    Sum* cp = (Sum*)parts + places * a.I * a.J;
     const dim3 grid = transform_grid(spans * ti * tj, 64 * WI * WJ), block(64 * WI * WJ);
     // (through registers the rows are rowmap's, or lie as they are summed: transform_sort knows the strides)
     const bool together = !a.rowmap && !transform_far(std::max(a.lda, a.ldb));
@@ -652,8 +653,9 @@ static int launch_sum_deep(lnasr_ctx* ctx, SumArgs a, const char* name) {
                    a.groups, a.I, a.J);
         void* parts = nullptr;
         const bool split = a.sg.rows > (1ll << ts);
-        if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * 4, &parts));
-        float* cp = (float*)parts + spans * a.I * a.J;
+        const int64_t places = sum_places(a, ts);
+        if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)places * size * 4, &parts));
+        float* cp = (float*)parts + places * a.I * a.J;
         if (pass) LN_LAUNCH(ctx, "sum_cols", (sum_cols<T>), transform_grid(spans * tiles, 256), dim3(256), 0, a, (unsigned)tiles, ts, cp);
         else LN_LAUNCH(ctx, name, (sum_deep<T>), transform_grid(spans * tiles, 512), dim3(512), 0, a, (unsigned)ti, (unsigned)tj, ts, (float*)parts);
         if (split) LN_TRY(join_t<T>(ctx, a, ts, parts, cp));

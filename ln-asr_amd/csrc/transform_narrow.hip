@@ -269,9 +269,9 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
     char* bs = as + (a_bytes + 15) / 16 * 16;
     const int64_t t = die_order(block_id(), block_count());
     int g, n;
-    int64_t q0;
+    int64_t q0, place;
     bool whole;
-    if (!sum_span(a, t, ts, &g, &q0, &n, &whole)) return;
+    if (!sum_span(a, t, ts, &g, &q0, &n, &whole, &place)) return;
 
     typename M::Acc acc[IF][JF];
 #pragma unroll
@@ -388,13 +388,13 @@ __global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void su
     for (int e = threadIdx.x; e < I * J; e += 256) {
         const Sum v = sum[e / J * W + e % J];
         if (whole) ((T*)a.out)[(int64_t)g * I * J + e] = (T)v;
-        else parts[t * I * J + e] = v;
+        else parts[place * I * J + e] = v;
     }
     if (a.cols)
         for (int i = threadIdx.x; i < I; i += 256) {
             const Sum v = sum[i * W + J];
             if (whole) ((T*)a.cols)[(int64_t)g * I + i] = (T)v;
-            else col_parts[t * I + i] = v;
+            else col_parts[place * I + i] = v;
         }
 }
 
@@ -413,8 +413,9 @@ static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name)
     LN_REQUIRE(spans < (1ll << 31), "%lld rows in %d groups are too many for one call", (long long)a.sg.rows, a.groups);
     void* parts = nullptr;
     const bool split = a.sg.rows > (1ll << ts);
-    if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)spans * size * sizeof(Sum), &parts));
-    Sum* cp = (Sum*)parts + spans * a.I * a.J;
+    const int64_t places = sum_places(a, ts);
+    if (split) LN_TRY(transform_ws(ctx, kTrPart, (size_t)places * size * sizeof(Sum), &parts));
+    Sum* cp = (Sum*)parts + places * a.I * a.J;
     const int wave_lds = (R * a.I * SZ + 15) / 16 * 16 + (R * a.J * SZ + 15) / 16 * 16;
     const int lds = std::max(4 * wave_lds, 16 * IF * 16 * JF * (int)sizeof(Sum));
     LN_LAUNCH(ctx, name, (sum_narrow<T, IF, JF, HA, HB>), transform_grid(spans, 256), dim3(256), lds, a, ts, (Sum*)parts, cp, wave_lds);
