@@ -755,8 +755,10 @@ static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         // 2048 x 2048 1185 / 634 / 496; 16,384 x 1024 x 1024 65 / 47 / 36), as long as there is one for every CU.  32 and 64 bits
         // have time for that: 64 x 64 leaves the least over at the ends (f32 120,011 x 351 x 128 105 against 142 us, f64 16,384 x
         // 1024 x 1024 609 against 640; f32 65,536 x 1024 x 1024 1169 against 1165).
+        // Tiles of one segment's rows want segments about as long: 256 of 192 rows x 2048 -> 2048 1002 / 620 / 556, 512 of 96 1125 / 763 /
+        // 866, 4096 of 8 4369 / 4288 / 6198.
         if constexpr (sizeof(T) == 2) {
-            if (rows / 256 * (a.N / 256) >= cus) return launch_deep<T, KN, LOW>(ctx, a, name);
+            if (rows / 256 * (a.N / 256) >= cus && (LOW || rows / a.sg.S >= 192)) return launch_deep<T, KN, LOW>(ctx, a, name);
             if ((rows / 128 + a.sg.S / 2) * ((a.N + 127) / 128) >= 2 * cus) return launch_tile<T, 128, 128, 2, 2, KN, LOW>(ctx, a, name);
         }
     }
@@ -767,8 +769,14 @@ template <typename T, bool KN>
 static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int64_t cus = ctx->prop.multiProcessorCount, rows = a.sg.rows, mean = rows / a.sg.S;
     if (a.w_stride) {
-        if (mean <= 16) return launch_few<T, KN, 1, 0>(ctx, a, name);
-        if (mean <= 32) return launch_few<T, KN, 2, 0>(ctx, a, name);
+        // Short segments, as long as the blocks of 16 x 16 find room on the CUs; past that each block's pass over x and W by itself
+        // costs more than the tiles' empty rows, all the more where the mean hides a long segment.  us, few / tile (S segments of the
+        // mean): bf16 512 -> 256, 64 of 1 12.0 / 12.0, 256 of 1 23 / 13; 2048 -> 2048, 1024 of 1 1498 / 1067; f64 351 -> 128, 64 of 1
+        // 11.7 / 17.4, 256 of 1 25 / 40, 512 of 8 54 / 51; f32 512 -> 512, 64 of 24 33 / 30; bf16 1024 -> 1024, 10,000 of 1 and one of
+        // 100,000 8500 / 2930.
+        const int64_t blocks = (rows / 16 + a.sg.S) * ((a.N + 15) / 16);
+        if (mean <= 16 && blocks <= (sizeof(T) == 2 ? 4 : 12) * cus) return launch_few<T, KN, 1, 0>(ctx, a, name);
+        if (mean <= 32 && blocks <= 4 * cus) return launch_few<T, KN, 2, 0>(ctx, a, name);
         return rows_t<T, KN, 0>(ctx, a, name);
     }
     // up to two blocks of 64 x 16 for every CU; lower ones where that leaves CUs without (64 rows x 2048: 23.1 us with 64 rows a block,
