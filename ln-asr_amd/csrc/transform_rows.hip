@@ -198,8 +198,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 //   k strided (w [k, n]): lines of k (spread, strided_fragment)
 // The first `full` steps go by LDS-DMA, the rest -- a last step that ends inside a piece -- through registers.
 // LOW: 0 tiles are spans of one segment, with its matrix.  One matrix for all rows, tiles of rows that lie together, and the
-// adapters of the segments that a tile meets join in: 1 through LDS, a step for each; 2 straight from memory (add_adapters), for
-// segments shorter than a tile.
+// adapters of the segments that a tile meets join in: 1 through LDS, a step for each; 2 straight from memory (add_adapters): rows_kn.
 // f32 and f64 are bound by the matrix cores, and by the uneven last turn of the CUs: f32 120,011 x 351 x 128 with adapters of rank 8
 // 122 us, 88 TFLOP/s of the 153 of a large library product; 20,011 x 512 x 429 100 us, cores busy 59 % of the time.  With few results
 // they wait for memory: f32 200,003 x 351 x 40 95 us, 3.3 TB/s (rows of 351 values begin off any alignment: 352 take a fifth less).
@@ -747,7 +746,10 @@ static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
             return launch_tile<T, 64, 64, 2, 2, KN, LOW, Mid<T>>(ctx, a, name);
         }
     }
-    if constexpr (LOW != 2) {
+    // (16-bit adapters from memory: short segments, whose time the adapters are)
+    if constexpr (LOW != 2 || sizeof(T) != 2) {
+        // few results: us, 64 x 64 / as wide as they are: f32 200,003 x 351 -> 8 99 / 57, -> 24 98 / 72, -> 48 104 / 90; f64 60,001 x
+        // 351 -> 16 50 / 29; bf16 200,003 x 512 -> 16 38 / 32, -> 48 39 / 39
         if (a.N <= 16) return launch_tile<T, 64, 16, 4, 1, KN, LOW>(ctx, a, name);
         if (a.N <= 32) return launch_tile<T, 64, 32, 4, 1, KN, LOW>(ctx, a, name);
         if (a.N <= 48) return launch_tile<T, 64, 48, 4, 1, KN, LOW>(ctx, a, name);
@@ -787,7 +789,12 @@ static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         if (rows <= 32 || (rows + 63) / 64 * wide < cus) return launch_few<T, KN, 2, 2>(ctx, a, name);
         return launch_few<T, KN, 4, 2>(ctx, a, name);
     }
-    if (mean >= 64) return rows_t<T, KN, 1>(ctx, a, name);
+    // Adapters through LDS or straight from memory: us, f16 16,384 x 1024 -> 2048, rank 32, segments of 16 rows 221 / 245, of 32 161 /
+    // 204, of 512 100 / 160; bf16 16,384 x 1024 -> 1024, rank 16, of 16 125 / 99, of 32 91 / 87, of 64 72 / 80; f32 120,011 x 351 -> 128,
+    // rank 8, of 16 272 / 247, of 128 155 / 146, of 512 147 / 142, rank 64, of 64 232 / 228; f64 20,011 x 351 -> 128, rank 16, of 32 81 /
+    // 77, of 512 61 / 59.
+    if constexpr (sizeof(T) == 2)
+        if (mean >= 32) return rows_t<T, KN, 1>(ctx, a, name);
     return rows_t<T, KN, 2>(ctx, a, name);
 }
 
