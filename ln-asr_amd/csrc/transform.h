@@ -346,7 +346,7 @@ int transform_join(lnasr_ctx* ctx, const SumArgs& a, int dtype, int ts, const vo
 inline bool transform_far(int64_t ld) { return ld * 128 >= (1ll << 31); }
 // Sorts the segments by group (stable): group_off, ord, place, rowmap of a.  Without slots the rows are sorted as they lie.
 // ld: the largest row stride of what will be summed.
-int transform_sort(lnasr_ctx* ctx, int dtype, int64_t ld, SumArgs* a);
+int transform_sort(lnasr_ctx* ctx, int64_t ld, SumArgs* a);
 
 // Workspace `i` of the feature transforms with room for `bytes`
 int transform_ws(lnasr_ctx* ctx, int i, size_t bytes, void** out);

@@ -266,7 +266,7 @@ int lnasr_affine_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows, in
         a.sg = sg;
         a.group_step = 1;
         a.groups = G;
-        LN_TRY(transform_sort(ctx, dtype, std::max(ldx, lddy), &a));
+        LN_TRY(transform_sort(ctx, std::max(ldx, lddy), &a));
         a.a = d_dy;
         a.lda = lddy;
         a.I = dout;
@@ -430,7 +430,7 @@ int lnasr_projection_grad(lnasr_ctx* ctx, int dtype, const void* x, int64_t rows
     if (d_da || d_db) {
         t.group_step = 1;
         t.groups = G;
-        if (S > 0) LN_TRY(transform_sort(ctx, dtype, std::max(ldx, lddy), &t));
+        if (S > 0) LN_TRY(transform_sort(ctx, std::max(ldx, lddy), &t));
     }
     if (d_da) {
         t.a = dp;

@@ -123,10 +123,12 @@ __global__ __launch_bounds__(256) void map_rows(Segments sg, const int* ord, con
     rowmap[q] = row < sg.rows ? row : sg.rows - 1;
 }
 
-// Segments long enough for their rows to be taken run by run: four steps of 128 bytes' worth of rows
-static bool rows_together(const Segments& sg, int dtype) { return sg.rows / sg.S >= 4 * 128 / (int64_t)transform_size(dtype); }
+// Segments long enough for their rows to be taken run by run.  us, run by run / row by row, segments of 32, 64 and 128 rows: bf16
+// 32,768 x 2048 x 1024 660 / 584, 426 / 636, 345 / 679; 16,384 x 512 x 512 105 / 98, 82 / 96, 69 / 92; f32 20,011 x 512 x 429 236 /
+// 210, 188 / 210, 150 / 208; f64 20,011 x 128 x 351 92 / 104, 80 / 94, 72 / 107.
+static bool rows_together(const Segments& sg) { return sg.rows / sg.S >= 64; }
 
-int transform_sort(lnasr_ctx* ctx, int dtype, int64_t ld, SumArgs* a) {
+int transform_sort(lnasr_ctx* ctx, int64_t ld, SumArgs* a) {
     const Segments& sg = a->sg;
     a->rowmap = a->place = nullptr;
     a->ord = nullptr;
@@ -141,7 +143,7 @@ int transform_sort(lnasr_ctx* ctx, int dtype, int64_t ld, SumArgs* a) {
     int64_t* goff = place + sg.S + 1;
     int* ord0 = (int*)(goff + sg.G + 1);
     a->group_off = goff;
-    const bool mapped = sg.rows > 0 && (!rows_together(sg, dtype) || transform_far(ld));
+    const bool mapped = sg.rows > 0 && (!rows_together(sg) || transform_far(ld));
     if (mapped) a->rowmap = map;
     a->place = place;
     a->ord = ord0;
@@ -677,12 +679,18 @@ static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
             return launch_sum<T, 64, 64, 2, 2, T, Mid<T>>(ctx, a, name);
         }
     }
+    // few results on one side: us, 64 x 64 / as narrow as they are: bf16 16,384 x 16 x 1024 26 / 23, f32 20,011 x 16 x 429 33 / 25,
+    // x 32 33 / 30, f64 20,011 x 16 x 351 42 / 28, x 32 44 / 37
     if (a.I <= 16) return launch_sum<T, 16, 128, 1, 4>(ctx, a, name);
     if (a.J <= 16) return launch_sum<T, 128, 16, 4, 1>(ctx, a, name);
     if (a.I <= 32) return launch_sum<T, 32, 128, 1, 4>(ctx, a, name);
     if (a.J <= 32) return launch_sum<T, 128, 32, 4, 1>(ctx, a, name);
     if constexpr (sizeof(T) == 2) {
-        if ((int64_t)(a.I / 256) * (a.J / 256) * std::max<int64_t>(a.groups, a.sg.rows >> 11) >= 128 && (!a.place || a.sg.rows / a.sg.S >= 512) &&
+        // 256 x 256 for enough of them with 2048 rows each, from segments long enough for its steps of 64 (us, 64 x 64 / 128 x 128 /
+        // 256 x 256; 32,768 x 2048 x 1024 in 1 group 359 / 268 / 146, in 16 323 / 272 / 164, in 64 528 / 418 / 309; 8192 x 1024 x 1024
+        // in 16 66 / 61 / 70; 32,768 x 512 x 512 in 1 56 / 57 / 50, in 64 65 / 53 / 78; sorted segments of 128, 256 and 512 rows - / 341
+        // / 364, - / 312 / 293, - / 253 / 207).
+        if ((int64_t)(a.I / 256) * (a.J / 256) * (a.sg.rows >> 11) >= 128 && (!a.place || a.sg.rows / a.sg.S >= 256) &&
             !transform_far(std::max(a.lda, a.ldb)))
             return launch_sum_deep<T>(ctx, a, name);
         if (a.I > 64 && a.J > 64) return launch_sum<T, 128, 128, 2, 2>(ctx, a, name);

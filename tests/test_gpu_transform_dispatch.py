@@ -67,3 +67,20 @@ def test_a_long_segment_costs_what_it_costs_alone(ctx):
     ratio = best(many, w, slots=slots) / best(one, w)
     print("ratio %.1f" % ratio)
     assert ratio < 10
+
+
+@pytest.mark.parametrize("size,slots", [((33000, 520, 1030, 30, 9, 8), True), ((33000, 1030, 520, 120, 9, 8), True), ((33000, 513, 1024, 90, 90, 8), False)],
+                         ids=str)
+def test_largest_sums(ctx, size, slots):
+    """256 x 256 sums over sorted segments, over segments as they lie, over the batch as one: groups without rows, uneven edges, short
+    last steps."""
+    d = ref.make(75, size, slots=slots)
+    d = {k: v if v is None or k in ("offsets", "slots", "scale") else v.astype(np.float16) for k, v in d.items()}
+    got = ctx.affine_grad(d["x"], d["offsets"], d["w3"], d["dy"], d["slots"], want=("w", "bias"))
+    want, err = ref.affine_grad("float16", d["x"], d["offsets"], d["w3"], d["dy"], d["slots"], d["dx0"])
+    for k in got:
+        ref.check(got[k], want[k], err[k], "affine_grad " + k)
+    got = ctx.projection_grad(d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"], want=("w", "bias", "a"))
+    want, err = ref.projection_grad("float16", d["x"], d["offsets"], d["w"], d["a"], d["b"], d["dy"], d["scale"], d["slots"], d["dx0"])
+    for k in got:
+        ref.check(got[k], want[k], err[k], "projection_grad " + k)
