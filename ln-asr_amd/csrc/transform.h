@@ -335,8 +335,8 @@ __device__ __forceinline__ void each_run(const SumArgs& a, int64_t q, int64_t en
 }
 
 int transform_sum(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);
-// transform_narrow.hip: the same for contiguous rows of up to 64 values
-bool rows_narrow_ok(const RowsArgs& a);
+// transform_narrow.hip: the same for contiguous rows of a few dozen values of `size` bytes
+bool rows_narrow_ok(const RowsArgs& a, int size);
 int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name);
 bool sum_narrow_ok(const SumArgs& a);
 int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name);

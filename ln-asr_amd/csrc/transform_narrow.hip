@@ -1,5 +1,4 @@
-// Feature transforms of up to 64 values a row: MFCC frames (39), spliced and reduced features (40), their gradients.  Such a
-// product is bound by the memory it moves (39 x 39 in fp64: 5 operations a byte), so rows are read and written as the contiguous
+// Feature transforms of a few dozen values a row: MFCC frames (39) and the like, their gradients.  Such a product is bound by the memory it moves (39 x 39 in fp64: 5 operations a byte), so rows are read and written as the contiguous
 // bytes they are, whatever their width, and the matrix stays in registers.
 #include <algorithm>
 #include <type_traits>
@@ -79,7 +78,7 @@ __device__ __forceinline__ void put_chunk(char* to, const char* lds, int bytes) 
 // latencies of memory.
 // ------------------------------------------------------------------------------------------
 template <typename T, int NF, int HF>
-__global__ __launch_bounds__(256, NF * HF <= 15 ? 3 : 1) void rows_narrow(RowsArgs a, int ts, int wave_lds) {
+__global__ __launch_bounds__(256, 3) void rows_narrow(RowsArgs a, int ts, int wave_lds) {
     using M = Mat<T>;
     using Sum = typename M::Sum;
     constexpr int SZ = (int)sizeof(T), E = M::E, HO = (16 * 16 * NF * SZ + 1023) / 1024;
@@ -215,29 +214,31 @@ static int launch_narrow(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 template <typename T, int HF>
 static int narrow_n(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     if (a.N <= 16) return launch_narrow<T, 1, HF>(ctx, a, name);
-    if (a.N <= 48) return launch_narrow<T, 3, HF>(ctx, a, name);
-    return launch_narrow<T, 4, HF>(ctx, a, name);
+    if constexpr (sizeof(T) == 2)
+        if (a.N > 48) return launch_narrow<T, 4, HF>(ctx, a, name);
+    return launch_narrow<T, 3, HF>(ctx, a, name);
 }
+
+// bytes of a row (and the one behind it that meets the bias) that fragments hold
+constexpr int narrow_row(int size) { return size == 8 ? 320 : size == 4 ? 192 : 128; }
 
 template <typename T>
 static int narrow_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
     const int bytes = (a.K + (a.bias ? 1 : 0)) * (int)sizeof(T);
-    if constexpr (sizeof(T) == 8) {
-        if (bytes <= 128) return narrow_n<T, 2>(ctx, a, name);
-        if (bytes <= 320) return narrow_n<T, 5>(ctx, a, name);
-        return narrow_n<T, 8>(ctx, a, name);
-    } else if constexpr (sizeof(T) == 4) {
-        if (bytes <= 64) return narrow_n<T, 1>(ctx, a, name);
-        if (bytes <= 192) return narrow_n<T, 3>(ctx, a, name);
-        return narrow_n<T, 4>(ctx, a, name);
-    } else {
-        if (bytes <= 64) return narrow_n<T, 1>(ctx, a, name);
-        return narrow_n<T, 2>(ctx, a, name);
-    }
+    constexpr int HF = narrow_row((int)sizeof(T)) / 64, LOW = sizeof(T) == 8 ? 2 : 1;
+    return bytes <= 64 * LOW ? narrow_n<T, LOW>(ctx, a, name) : narrow_n<T, HF>(ctx, a, name);
 }
 
-bool rows_narrow_ok(const RowsArgs& a) {
-    return a.w_stride && a.K + (a.bias ? 1 : 0) <= 64 && a.N <= 64 && a.ldx == a.K && a.ldy == a.N;
+// Up to 40 fp64, 48 fp32 or 64 16-bit values, and as many results (fp64: 48); but not rows of whole 128 bytes, which begin in the same
+// banks of the LDS, nor, where W is read across its lines (y = W x) in fewer bits than 64, of whole 32 bytes: the tiles then have
+// aligned pieces.  us, tiles / this, 300,007 rows: y with a bias, fp64 39 -> 39 50 / 48, 32 -> 32 30 / 53, 41 -> 41 56 / 73, 51 -> 51 73 /
+// 116; fp32 39 -> 39 40 / 36, 40 -> 40 39 / 48, 48 -> 48 39 / 55, 51 -> 51 51 / 54; bf16 39 -> 39 40 / 31, 48 -> 48 36 / 53, 51 -> 51 62 / 45,
+// 56 -> 56 44 / 44; dx, fp64 40 -> 40 50 / 42, 32 -> 32 29 / 47; fp32 32 -> 32 20 / 32, 48 -> 48 37 / 28; bf16 48 -> 48 29 / 24, 51 -> 51
+// 58 / 34, 64 -> 64 28 / 32.
+bool rows_narrow_ok(const RowsArgs& a, int size) {
+    const int row = a.K * size, whole = a.kn || size == 8 ? 128 : 32;
+    return a.w_stride && (a.K + (a.bias ? 1 : 0)) * size <= narrow_row(size) && a.N <= (size == 2 ? 64 : 48) && a.ldx == a.K && a.ldy == a.N &&
+           (row % whole != 0 || row <= 32);
 }
 
 int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name) {
@@ -250,14 +251,14 @@ int transform_rows_narrow(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const ch
 }
 
 // ------------------------------------------------------------------------------------------
-// out = sum over the rows of a span of a[r]^T b[r], up to 64 x 64: each of the four waves sums its own chunks of R rows (the k of
+// out = sum over the rows of a span of a[r]^T b[r], up to 48 x 48: each of the four waves sums its own chunks of R rows (the k of
 // one matrix instruction's piece, or two), whole, and the block adds the four at the end.  The column sums of a come with the
 // product: b has a column of ones behind its last.  Rows of two segments, and a span's last ones, come ahead as whole chunks do:
 // looked up one by one when their turn came, each such chunk held its block up (fp64 300,007 x 39 x 39 in 300 segments 77 us, so
 // 60).  187 MB take 36 us at a large copy's rate; the rest is the blocks' start and end, eight to sixteen chunks a wave.
 // ------------------------------------------------------------------------------------------
 template <typename T, int IF, int JF, int HA, int HB>
-__global__ __launch_bounds__(256, sizeof(T) < 8 || IF * JF <= 9 ? 2 : 1) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts,
+__global__ __launch_bounds__(256, 2) void sum_narrow(SumArgs a, int ts, typename Mat<T>::Sum* parts,
                                                                                     typename Mat<T>::Sum* col_parts, int wave_lds) {
     using M = Mat<T>;
     using Sum = typename M::Sum;
@@ -426,17 +427,14 @@ static int launch_sum_narrow(lnasr_ctx* ctx, const SumArgs& a, const char* name)
 template <typename T>
 static int sum_narrow_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     const int j = a.J + (a.cols ? 1 : 0);              // columns of b, and the ones
-    if (a.I <= 16) return j <= 48 ? launch_sum_narrow<T, 1, 3>(ctx, a, name) : launch_sum_narrow<T, 1, 4>(ctx, a, name);
-    if (a.I <= 48) {
-        if (j <= 16) return launch_sum_narrow<T, 3, 1>(ctx, a, name);
-        return j <= 48 ? launch_sum_narrow<T, 3, 3>(ctx, a, name) : launch_sum_narrow<T, 3, 4>(ctx, a, name);
-    }
-    if (j <= 16) return launch_sum_narrow<T, 4, 1>(ctx, a, name);
-    return j <= 48 ? launch_sum_narrow<T, 4, 3>(ctx, a, name) : launch_sum_narrow<T, 4, 4>(ctx, a, name);
+    if (a.I <= 16) return launch_sum_narrow<T, 1, 3>(ctx, a, name);
+    return j <= 16 ? launch_sum_narrow<T, 3, 1>(ctx, a, name) : launch_sum_narrow<T, 3, 3>(ctx, a, name);
 }
 
+// us, tiles / this, 300,007 rows in 300 segments of 64 groups: fp64 39 x 39 83 / 67, 48 x 48 82 / 70, 49 x 49 87 / 133; fp32 39 x 39 58 / 46,
+// 49 x 49 58 / 62; bf16 39 x 39 36 / 32, 32 x 32 27 / 31, 49 x 49 37 / 62
 bool sum_narrow_ok(const SumArgs& a) {
-    return a.I <= 64 && a.J + (a.cols ? 1 : 0) <= 64 && a.lda == a.I && a.ldb == a.J;
+    return a.I <= 48 && a.J + (a.cols ? 1 : 0) <= 48 && a.lda == a.I && a.ldb == a.J;
 }
 
 int transform_sum_narrow(lnasr_ctx* ctx, int dtype, const SumArgs& a, const char* name) {

@@ -805,7 +805,8 @@ static int rows_any(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
 
 int transform_rows(lnasr_ctx* ctx, int dtype, const RowsArgs& a, const char* name) {
     if (a.sg.rows == 0 || a.sg.S == 0 || a.N == 0) return 0;
-    if (rows_narrow_ok(a) && !(a.mid && transform_size(dtype) == 2)) return transform_rows_narrow(ctx, dtype, a, name);
+    const int size = (int)transform_size(dtype);
+    if (rows_narrow_ok(a, size) && !(a.mid && size == 2)) return transform_rows_narrow(ctx, dtype, a, name);
     switch (dtype) {
         case LNASR_F64: return rows_any<double>(ctx, a, name);
         case LNASR_F32: return rows_any<float>(ctx, a, name);
