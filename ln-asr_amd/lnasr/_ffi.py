@@ -336,7 +336,8 @@ class _Arg:
                     raise LnasrError("%s must be contiguous" % name)
         else:
             if out:
-                if not isinstance(x, np.ndarray) or not x.flags.c_contiguous or not x.flags.writeable:
+                # (another byte order has the same name)
+                if not isinstance(x, np.ndarray) or not x.flags.c_contiguous or not x.flags.writeable or not x.dtype.isnative:
                     raise LnasrError("%s must be a writable C-contiguous numpy array, a DeviceArray or a tensor" % name)
             else:
                 x = np.asarray(x)

@@ -31,3 +31,14 @@ def test_a_tensor_that_requires_a_gradient_is_refused_where_that_is_recorded(mon
     monkeypatch.setattr(_Tensor, "requires_grad", False)
     on.is_grad_enabled = lambda: True
     assert arg().kind == "float32"
+
+
+def test_an_output_of_another_byte_order_is_refused():
+    """Its type has the same name, but results written there would be other numbers; an input is converted."""
+    from lnasr import _ffi
+    other = np.dtype(np.float64).newbyteorder()
+    assert other.name == "float64"
+    with pytest.raises(_ffi.LnasrError, match="writable"):
+        _ffi._Arg(_Ctx, np.zeros((2, 3), other), "out", 2, out=True)
+    a = _ffi._Arg(_Ctx, np.ones((2, 3), other), "x", 2)
+    assert a.obj.dtype.isnative and a.obj.sum() == 6
