@@ -51,7 +51,7 @@ class Recognizer:
         d_pcm = ctx.to_device(data)
         _, _, feat, _ = ctx.mfcc(d_pcm, np.array([0, len(data)], dtype=np.int64), cfg, win, bank, False, False)
         if self.transforms is not None:
-            feat = self.transforms.apply(feat, np.array([0, feat.shape[0]], dtype=np.int64), np.array([speaker], dtype=np.int32))
+            feat = self.transforms.apply(feat, np.array([0, feat.shape[0]], dtype=np.int64), np.array([speaker]))
         return gh.decode(feat)
 
     def recognize_batch(self, utterances, speakers=None):
@@ -68,7 +68,7 @@ class Recognizer:
         d_pcm = ctx.to_device(np.concatenate(utterances).astype(dt))
         _, _, feat, rows = ctx.mfcc(d_pcm, offsets, cfg, win, bank, False, False)
         if self.transforms is not None:
-            speakers = np.zeros(len(utterances), dtype=np.int32) if speakers is None else np.asarray(speakers, dtype=np.int32)
+            speakers = np.zeros(len(utterances), dtype=np.int32) if speakers is None else np.asarray(speakers)
             feat = self.transforms.apply(feat, rows, speakers)
         obs, lens = ctx.pad_rows(feat, rows)
         gh.upload()
