@@ -138,7 +138,8 @@ int segments(Call& c, const int64_t* offsets, const int32_t* slots, int S, int G
     LN_REQUIRE(S >= 0 && G >= 0 && rows >= 0, "negative size: %d segments, %d groups, %lld rows", S, G, (long long)rows);
     LN_REQUIRE(rows < (1ll << 40), "%lld rows", (long long)rows);
     LN_REQUIRE(S == 0 || offsets, "offsets is null");
-    LN_REQUIRE(slots || S == G, "%d segments of %d groups: without slots there is one segment for each group", S, G);
+    // (no segments: an empty array of slots may well be a null pointer)
+    LN_REQUIRE(slots || S == G || S == 0, "%d segments of %d groups: without slots there is one segment for each group", S, G);
     *covered = rows == 0;
     *sg = Segments{nullptr, nullptr, S, G, rows};
     if (S == 0) return 0;

@@ -97,3 +97,20 @@ def test_narrow_rows_of_every_fragment_width(ctx, kind, K):
         ref.check(y, *ref.affine(kind, d["x"], d["offsets"], d["w3"], d["bias2"], d["slots"], d["y0"]), "y")
         y = ctx.affine(d["x"], d["offsets"], d["w3"], None, d["slots"], out=d["y0"].copy())
         ref.check(y, *ref.affine(kind, d["x"], d["offsets"], d["w3"], None, d["slots"], d["y0"]), "y without bias")
+
+
+def test_no_segments_and_a_null_pointer_for_their_slots(ctx):
+    """An empty tensor of slots has no memory: a batch without segments is one all the same."""
+    from lnasr import _ffi
+    l = _ffi.lib()
+    x, dy, w, a, b = (ctx.to_device(np.ones(s)) for s in ((6, 5), (6, 4), (3, 4, 5), (3, 2, 5), (3, 4, 2)))
+    off, y = ctx.to_device(np.zeros(1, dtype=np.int64)), ctx.to_device(np.full((6, 4), 7.0))
+    dw, db = ctx.to_device(np.full((3, 4, 5), np.nan)), ctx.to_device(np.full((3, 4), np.nan))
+    _ffi.check(l.lnasr_affine(ctx.handle, 0, x.ptr, 6, 5, 5, off.ptr, None, 0, w.ptr, None, 3, 4, y.ptr, 4))
+    _ffi.check(l.lnasr_affine_grad(ctx.handle, 0, x.ptr, 6, 5, 5, off.ptr, None, 0, w.ptr, 3, 4, dy.ptr, 4, None, 0, dw.ptr, db.ptr))
+    assert (y.to_host() == 7.0).all() and not dw.to_host().any() and not db.to_host().any()
+    da, d2 = ctx.to_device(np.full((3, 2, 5), np.nan)), ctx.to_device(np.full((3, 4, 2), np.nan))
+    _ffi.check(l.lnasr_projection(ctx.handle, 0, x.ptr, 6, 5, 5, off.ptr, None, 0, w.ptr, None, 4, a.ptr, b.ptr, None, 3, 2, y.ptr, 4))
+    _ffi.check(l.lnasr_projection_grad(ctx.handle, 0, x.ptr, 6, 5, 5, off.ptr, None, 0, w.ptr, 4, a.ptr, b.ptr, None, 3, 2, dy.ptr, 4,
+                                       None, 0, da.ptr, d2.ptr, None, None))
+    assert (y.to_host() == 7.0).all() and not da.to_host().any() and not d2.to_host().any()
