@@ -434,6 +434,8 @@ class Context:
         such a call."""
         if stream is not None and not isinstance(stream, int):
             stream = stream.cuda_stream
+        if stream is not None and stream == self._stream and stream == getattr(self._choice, "stream", None):
+            return                    # (where this thread's calls go already)
         with self._order:
             self._go(stream)
             self._choice.stream = stream
@@ -953,12 +955,17 @@ class Context:
     # -- feature transforms ------------------------------------------------------------------------
     # (lnasr/transform.py has what the arguments mean)
     def _call(self, fn, arrays, *args):
+        loose = tensors = False
+        for a in arrays:
+            if a is not None:
+                loose = loose or a.loose
+                tensors = tensors or a.tensor
         with self._order:
-            loose = any(a.loose for a in arrays if a)
-            if any(a.tensor for a in arrays if a):
+            if tensors:
                 stream = getattr(self._choice, "stream", None)
                 if stream is not None:
-                    self._go(stream)
+                    if stream != self._stream:
+                        self._go(stream)
                 elif not loose:       # (a thread of the library's own may call while another captures: it cannot wait)
                     rc = lib().lnasr_ctx_capturing(self.handle)
                     if rc < 0:
