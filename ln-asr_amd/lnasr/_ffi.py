@@ -373,8 +373,8 @@ class _Arg:
 
 
 def _need(arg, name, shape):
-    if tuple(arg.shape) != tuple(shape):
-        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(arg.shape)))
+    if arg.shape != shape:                      # (both tuples)
+        raise ValueError("%s must have shape %s, got %s" % (name, shape, arg.shape))
 
 
 class Context:
