@@ -182,7 +182,7 @@ __device__ __forceinline__ int64_t longest_span(const SumArgs& a, int spans, int
 // bits or more per span, which join_parts adds in the order of the spans.
 // A: the type of a, B: of b; where they differ (the gradients of adapters) both are multiplied in the wider one, C.
 // f32 20,011 rows x 512 x 429: 98 us, 90 TFLOP/s of the 153 of a large library product (CUs busy 72 % of the time: 1120 blocks on
-// 1280 places).  bf16 16,384 rows x 16 x 1024: 11.6 us, 34 MB.
+// 1280 places).  bf16 16,384 rows x 16 x 1024, the 16 in f32: 14.8 us, 35 MB (all of it in bf16: 11.6).
 // ------------------------------------------------------------------------------------------
 template <typename A, typename B>
 using Wider = std::conditional_t<(sizeof(A) >= sizeof(B)), A, B>;
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(512, 2) void sum_deep(SumArgs a, unsigned tiles_i, 
 }
 
 // Column sums of a beside sum_deep: cols[k, i] = sum of a[r, i], a span and 512 columns a block, eight of them a thread; the rows of the
-// span go to the four waves in turn, which meet in LDS.  bf16 32,768 x 2048: 28 us, 4.8 TB/s.  (Summed beside the products instead, by
+// span go to the four waves in turn, which meet in LDS.  bf16 32,768 x 2048: 25 us, 5.3 TB/s.  (Summed beside the products instead, by
 // matrix instructions or from LDS, it has no registers left.)
 template <typename T>
 __global__ __launch_bounds__(256) void sum_cols(SumArgs a, unsigned tiles, int ts, float* col_parts) {
@@ -668,6 +668,7 @@ static int launch_sum_deep(lnasr_ctx* ctx, SumArgs a, const char* name) {
 template <typename T>
 static int sum_t(lnasr_ctx* ctx, const SumArgs& a, const char* name) {
     if constexpr (!std::is_same<T, Mid<T>>::value) {
+        // (32-bit instructions: tiles of 128 x 128 have nothing to save)
         if (a.mid_a) {
             if (a.I <= 16) return launch_sum<T, 16, 128, 1, 4, Mid<T>, T>(ctx, a, name);
             if (a.I <= 32) return launch_sum<T, 32, 128, 1, 4, Mid<T>, T>(ctx, a, name);

@@ -121,8 +121,8 @@ __device__ __forceinline__ void put_tile(const RowsArgs& a, int64_t row0, int64_
 // ------------------------------------------------------------------------------------------
 // A few rows: 16 MR rows x 16 results a block, its eight waves divide k between them.  Bound by the latency of memory and, with many
 // groups, by the matrices read once: fragments go from memory to registers, many at a time, and meet in LDS at the end.
-// bf16 64 single rows x 2048 -> 2048, 48 adapters of rank 16: 5.5 us for the middle and 12 for the rest, 15 MB; through the
-// tiles below 120.
+// bf16 64 single rows x 2048 -> 2048, 48 adapters of rank 16: 5.5 us for the middle and 12 for the rest, 15 MB, a pass 19; through
+// the tiles below a pass takes 45.
 // ------------------------------------------------------------------------------------------
 template <typename T, typename Y, bool KN, int MR, int LOW>
 __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, int ts) {
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(512) void rows_few(RowsArgs a, unsigned tiles_n, in
 // LOW: 0 tiles are spans of one segment, with its matrix.  One matrix for all rows, tiles of rows that lie together, and the
 // adapters of the segments that a tile meets join in: 1 through LDS, a step for each; 2 straight from memory (add_adapters): rows_kn.
 // f32 and f64 are bound by the matrix cores, and by the uneven last turn of the CUs: f32 120,011 x 351 x 128 with adapters of rank 8
-// 122 us, 88 TFLOP/s of the 153 of a large library product; 20,011 x 512 x 429 100 us, cores busy 59 % of the time.  With few results
+// 122 us, 88 TFLOP/s of the 153 of a large library product; 20,011 x 512 x 429 95 us, cores busy 59 % of the time.  With few results
 // they wait for memory: f32 200,003 x 351 x 40 95 us, 3.3 TB/s (rows of 351 values begin off any alignment: 352 take a fifth less).
 // ------------------------------------------------------------------------------------------
 template <typename T, typename Y, int TM, int TN, int WM, int WN, bool KN, int LOW>
@@ -428,8 +428,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows_tile(RowsArgs a, unsigne
 // step after next and x of the one behind it are asked for in the middle of each step, where its own buffers fall free: the matrix
 // cores, the LDS and the memory each work ahead of one another, with one barrier a step and a wait that counts (the newest four
 // requests, x of the step after next, may be out).
-// bf16 65,536 x 2048 x 2048 in 32 equal groups: 496 us, 1110 TFLOP/s (a library's product of 8192^3: 1273); in ragged ones 515-550,
-// 8.5 turns of the CUs taking nine.  16,384 x 1024 x 1024: 36 us, 950; with adapters of rank 16 44, a step each through registers.
+// bf16 65,536 x 2048 x 2048 in 32 equal groups: 500-520 us, 1060-1100 TFLOP/s (a library's product of 8192^3: 1270-1310); in ragged
+// ones 515-535, 8.5 turns of the CUs taking nine.  16,384 x 1024 x 1024: 36 us, 960; with adapters of rank 16 47, a step each through
+// registers and 32-bit instructions, of a sixteenth of the rate.
 // ------------------------------------------------------------------------------------------
 // Up to 64 segments, a lane each: the tiles of 256 rows numbered without gaps (find_span leaves some), so that the dies get equally
 // many: 16,384 x 1024 x 1024 of one group 55 -> 36 us.  (All whole tiles before the segments' last ones, for a shorter last turn of
