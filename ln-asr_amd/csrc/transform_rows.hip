@@ -782,13 +782,17 @@ static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         if (mean <= 32 && blocks <= 4 * cus) return launch_few<T, KN, 2, 0>(ctx, a, name);
         return rows_t<T, KN, 0>(ctx, a, name);
     }
-    // up to two blocks of 64 x 16 for every CU; lower ones where that leaves CUs without (64 rows x 2048: 23.1 us with 64 rows a block,
-    // 15.4 with 32, 15.6 with 16)
+    // Up to two blocks of 64 x 16 for every CU; lower ones where that leaves CUs without, and for 64 bits, whose 64 rows find no
+    // registers.  us, tiles / 16 / 32 / 64 rows a block, adapters of rank 16 or 8: bf16 2048 -> 2048, 64 single rows 45 / 20.0 / 19.4 / 26.5,
+    // 256 53 / 52 / 42 / 47, 512 59 / 94 / 73 / 84; segments of 64 rows, 128 rows 27 / 30 / 26 / 24, 256 33 / 45 / 37 / 35; f32 1024 -> 1024,
+    // 256 rows 36 / 32 / 28 / 26; 351 -> 128, 64 single rows 48 / 16.8 / 17.2 / 21.5, 4096 78 / 68 / 62 / 66; f64 351 -> 128, 1000 rows 31 /
+    // 18.1 / 18.2 / 21.5.
     if (rows * a.N <= 64 * 16 * 2 * cus) {
         const int64_t wide = (a.N + 15) / 16;
         if (rows <= 16 || (rows + 31) / 32 * wide < cus / 2) return launch_few<T, KN, 1, 2>(ctx, a, name);
-        if (rows <= 32 || (rows + 63) / 64 * wide < cus) return launch_few<T, KN, 2, 2>(ctx, a, name);
-        return launch_few<T, KN, 4, 2>(ctx, a, name);
+        if constexpr (sizeof(T) < 8)
+            if (rows > 32 && (rows + 63) / 64 * wide >= cus) return launch_few<T, KN, 4, 2>(ctx, a, name);
+        return launch_few<T, KN, 2, 2>(ctx, a, name);
     }
     // Adapters through LDS or straight from memory: us, f16 16,384 x 1024 -> 2048, rank 32, segments of 16 rows 221 / 245, of 32 161 /
     // 204, of 512 100 / 160; bf16 16,384 x 1024 -> 1024, rank 16, of 16 125 / 99, of 32 91 / 87, of 64 72 / 80; f32 120,011 x 351 -> 128,
