@@ -776,9 +776,12 @@ static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         // costs more than the tiles' empty rows, all the more where the mean hides a long segment.  us, few / tile (S segments of the
         // mean): bf16 512 -> 256, 64 of 1 12.0 / 12.0, 256 of 1 23 / 13; 2048 -> 2048, 1024 of 1 1498 / 1067; f64 351 -> 128, 64 of 1
         // 11.7 / 17.4, 256 of 1 25 / 40, 512 of 8 54 / 51; f32 512 -> 512, 64 of 24 33 / 30; bf16 1024 -> 1024, 10,000 of 1 and one of
-        // 100,000 8500 / 2930.
+        // 100,000 8500 / 2930.  With few results of many values in 32 or 64 bits x alone counts, and k is divided: f64 2048 -> 16, 16,384
+        // of 1 612 / 963, 2048 of 8 118 / 182; 351 -> 8, 4096 of 1 42 / 57; f32 2048 -> 16, 2048 of 8 68 / 89, of 24 149 / 117; 351 -> 8,
+        // 16,384 of 1 135 / 125.
         const int64_t blocks = (rows / 16 + a.sg.S) * ((a.N + 15) / 16);
-        if (mean <= 16 && blocks <= (sizeof(T) == 2 ? 4 : 12) * cus) return launch_few<T, KN, 1, 0>(ctx, a, name);
+        const bool thin = sizeof(T) != 2 && a.N <= 32 && a.K * (int64_t)sizeof(T) >= 2048 && mean <= 12;
+        if (mean <= 16 && (thin || blocks <= (sizeof(T) == 2 ? 4 : 12) * cus)) return launch_few<T, KN, 1, 0>(ctx, a, name);
         if (mean <= 32 && blocks <= 4 * cus) return launch_few<T, KN, 2, 0>(ctx, a, name);
         return rows_t<T, KN, 0>(ctx, a, name);
     }
