@@ -759,13 +759,27 @@ static int rows_t(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         // have time for that: 64 x 64 leaves the least over at the ends (f32 120,011 x 351 x 128 105 against 142 us, f64 16,384 x
         // 1024 x 1024 609 against 640; f32 65,536 x 1024 x 1024 1169 against 1165).
         // Tiles of one segment's rows want segments about as long: 256 of 192 rows x 2048 -> 2048 1002 / 620 / 556, 512 of 96 1125 / 763 /
-        // 866, 4096 of 8 4369 / 4288 / 6198.
+        // 866, 1024 of 32 1184 / 1134 / 1581; 4096 of 4 x 1024 -> 256 231 / 268 / -, x 1000 -> 64 67 / 138 / -.
         if constexpr (sizeof(T) == 2) {
             if (rows / 256 * (a.N / 256) >= cus && (LOW || rows / a.sg.S >= 192)) return launch_deep<T, KN, LOW>(ctx, a, name);
-            if ((rows / 128 + a.sg.S / 2) * ((a.N + 127) / 128) >= 2 * cus) return launch_tile<T, 128, 128, 2, 2, KN, LOW>(ctx, a, name);
+            if (a.N > 64 && (LOW || rows / a.sg.S >= 32) && (rows / 128 + a.sg.S / 2) * ((a.N + 127) / 128) >= 2 * cus) return launch_tile<T, 128, 128, 2, 2, KN, LOW>(ctx, a, name);
         }
     }
     return launch_tile<T, 64, 64, 2, 2, KN, LOW>(ctx, a, name);
+}
+
+// The mean rows of a segment up to which rows_few, which divides k, is faster than the tiles at any number of segments; 0: at none.
+// us, few / tile: f64 2048 -> 16, 4096 of 2 rows 167 / 266, 1024 of 12 74 / 100; 1024 -> 256, 4096 of 4 1513 / 1847, 1024 of 12 506 / 498
+// (dx 403 / 532); 351 -> 40, 4096 of 4 137 / 146; 351 -> 128, 2048 of 8 204 / 191.  f32 2048 -> 16, 1024 of 12 44 / 53; 1024 -> 256, 8192 of 1
+// 1742 / 1903, 4096 of 4 943 / 958, 1024 of 12 310 / 273; 512 -> 64, 4096 of 2 145 / 139; 351 -> 8, 8192 of 1 66 / 68.  bf16 2048 -> 8, 8192 of
+// 1 83 / 98, 4096 of 4 49 / 55, 1024 of 12 21 / 19; -> 16, 8192 of 1 103 / 98; dx 15 <- 1823, 8192 of 1 114 / 205, 1024 of 12 33 / 46; 16 <-
+// 2048, 8192 of 1 104 / 98.
+template <typename T, bool KN>
+static int few_mean(const RowsArgs& a) {
+    const int64_t line = a.K * (int64_t)sizeof(T);
+    if (sizeof(T) == 2) return a.K < 1024 ? 0 : KN ? (a.N <= 16 && a.N % 8 ? 12 : 0) : a.N <= 8 ? 4 : 0;
+    if (a.N <= 32) return line >= 2048 ? 12 : 0;
+    return line >= 4000 ? (sizeof(T) == 8 ? 12 : 4) : sizeof(T) == 8 && line >= 2048 ? 4 : 0;
 }
 
 template <typename T, bool KN>
@@ -776,12 +790,9 @@ static int rows_kn(lnasr_ctx* ctx, const RowsArgs& a, const char* name) {
         // costs more than the tiles' empty rows, all the more where the mean hides a long segment.  us, few / tile (S segments of the
         // mean): bf16 512 -> 256, 64 of 1 12.0 / 12.0, 256 of 1 23 / 13; 2048 -> 2048, 1024 of 1 1498 / 1067; f64 351 -> 128, 64 of 1
         // 11.7 / 17.4, 256 of 1 25 / 40, 512 of 8 54 / 51; f32 512 -> 512, 64 of 24 33 / 30; bf16 1024 -> 1024, 10,000 of 1 and one of
-        // 100,000 8500 / 2930.  With few results of many values in 32 or 64 bits x alone counts, and k is divided: f64 2048 -> 16, 16,384
-        // of 1 612 / 963, 2048 of 8 118 / 182; 351 -> 8, 4096 of 1 42 / 57; f32 2048 -> 16, 2048 of 8 68 / 89, of 24 149 / 117; 351 -> 8,
-        // 16,384 of 1 135 / 125.
+        // 100,000 8500 / 2930.
         const int64_t blocks = (rows / 16 + a.sg.S) * ((a.N + 15) / 16);
-        const bool thin = sizeof(T) != 2 && a.N <= 32 && a.K * (int64_t)sizeof(T) >= 2048 && mean <= 12;
-        if (mean <= 16 && (thin || blocks <= (sizeof(T) == 2 ? 4 : 12) * cus)) return launch_few<T, KN, 1, 0>(ctx, a, name);
+        if (mean <= 16 && (mean <= few_mean<T, KN>(a) || blocks <= (sizeof(T) == 2 ? 4 : 12) * cus)) return launch_few<T, KN, 1, 0>(ctx, a, name);
         if (mean <= 32 && blocks <= 4 * cus) return launch_few<T, KN, 2, 0>(ctx, a, name);
         return rows_t<T, KN, 0>(ctx, a, name);
     }
